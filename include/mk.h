@@ -412,6 +412,95 @@ int mk_allreduce_add_rmsnorm(const uint64_t* peers, int32_t rank, int32_t world,
  * in the reference (its kernel has no software ring). */
 int mk_schedule_gap(const MkConfig* cfg, int32_t batch, int32_t grid, int32_t* gap);
 
+/* ---- Speculative decoding over a paged cache, bf16 or 8-bit -----------------
+ *
+ * The reference decodes one token per step over a bf16 cache
+ * (nki_kernels/attention.py:77-492) and takes the argmax of the logits
+ * (llama.py:1208-1227); these operators verify several drafted tokens of a
+ * sequence in one pass, over a cache of half the bytes where wanted, and score
+ * them. All are asynchronous on `stream`; device-side failures set *error
+ * (device, zeroed by the caller) to the code named at each entry point, and
+ * nothing outside the caller's buffers is read or written.
+ *
+ * One layer of a paged cache. MK_KV_BF16: k_pages / v_pages as in MkKVCache,
+ * scales NULL. MK_KV_E4M3: pages hold e4m3 codes and k_scales / v_scales one
+ * E8M0 byte per row: dim d of a row is code_d * 2^(byte - 127), byte 255 a row
+ * of NaN. page_size a multiple of 8; pools 16-byte aligned. */
+#define MK_KV_BF16 0
+#define MK_KV_E4M3 1
+typedef struct MkKVLayer {
+  void* k_pages;               /* [num_pages][num_kv_heads][page_size][64] */
+  void* v_pages;
+  void* k_scales;              /* [num_pages][num_kv_heads][page_size] */
+  void* v_scales;
+  const int32_t* block_tables; /* [batch][max_blocks] */
+  int32_t format;
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t num_kv_heads;
+  int32_t max_blocks;
+} MkKVLayer;
+
+/* Rotate and store new rows: qkv [rows][(nq + 2 nkv) * 64] bf16 in the packed
+ * RoPE-pair order (mk_rope_scatter's). Row r is rotated for positions[r] (rows of
+ * the bf16 tables [rope_len][64]), its q goes to q_out [rows][nq][64] bf16 and its
+ * K/V to place slots[r] of sequence seqs[r] (slots of a tree's siblings differ
+ * where their positions do not); slot -1 is a padding row, whose K/V is not
+ * stored. Rotation in fp32, each stored value rounded once. An 8-bit row takes
+ * the scale 2^e, e the smallest exponent >= -110 with max|x| <= 448 * 2^e; a row
+ * with a non-finite value is stored as NaN. *error = 1: a sequence, slot,
+ * position or page id out of range; that row is not stored. */
+int mk_kv_write(const MkKVLayer* kv, int32_t batch, const void* qkv, const void* rope_cos,
+                const void* rope_sin, int32_t rope_len, const int32_t* seqs, const int32_t* slots,
+                const int32_t* positions, int32_t rows, int32_t num_q_heads, void* q_out,
+                int32_t* error, void* stream);
+
+/* Read rows back: positions [0, lengths[b]) of every sequence as bf16 into
+ * k_out / v_out [batch][nkv][max_len][64], zeros behind them (a length above
+ * max_len counts as max_len). Exact but for values below bf16's smallest.
+ * *error = 1: a page id out of range; that row reads as zeros. */
+int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32_t max_len,
+               void* k_out, void* v_out, int32_t* error, void* stream);
+
+/* Attention of drafted nodes: sequence b has prefix_lens[b] committed positions
+ * and the nodes cu_nodes[b] .. cu_nodes[b + 1] - 1 (cu_nodes [batch + 1]), whose
+ * K/V rows are already at its positions prefix_lens[b] + 0, 1, ...; q
+ * [rows][num_q_heads][64] bf16 (rotated) holds all nodes. A node attends every
+ * committed position and the nodes j of its sequence whose bit j % 64 of
+ * mask[node][j / 64] is set (mask [rows][ceil(max_nodes / 64)], bits past the
+ * sequence's nodes ignored). out [rows][num_q_heads][64] bf16 = softmax(scale
+ * q K^T) V; lse [rows][num_q_heads] fp32 (may be NULL) the log of the
+ * normaliser. A node that attends nothing gets out 0, lse -inf; what masked
+ * places and the pages behind the last node hold has no effect on a row. A
+ * row that attends a node whose K or V is not finite is not finite.
+ * num_q_heads is 1, 2, 4 or 8 times num_kv_heads; max_nodes (1..256) and max_len
+ * bound every sequence's nodes and prefix + nodes. One node per sequence with
+ * its own bit is a plain decode step. *error = 1: lengths or node ranges beyond
+ * the bounds (that sequence is not computed) or a page id out of range (its
+ * positions are skipped); 2: a device-side wait ran out (2 s). */
+int64_t mk_tree_attention_workspace(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                    int32_t max_nodes, int32_t max_len);
+int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_nodes,
+                      const uint64_t* mask, const int32_t* prefix_lens, int32_t batch, int32_t rows,
+                      int32_t max_nodes, int32_t max_len, int32_t num_q_heads, float scale,
+                      void* workspace, int64_t workspace_bytes, void* out, float* lse,
+                      int32_t* error, void* stream);
+
+/* Log probabilities from logits [rows][ld] (the first `vocab` columns; dtype
+ * MK_F32 or MK_BF16): logprobs [rows][num_targets] of targets (int32; negative:
+ * no token, 0 is written), entropy [rows] in nats, and the `top` (0..32) most
+ * likely ids with their log probabilities, ties to the lower id. Logits of -inf
+ * are forbidden tokens. A row of nothing else has log probabilities -inf and
+ * entropy 0; one with a NaN or +inf has NaN for both. *error = 1: a target
+ * >= vocab (its log probability is NaN). */
+#define MK_F32 0
+#define MK_BF16 1
+int64_t mk_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top);
+int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t ld,
+                      const int32_t* targets, int32_t num_targets, int32_t top, void* workspace,
+                      int64_t workspace_bytes, float* logprobs, float* entropy, int32_t* top_ids,
+                      float* top_logprobs, int32_t* error, void* stream);
+
 /* Last error message of the calling thread ("" if none). */
 const char* mk_last_error(void);
 

@@ -14,6 +14,8 @@ LIB_PATH = _HERE / "libmk.so"
 
 MK_OK, MK_EINVAL, MK_ECUDA, MK_ETIMEOUT, MK_ENOMEM, MK_ESTATE, MK_EDEVICE = range(7)
 MK_FLAG_FEEDBACK = 1
+MK_KV_BF16, MK_KV_E4M3 = 0, 1
+MK_F32, MK_BF16 = 0, 1
 
 STATUS_NAMES = {
     MK_OK: "MK_OK", MK_EINVAL: "MK_EINVAL", MK_ECUDA: "MK_ECUDA", MK_ETIMEOUT: "MK_ETIMEOUT",
@@ -29,7 +31,8 @@ EXPORTED = (
     "mk_paged_attention", "mk_gemm_workspace", "mk_gemm_bf16", "mk_rmsnorm_rows", "mk_rope_scatter", "mk_swiglu", "mk_argmax_rows",
     "mk_add_rmsnorm_rows", "mk_argmax_keys", "mk_keys_to_ids", "mk_tp_setup", "mk_tp_connect",
     "mk_xbuf_bytes", "mk_xbuf_alloc", "mk_xbuf_open", "mk_xbuf_close", "mk_xbuf_free", "mk_step_epoch",
-    "mk_allreduce_add_rmsnorm", "mk_last_error",
+    "mk_allreduce_add_rmsnorm", "mk_kv_write", "mk_kv_read", "mk_tree_attention_workspace",
+    "mk_tree_attention", "mk_token_logprobs_workspace", "mk_token_logprobs", "mk_last_error",
     "mk_destroy",
 )
 
@@ -67,6 +70,14 @@ class MkSampling(ctypes.Structure):
 
 class MkIpcHandle(ctypes.Structure):
     _fields_ = [("bytes", ctypes.c_ubyte * 64)]
+
+
+class MkKVLayer(ctypes.Structure):
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+                ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("block_tables", ctypes.c_void_p), ("format", ctypes.c_int32),
+                ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("num_kv_heads", ctypes.c_int32), ("max_blocks", ctypes.c_int32)]
 
 
 class MkKVCache(ctypes.Structure):
@@ -129,12 +140,23 @@ def load() -> ctypes.CDLL:
     lib.mk_step_epoch.argtypes = [VP, VP]
     lib.mk_allreduce_add_rmsnorm.argtypes = [VP, I32, I32, I32, I32, VP, VP, VP, ctypes.c_float,
                                              I32, I32, VP, VP, ctypes.c_uint64, VP]
+    lib.mk_kv_write.argtypes = [P(MkKVLayer), I32, VP, VP, VP, I32, VP, VP, VP, I32, I32, VP, VP, VP]
+    lib.mk_kv_read.argtypes = [P(MkKVLayer), VP, I32, I32, VP, VP, VP, VP]
+    lib.mk_tree_attention_workspace.argtypes = [I32, I32, I32, I32, I32]
+    lib.mk_tree_attention_workspace.restype = ctypes.c_int64
+    lib.mk_tree_attention.argtypes = [VP, P(MkKVLayer), VP, VP, VP, I32, I32, I32, I32, I32,
+                                      ctypes.c_float, VP, ctypes.c_int64, VP, VP, VP, VP]
+    lib.mk_token_logprobs_workspace.argtypes = [I32, I32, I32]
+    lib.mk_token_logprobs_workspace.restype = ctypes.c_int64
+    lib.mk_token_logprobs.argtypes = [VP, I32, I32, I32, ctypes.c_int64, VP, I32, I32, VP,
+                                      ctypes.c_int64, VP, VP, VP, VP, VP, VP]
     lib.mk_last_error.argtypes = []
     lib.mk_last_error.restype = ctypes.c_char_p
     lib.mk_destroy.argtypes = [VP]
     for name in EXPORTED:
         if name not in ("mk_last_error", "mk_paged_attention_workspace", "mk_gemm_workspace",
-                        "mk_xbuf_bytes"):
+                        "mk_xbuf_bytes", "mk_tree_attention_workspace",
+                        "mk_token_logprobs_workspace"):
             getattr(lib, name).restype = ctypes.c_int
     _lib = lib
     return lib

@@ -17,7 +17,7 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
-SOURCES = [HERE / "csrc" / "mk_api.cu"]
+SOURCES = [HERE / "csrc" / "mk_api.cu", HERE / "csrc" / "mk_spec.cu"]
 DEPS = SOURCES + sorted((HERE / "csrc").glob("*.cuh")) + [ROOT / "include" / "mk.h"]
 OUT = HERE / "libmk.so"
 
@@ -25,7 +25,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-shared",
-    "-Xptxas", "-v",
+    "-Xptxas", "-v", "--threads", "0",  # the sources compile in parallel
 ]
 
 

@@ -8,45 +8,25 @@
 
 #include <algorithm>
 #include <array>
-#include <cstdarg>
 #include <cstdint>
-#include <cstdio>
 #include <cstring>
 #include <mutex>
 #include <string>
 #include <vector>
 
 #include "../../include/mk.h"
+#include "mk_host.cuh"
 #include "mk_kernel.cuh"
 #include "mk_sample.cuh"
 #include "mk_attn.cuh"
 #include "mk_batched.cuh"
 #include "mk_gemm.cuh"
 
+using namespace mk::host;
+
 namespace {
 
-thread_local std::string g_last_error;
-
 constexpr uint64_t kPartTagLimit = 0xFFFFFFFFull;  // attention partial tags stay below this
-
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return code;
-}
-
-#define MK_CUDA(call)                                                                    \
-  do {                                                                                   \
-    cudaError_t e_ = (call);                                                             \
-    if (e_ != cudaSuccess) return fail(MK_ECUDA, "%s: %s", #call, cudaGetErrorString(e_)); \
-  } while (0)
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
 
@@ -407,54 +387,8 @@ int static_setup(int device, void** out) {
 }  // namespace
 
 namespace {
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// A 2-D bf16 tensor map [rows][cols] (cols contiguous), box {64 cols, box_rows},
-// 128-byte swizzle: the K-major operand layout of the tcgen05 GEMM.
-int encode_sw128(CUtensorMap* out, const void* base, long long rows, long long cols, int box_rows) {
-  static EncodeTiledFn enc = nullptr;
-  if (!enc) {
-    cudaDriverEntryPointQueryResult q;
-    void* fn = nullptr;
-    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn)
-      return fail(MK_ECUDA, "cuTensorMapEncodeTiled unavailable");
-    enc = reinterpret_cast<EncodeTiledFn>(fn);
-  }
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-  cuuint32_t box[2] = {(cuuint32_t)mk::kGemmTileK, (cuuint32_t)box_rows};
-  cuuint32_t es[2] = {1, 1};
-  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides,
-                   box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(MK_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return MK_OK;
-}
-
 // K blocks per split for an n x k GEMM: narrow W is split along K so the
 // grid covers the SMs.
-// Launch with programmatic stream serialization: the kernel (which calls
-// pdl_trigger / pdl_wait) may start while the previous one in the stream ends.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                       cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 constexpr int kGemmMaxCluster = 8;  // portable thread-block cluster size
 int gemm_kblocks_per_split(int n, int k, int sms) {
   const int tiles = (n + mk::kGemmTileN - 1) / mk::kGemmTileN, kblocks = k / mk::kGemmTileK;
@@ -538,11 +472,6 @@ int attn_split_len(int batch, int num_kv_heads, int max_len, int sms, int fixed_
     if (len == 128) break;
   }
   return best < 128 ? 128 : best;
-}
-int device_sms() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
 }
 }  // namespace
 

@@ -1,0 +1,186 @@
+// mk_spec.cu — C ABI (include/mk.h) of the speculative-decoding operators:
+// cache rows written and read back (mk_kv8.cuh), attention of drafted tokens
+// (mk_tree.cuh), log probabilities of tokens (mk_logprobs.cuh).
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/mk.h"
+#include "mk_host.cuh"
+#include "mk_kv8.cuh"
+#include "mk_logprobs.cuh"
+#include "mk_tree.cuh"
+
+using namespace mk::host;
+
+namespace {
+
+int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
+  if (!kv || !kv->k_pages || !kv->v_pages || !kv->block_tables) return fail(MK_EINVAL, "NULL argument");
+  if (kv->format != MK_KV_BF16 && kv->format != MK_KV_E4M3) return fail(MK_EINVAL, "cache format %d", kv->format);
+  if (kv->format == MK_KV_E4M3 && (!kv->k_scales || !kv->v_scales))
+    return fail(MK_EINVAL, "an 8-bit cache needs k_scales and v_scales");
+  if (kv->page_size < 8 || kv->page_size % 8 || kv->num_pages < 1 || kv->num_kv_heads < 1 ||
+      kv->num_kv_heads > 65535 || kv->max_blocks < 1 ||
+      (long long)kv->page_size * kv->max_blocks > 0x7fffffffLL)
+    return fail(MK_EINVAL, "cache geometry (page_size %d, num_pages %d, num_kv_heads %d, max_blocks %d)",
+                kv->page_size, kv->num_pages, kv->num_kv_heads, kv->max_blocks);
+  if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages) || !aligned16(kv->k_scales) || !aligned16(kv->v_scales))
+    return fail(MK_EINVAL, "the page pools must be 16-byte aligned");
+  if (batch < 1 || batch > 65535) return fail(MK_EINVAL, "batch %d outside [1, 65535]", batch);
+  out->k = static_cast<uint8_t*>(kv->k_pages);
+  out->v = static_cast<uint8_t*>(kv->v_pages);
+  out->k_scales = static_cast<uint8_t*>(kv->k_scales);
+  out->v_scales = static_cast<uint8_t*>(kv->v_scales);
+  out->block_tables = kv->block_tables;
+  out->ps = kv->page_size;
+  out->num_pages = kv->num_pages;
+  out->NKV = kv->num_kv_heads;
+  out->max_blocks = kv->max_blocks;
+  out->batch = batch;
+  return MK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mk_kv_write(const MkKVLayer* kv, int32_t batch, const void* qkv, const void* rope_cos,
+                const void* rope_sin, int32_t rope_len, const int32_t* seqs, const int32_t* slots,
+                const int32_t* positions, int32_t rows, int32_t num_q_heads, void* q_out,
+                int32_t* error, void* stream) {
+  mk::KVWriteParams p{};
+  if (int rc = check_layer(kv, batch, &p.kv)) return rc;
+  if (!qkv || !rope_cos || !rope_sin || !seqs || !slots || !positions || !q_out || !error)
+    return fail(MK_EINVAL, "NULL argument");
+  if (rows < 0 || num_q_heads < 1 || num_q_heads > 65535 || rope_len < 1)
+    return fail(MK_EINVAL, "rows %d, num_q_heads %d, rope_len %d", rows, num_q_heads, rope_len);
+  if (!aligned16(qkv) || !aligned16(rope_cos) || !aligned16(rope_sin) || !aligned16(q_out))
+    return fail(MK_EINVAL, "qkv, the RoPE tables and q_out must be 16-byte aligned");
+  if (rows == 0) return MK_OK;
+  p.qkv = static_cast<const uint8_t*>(qkv);
+  p.cos_t = static_cast<const __nv_bfloat16*>(rope_cos);
+  p.sin_t = static_cast<const __nv_bfloat16*>(rope_sin);
+  p.seqs = seqs;
+  p.slots = slots;
+  p.positions = positions;
+  p.rows = rows;
+  p.NQ = num_q_heads;
+  p.rope_len = rope_len;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.error = error;
+  const int64_t heads = (int64_t)rows * (num_q_heads + 2 * kv->num_kv_heads);
+  const int64_t ctas = (heads + 31) / 32;
+  if (ctas > 0x7fffffffLL) return fail(MK_EINVAL, "%d rows of %lld heads", rows, (long long)(heads / rows));
+  MK_CUDA(launch_pdl(kv->format == MK_KV_E4M3 ? mk::kv_write_kernel<true> : mk::kv_write_kernel<false>,
+                     dim3((unsigned)ctas), dim3(256), 0, static_cast<cudaStream_t>(stream), p));
+  return MK_OK;
+}
+
+int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32_t max_len,
+               void* k_out, void* v_out, int32_t* error, void* stream) {
+  mk::KVReadParams p{};
+  if (int rc = check_layer(kv, batch, &p.kv)) return rc;
+  if (!lengths || !k_out || !v_out || !error) return fail(MK_EINVAL, "NULL argument");
+  if (max_len < 0 || max_len > (long long)kv->page_size * kv->max_blocks)
+    return fail(MK_EINVAL, "max_len %d outside [0, page_size * max_blocks]", max_len);
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(MK_EINVAL, "k_out and v_out must be 16-byte aligned");
+  if (max_len == 0) return MK_OK;
+  p.lengths = lengths;
+  p.max_len = max_len;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.error = error;
+  MK_CUDA(launch_pdl(kv->format == MK_KV_E4M3 ? mk::kv_read_kernel<true> : mk::kv_read_kernel<false>,
+                     dim3((unsigned)(((int64_t)max_len * 8 + 255) / 256), kv->num_kv_heads, batch),
+                     dim3(256), 0, static_cast<cudaStream_t>(stream), p));
+  return MK_OK;
+}
+
+int64_t mk_tree_attention_workspace(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                    int32_t max_nodes, int32_t max_len) {
+  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_nodes < 1 || max_len < 1) return 0;
+  return 0;
+}
+
+int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_nodes,
+                      const uint64_t* mask, const int32_t* prefix_lens, int32_t batch, int32_t rows,
+                      int32_t max_nodes, int32_t max_len, int32_t num_q_heads, float scale,
+                      void* workspace, int64_t workspace_bytes, void* out, float* lse,
+                      int32_t* error, void* stream) {
+  mk::TreeParams p{};
+  if (int rc = check_layer(kv, batch, &p.kv)) return rc;
+  if (!q || !cu_nodes || !mask || !prefix_lens || !out || !error) return fail(MK_EINVAL, "NULL argument");
+  const int nkv = kv->num_kv_heads;
+  const int group = num_q_heads / nkv;
+  if (num_q_heads < 1 || num_q_heads % nkv || (group != 1 && group != 2 && group != 4 && group != 8))
+    return fail(MK_EINVAL, "num_q_heads %d must be 1, 2, 4 or 8 times num_kv_heads %d", num_q_heads, nkv);
+  if (max_nodes < 1 || max_nodes > mk::kTreeMaxNodes)
+    return fail(MK_EINVAL, "max_nodes %d outside [1, %d]", max_nodes, mk::kTreeMaxNodes);
+  if (rows < 0 || max_len < 1 || max_len > (long long)kv->page_size * kv->max_blocks)
+    return fail(MK_EINVAL, "rows %d, max_len %d (page_size %d, max_blocks %d)", rows, max_len, kv->page_size,
+                kv->max_blocks);
+  if (!aligned16(q) || !aligned16(out)) return fail(MK_EINVAL, "q and out must be 16-byte aligned");
+  const int64_t need = mk_tree_attention_workspace(batch, num_q_heads, nkv, max_nodes, max_len);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(MK_EINVAL, "workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
+  if (rows == 0) return MK_OK;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.cu_nodes = cu_nodes;
+  p.mask = reinterpret_cast<const unsigned long long*>(mask);
+  p.prefix = prefix_lens;
+  p.rows = rows;
+  p.words = (max_nodes + 63) / 64;
+  p.max_nodes = max_nodes;
+  p.max_len = max_len;
+  p.NQ = num_q_heads;
+  p.group = group;
+  p.scale = scale;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.error = error;
+  MK_CUDA(launch_pdl(kv->format == MK_KV_E4M3 ? mk::tree_attn_kernel<true> : mk::tree_attn_kernel<false>,
+                     dim3(max_nodes, nkv, batch), dim3(32 * group), 0, static_cast<cudaStream_t>(stream), p));
+  return MK_OK;
+}
+
+int64_t mk_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top) {
+  if (rows < 1 || vocab < 1 || top < 0 || top > mk::kLogprobsMaxTop) return 0;
+  return 0;
+}
+
+int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t ld,
+                      const int32_t* targets, int32_t num_targets, int32_t top, void* workspace,
+                      int64_t workspace_bytes, float* logprobs, float* entropy, int32_t* top_ids,
+                      float* top_logprobs, int32_t* error, void* stream) {
+  if (!logits || !entropy || !error) return fail(MK_EINVAL, "NULL argument");
+  if (dtype != MK_F32 && dtype != MK_BF16) return fail(MK_EINVAL, "logits type %d", dtype);
+  if (rows < 0 || vocab < 1 || ld < vocab) return fail(MK_EINVAL, "rows %d, vocab %d, ld %lld", rows, vocab, (long long)ld);
+  if (num_targets < 0 || (num_targets && (!targets || !logprobs)))
+    return fail(MK_EINVAL, "num_targets %d needs targets and logprobs", num_targets);
+  if (top < 0 || top > mk::kLogprobsMaxTop || top > vocab || (top && (!top_ids || !top_logprobs)))
+    return fail(MK_EINVAL, "top %d must be in [0, min(%d, vocab)] and needs top_ids and top_logprobs", top,
+                mk::kLogprobsMaxTop);
+  const int64_t need = mk_token_logprobs_workspace(rows, vocab, top);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(MK_EINVAL, "workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
+  if (rows == 0) return MK_OK;
+  mk::LogprobsParams p{};
+  p.logits = logits;
+  p.ld = ld;
+  p.rows = rows;
+  p.V = vocab;
+  p.num_targets = num_targets;
+  p.top = top;
+  p.targets = targets;
+  p.logprobs = logprobs;
+  p.entropy = entropy;
+  p.top_ids = top_ids;
+  p.top_logprobs = top_logprobs;
+  p.error = error;
+  MK_CUDA(launch_pdl(dtype == MK_F32 ? mk::logprobs_kernel<float> : mk::logprobs_kernel<__nv_bfloat16>, dim3(rows),
+                     dim3(256), 0, static_cast<cudaStream_t>(stream), p));
+  return MK_OK;
+}
+
+}  // extern "C"
