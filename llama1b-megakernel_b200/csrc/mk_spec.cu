@@ -41,6 +41,69 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
   return MK_OK;
 }
 
+// How the positions of a sequence are split over CTAs. Two CTAs fit an SM, so a
+// launch of n CTAs takes about ceil(n / (2 SMs)) waves of one range each; a
+// range costs its blocks and a fixed part (launch, first bytes, the store),
+// taken as kTreeFixedBlocks blocks, and joining the ranges kTreeJoinBlocks more.
+struct TreeSplit {
+  int splits, len;
+};
+constexpr int kTreeFixedBlocks = 3;
+constexpr int kTreeJoinBlocks = 2;
+TreeSplit tree_split(int batch, int num_kv_heads, int rows, int max_len) {
+  const int tiles = (rows + mk::kTreeRows - 1) / mk::kTreeRows;
+  const int blocks = (max_len + mk::kTreeBlock - 1) / mk::kTreeBlock;
+  const long long ctas = (long long)batch * num_kv_heads * tiles, slots = 2LL * device_sms();
+  TreeSplit best{1, blocks * mk::kTreeBlock};
+  long long best_cost = -1;
+  for (int per = blocks; per >= 1; --per) {
+    const int splits = (blocks + per - 1) / per;
+    const long long waves = (ctas * splits + slots - 1) / slots;
+    const long long cost = waves * (per + kTreeFixedBlocks) + (splits > 1 ? kTreeJoinBlocks : 0);
+    if (best_cost < 0 || cost < best_cost) {
+      best_cost = cost;
+      best = {splits, per * mk::kTreeBlock};
+    }
+  }
+  return best;
+}
+
+// A page pool as rows of 64 values, boxes of `box` whole rows: bf16 rows with the
+// 128-byte swizzle that the tensor cores read, codes with the 64-byte one.
+int encode_rows(CUtensorMap* out, const void* pool, long long rows, int box, bool fp8) {
+  if (!fp8) return encode_sw128(out, pool, rows, 64, box);
+  EncodeTiledFn enc = nullptr;
+  if (int rc = encode_tiled_fn(&enc)) return rc;
+  cuuint64_t dims[2] = {64, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {64};
+  cuuint32_t boxes[2] = {64, (cuuint32_t)box};
+  cuuint32_t es[2] = {1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pool), dims, strides, boxes, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MK_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return MK_OK;
+}
+
+// The kernel's shared-memory limit, once per device.
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && done[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev] = true;
+  return e;
+}
+
+template <bool kFp8>
+cudaError_t launch_tree(const mk::TreeTmaParams& tp, dim3 grid, cudaStream_t st) {
+  static bool done[64];
+  constexpr int smem = mk::TreeSmem<kFp8>::kBytes;
+  if (cudaError_t e = allow_smem(mk::tree_attn_kernel<kFp8>, smem, done)) return e;
+  return launch_pdl(mk::tree_attn_kernel<kFp8>, grid, dim3(mk::kTreeThreads), smem, st, tp);
+}
+
 }  // namespace
 
 extern "C" {
@@ -100,7 +163,10 @@ int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32
 int64_t mk_tree_attention_workspace(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                     int32_t max_nodes, int32_t max_len) {
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_nodes < 1 || max_len < 1) return 0;
-  return 0;
+  const int group = num_q_heads / num_kv_heads;
+  const TreeSplit sp = tree_split(batch, num_kv_heads, max_nodes * group, max_len);
+  if (sp.splits == 1) return 0;
+  return (int64_t)batch * num_kv_heads * sp.splits * max_nodes * group * mk::kTreePartial * 4;
 }
 
 int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_nodes,
@@ -108,7 +174,8 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
                       int32_t max_nodes, int32_t max_len, int32_t num_q_heads, float scale,
                       void* workspace, int64_t workspace_bytes, void* out, float* lse,
                       int32_t* error, void* stream) {
-  mk::TreeParams p{};
+  mk::TreeTmaParams tp{};
+  mk::TreeParams& p = tp.p;
   if (int rc = check_layer(kv, batch, &p.kv)) return rc;
   if (!q || !cu_nodes || !mask || !prefix_lens || !out || !error) return fail(MK_EINVAL, "NULL argument");
   const int nkv = kv->num_kv_heads;
@@ -120,7 +187,10 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   if (rows < 0 || max_len < 1 || max_len > (long long)kv->page_size * kv->max_blocks)
     return fail(MK_EINVAL, "rows %d, max_len %d (page_size %d, max_blocks %d)", rows, max_len, kv->page_size,
                 kv->max_blocks);
+  if (!(scale > 0.f) || !(scale < 3.0e38f)) return fail(MK_EINVAL, "scale %g must be positive and finite", (double)scale);
   if (!aligned16(q) || !aligned16(out)) return fail(MK_EINVAL, "q and out must be 16-byte aligned");
+  const long long pool_rows = (long long)kv->num_pages * nkv * kv->page_size;
+  if (pool_rows > 0x7fffffffLL) return fail(MK_EINVAL, "KV pool of %lld rows", pool_rows);
   const int64_t need = mk_tree_attention_workspace(batch, num_q_heads, nkv, max_nodes, max_len);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(MK_EINVAL, "workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
@@ -139,8 +209,21 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   p.error = error;
-  MK_CUDA(launch_pdl(kv->format == MK_KV_E4M3 ? mk::tree_attn_kernel<true> : mk::tree_attn_kernel<false>,
-                     dim3(max_nodes, nkv, batch), dim3(32 * group), 0, static_cast<cudaStream_t>(stream), p));
+  const TreeSplit sp = tree_split(batch, nkv, max_nodes * group, max_len);
+  p.tiles = (max_nodes * group + mk::kTreeRows - 1) / mk::kTreeRows;
+  p.splits = sp.splits;
+  p.split_len = sp.len;
+  p.work = static_cast<float*>(workspace);
+  p.box = 128;
+  while (kv->page_size % p.box) p.box /= 2;
+  const bool fp8 = kv->format == MK_KV_E4M3;
+  if (int rc = encode_rows(&tp.tm_k, kv->k_pages, pool_rows, p.box, fp8)) return rc;
+  if (int rc = encode_rows(&tp.tm_v, kv->v_pages, pool_rows, p.box, fp8)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(p.tiles * p.splits, nkv, batch);
+  MK_CUDA(fp8 ? launch_tree<true>(tp, grid, st) : launch_tree<false>(tp, grid, st));
+  if (p.splits > 1)
+    MK_CUDA(launch_pdl(mk::tree_merge_kernel, dim3((max_nodes * group + 7) / 8, nkv, batch), dim3(256), 0, st, p));
   return MK_OK;
 }
 

@@ -1,15 +1,39 @@
-// Attention of drafted tokens over a paged cache.
+// Attention of drafted tokens over a paged cache, on the tcgen05 tensor cores.
 //
 // Sequence b has prefix_b committed positions in its pages and, behind them, n_b
 // drafted nodes whose K/V rows sit at positions prefix_b + j. Node i sees every
 // committed position and those nodes j whose bit (i, j) is set (itself and its
 // ancestors in a tree; j <= i for a chunk of a prompt):
 //   s_j = scale q_i . k_j,  p_j = exp(s_j - m),  o = sum p_j v_j / sum p_j,
-//   lse = m + log sum p_j,  m = max_j s_j,
+//   lse = m + log sum p_j,  m >= max_j s_j - 8 log 2,
 // per query head, the sums in fp32. A row that sees nothing gets o = 0 and
 // lse = -inf.
+//
+// The query heads of a K/V head share its rows, so the nodes of a sequence and
+// those heads (row = node * group + head) are the rows of one matrix product, in
+// tiles of 128. A CTA takes a tile, a K/V head and a range of positions, 128 at a
+// time (a block):
+//  * a producer warp brings the block's K and V rows in by TMA (boxes of the
+//    largest power of two, at most 128, that divides the page size, so a box never
+//    leaves its page) into a ring of stages;
+//  * a warpgroup makes the block fit for the tensor cores. bf16: it only acts on
+//    blocks that reach past the committed positions: V rows behind the last node
+//    become zeros, and so do drafted V rows that hold an infinity or NaN (0 * inf
+//    in P V would reach rows that do not see them), which are noted in a bit mask.
+//    8-bit: it turns codes into bf16 rows of the value code * 2^e, exactly (see
+//    tree_decode), and treats the last block's V in the same way;
+//  * one thread issues S = Q K^T (M 128, N 128, 64 dims) and O += P V (N 64, 128
+//    positions) with P read from TMEM and V taken MN-major as it lies;
+//  * four warps do the softmax, one thread per row (TMEM lane): S from TMEM, the
+//    exponentials, P as bf16 pairs back to TMEM. O is only rescaled when a row's
+//    maximum has grown by more than 8 powers of two since it was last set:
+//    until then p is at most 256, which costs bf16 and fp32 nothing.
+// P is rounded to bf16 (relative 2^-8 at most, unbiased, as V is no more precise
+// itself); its sum is taken before the rounding. A range that is not the whole
+// sequence leaves (m, l, O) in the workspace for tree_merge_kernel.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
 
@@ -19,6 +43,25 @@
 namespace mk {
 
 constexpr int kTreeMaxNodes = 256;
+constexpr int kTreeRows = 128;     // rows of a tile (the MMA's M)
+constexpr int kTreeBlock = 128;    // positions of a block
+constexpr int kTreeThreads = 320;  // 4 softmax warps, 4 block warps, producer, issuer
+constexpr int kTreePartial = 66;   // m, l, o[64]
+constexpr uint32_t kTreeTmem = 256;  // columns: S 128, P 64, O 64
+constexpr uint32_t kTreeTileBytes = kTreeBlock * 128;  // a bf16 K or V block (and the Q tile)
+constexpr uint32_t kTreeRawBytes = kTreeBlock * 64;    // an 8-bit one
+
+template <bool kFp8>
+struct TreeSmem {
+  static constexpr int kStages = kFp8 ? 2 : 3;   // blocks in flight from memory
+  static constexpr int kReady = kFp8 ? 2 : 3;    // blocks ready for the tensor cores
+  static constexpr uint32_t kQ = 0;
+  static constexpr uint32_t kTiles = kTreeTileBytes;                        // kReady x (K, V) bf16
+  static constexpr uint32_t kRaw = kTiles + kReady * 2 * kTreeTileBytes;    // 8-bit: kStages x (K, V)
+  static constexpr uint32_t kScales = kRaw + (kFp8 ? kStages * 2 * kTreeRawBytes : 0);  // kStages x 256
+  static constexpr uint32_t kBars = kScales + (kFp8 ? kStages * 2 * kTreeBlock : 0);
+  static constexpr uint32_t kBytes = kBars + 256;
+};
 
 struct TreeParams {
   const __nv_bfloat16* q;           // [rows][NQ][64]
@@ -27,10 +70,19 @@ struct TreeParams {
   const unsigned long long* mask;   // [rows][words]
   const int* prefix;                // [batch]
   int rows, words, max_nodes, max_len, NQ, group;
+  int box;                          // rows of a TMA box
+  int tiles, splits, split_len;     // split_len: a multiple of kTreeBlock
   float scale;
+  float* work;                      // [batch][NKV][splits][max_nodes * group][kTreePartial]
   __nv_bfloat16* out;               // [rows][NQ][64]
   float* lse;                       // [rows][NQ] or null
   int* error;
+};
+
+struct alignas(64) TreeTmaParams {
+  CUtensorMap tm_k;  // the pool as rows of 64 values
+  CUtensorMap tm_v;
+  TreeParams p;
 };
 
 // The sequence's rows and lengths; false (and the error word) when they do not
@@ -47,74 +99,587 @@ __device__ __forceinline__ bool tree_sequence(const TreeParams& p, int b, int& r
   return true;
 }
 
-template <bool kFp8>
-__global__ void __launch_bounds__(256) tree_attn_kernel(const __grid_constant__ TreeParams p) {
-  pdl_trigger();
-  pdl_wait();
-  const KVLayer& kv = p.kv;
-  const int i = blockIdx.x, g = blockIdx.y, b = blockIdx.z, h = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int row0, nodes, prefix;
-  if (!tree_sequence(p, b, row0, nodes, prefix) || i >= nodes || h >= p.group) return;
-  const int row = row0 + i, head = g * p.group + h, end = prefix + nodes;
-  const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q + ((size_t)row * p.NQ + head) * 64);
-  auto value = [&](const uint8_t* pool, const uint8_t* scales, size_t r, int d2) {  // dims 2 d2, 2 d2 + 1
-    if (!kFp8) {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(pool)[r * 32 + d2];
-      return make_float2(bf_lo(w), bf_hi(w));
-    }
-    float2 f = e4m3x2_to_float2(reinterpret_cast<const uint16_t*>(pool)[r * 32 + d2]);
-    const float s = e8m0_value(scales[r]);
-    return make_float2(f.x * s, f.y * s);
-  };
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int c0 = 0; c0 < end; c0 += 32) {
-    const int pos = c0 + lane, j = pos - prefix;
-    bool seen = pos < end;
-    if (seen && j >= 0) seen = (p.mask[(size_t)row * p.words + (j >> 6)] >> (j & 63)) & 1;
-    int page = -1;
-    if (pos < end) {
-      page = kv.block_tables[(size_t)b * kv.max_blocks + pos / kv.ps];
-      if (page < 0 || page >= kv.num_pages) {
-        atomicExch(p.error, 1);
-        page = -1;
+// Wait with a limit of 2 s. A wait that runs out reports error 2 and raises the
+// CTA's abort word, on which every other wait of the CTA gives up.
+__device__ __noinline__ bool tree_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_word, int* error) {
+  const uint64_t t0 = global_ns();
+  for (uint32_t it = 0;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 15) == 15) {
+      if (*abort_word) return false;
+      if (global_ns() - t0 > 2000000000ull) {
+        *abort_word = 1;
+        atomicCAS(error, 0, 2);
+        return false;
       }
-    }
-    seen = seen && page >= 0;
-    const int64_t r = page >= 0 ? ((int64_t)page * kv.NKV + g) * kv.ps + pos % kv.ps : -1;
-    float s = -INFINITY;
-    if (seen) {
-      s = 0.f;
-      for (int d = 0; d < 32; ++d) {
-        const float2 k = value(kv.k, kv.k_scales, r, d);
-        const uint32_t w = q[d];
-        s = fmaf(bf_lo(w), k.x, fmaf(bf_hi(w), k.y, s));
-      }
-      s *= p.scale;
-    }
-    float cm = s;
-    for (int x = 16; x; x >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, x));
-    const float mn = fmaxf(m, cm);
-    // a maximum of -inf is taken as 0: exp(-inf) is 0 there, and a NaN score stays one
-    const float mu = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __expf(m - mu);
-    const float e = __expf(s - mu);
-    l = l * alpha + warp_sum(e);
-    m = mn;
-    o0 *= alpha;
-    o1 *= alpha;
-    for (int t = 0; t < 32; ++t) {
-      const float pt = __shfl_sync(0xffffffffu, e, t);
-      const int64_t rt = __shfl_sync(0xffffffffu, r, t);
-      if (!__shfl_sync(0xffffffffu, (int)seen, t)) continue;  // a masked row is not read at all
-      const float2 v = value(kv.v, kv.v_scales, rt, lane);
-      o0 = fmaf(pt, v.x, o0);
-      o1 = fmaf(pt, v.y, o1);
     }
   }
+}
+
+__device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_word, int* error) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok ? true : tree_wait_slow(bar, parity, abort_word, error);
+}
+
+__device__ __forceinline__ void tree_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tree_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// A 128-byte-swizzled operand of 128-byte rows, groups of 8 rows 1024 bytes apart:
+// K-major for Q and K (the rows are M or N), MN-major for V (the rows are K).
+__device__ __forceinline__ uint64_t tree_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// fp32 accumulator, bf16 operands, M 128, N n; trans_b: B is MN-major.
+__device__ __forceinline__ constexpr uint32_t tree_idesc(int n, bool trans_b) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((trans_b ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kTreeRows >> 4) << 24);
+}
+
+__device__ __forceinline__ void tree_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tree_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tree_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+__device__ __forceinline__ float tree_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Four e4m3 codes as bf16: {d0, d2} and {d1, d3}. A code s eeee mmm moved into
+// bf16's place for (exponent, mantissa) is its value times 2^(7 - 127), its
+// subnormals becoming bf16's, so one exact multiplication by 2^120 and the row's
+// scale (`f`, in both halves) gives the value.
+__device__ __forceinline__ uint2 tree_decode(uint32_t w, __nv_bfloat162 f) {
+  uint32_t a = ((w << 4) & 0x07F007F0u) | ((w << 8) & 0x80008000u);
+  uint32_t b = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);
+  __nv_bfloat162 x = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), f);
+  __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&b), f);
+  return make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
+}
+
+__device__ __forceinline__ __nv_bfloat162 tree_pow2(int biased) {  // 2^(biased - 127) twice
+  const uint32_t w = (uint32_t)biased << 7;
+  const uint32_t ww = w | (w << 16);
+  return *reinterpret_cast<const __nv_bfloat162*>(&ww);
+}
+
+__device__ __forceinline__ __nv_bfloat162 tree_nan2() {
+  const uint32_t w = 0x7FC07FC0u;
+  return *reinterpret_cast<const __nv_bfloat162*>(&w);
+}
+
+// 64 bits of row `mask` from bit j0 on (j0 may be negative: committed positions, all seen).
+__device__ __forceinline__ unsigned long long tree_bits(const unsigned long long* mask, int words, int nodes, int j0) {
+  auto word = [&](int w) -> unsigned long long {
+    if (w < 0) return ~0ull;
+    if (w >= words || 64 * w >= nodes) return 0;
+    const int left = nodes - 64 * w;
+    return mask[w] & (left >= 64 ? ~0ull : (1ull << left) - 1);
+  };
+  const int w = j0 >> 6, sh = j0 & 63;
+  const unsigned long long lo = word(w);
+  return sh ? (lo >> sh) | (word(w + 1) << (64 - sh)) : lo;
+}
+
+// Where a row's result goes: the output, or this split's partial.
+__device__ __forceinline__ void tree_store_row(const TreeParams& p, int row, int head, const float (&o)[64], float l,
+                                               float m2) {
   const bool any = l != 0.f;  // NaN counts as something
+  const float r = any ? 1.f / l : 0.f;
+  uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)row * p.NQ + head) * 64);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      __nv_bfloat162 h = __floats2bfloat162_rn(any ? o[8 * c + 2 * e] * r : 0.f, any ? o[8 * c + 2 * e + 1] * r : 0.f);
+      w[e] = *reinterpret_cast<uint32_t*>(&h);
+    }
+    dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (p.lse) p.lse[(size_t)row * p.NQ + head] = any ? m2 * 0.6931471805599453f + logf(l) : -INFINITY;
+}
+
+template <bool kFp8>
+__global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid_constant__ TreeTmaParams tp) {
+  using L = TreeSmem<kFp8>;
+  const TreeParams& p = tp.p;
+  const KVLayer& kv = p.kv;
+  pdl_trigger();
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, g = blockIdx.y, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
+  // barriers: full[3], empty[3], ready[3], free[3], q, s, pr, o; then words
+  const uint32_t bars = base + L::kBars;
+  auto full = [&](int i) { return bars + 8 * i; };
+  auto empty = [&](int i) { return bars + 24 + 8 * i; };
+  auto ready = [&](int i) { return bars + 48 + 8 * i; };
+  auto free_ = [&](int i) { return bars + 72 + 8 * i; };
+  const uint32_t b_q = bars + 96, b_s = bars + 104, b_p = bars + 112, b_o = bars + 120;
+  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 128);
+  volatile uint32_t* abort_word = words;      // words[1]: TMEM base
+  volatile uint32_t* bad = words + 4;         // [kReady][4] drafted positions whose V is not finite
+
+  pdl_wait();
+  int row0, nodes, prefix;
+  if (!tree_sequence(p, b, row0, nodes, prefix)) return;
+  if (base & 1023) {  // the swizzled layouts count on it
+    atomicCAS(p.error, 0, 2);
+    return;
+  }
+  const int trow0 = tile * kTreeRows;  // first row (node * group + head) of the tile
+  const int trows = min(kTreeRows, nodes * p.group - trow0);
+  const int end = prefix + nodes;
+  const int p0 = split * p.split_len, p1 = min(end, p0 + p.split_len);
+  if (trows <= 0 || p0 >= p1) return;
+  const int nblocks = (p1 - p0 + kTreeBlock - 1) / kTreeBlock;
+  const int active = (trows + 31) >> 5;  // softmax warps with a row
+
+  if (threadIdx.x == 0) {
+    auto init = [](uint32_t bar, uint32_t n) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+    };
+    for (int i = 0; i < 3; ++i) {
+      init(full(i), kFp8 ? 33 : 1);   // the expected bytes; each producer lane's scale bytes
+      init(empty(i), kFp8 ? 4 : 1);   // the block warps have read the codes; P V has read the rows
+      init(ready(i), 4);
+      init(free_(i), 1);
+    }
+    init(b_q, active);
+    init(b_s, 1);
+    init(b_p, active);
+    init(b_o, 1);
+    *abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 132),
+                 "r"(kTreeTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = words[1];
+  const uint32_t t_s = tmem, t_p = tmem + 128, t_o = tmem + 192;
+  auto wait = [&](uint32_t bar, uint32_t parity) { return tree_wait(bar, parity, abort_word, p.error); };
+  // the whole warp: the same answer in every lane, and all of them there again
+  auto wait_all = [&](uint32_t bar, uint32_t parity) {
+    return (bool)__all_sync(0xffffffffu, tree_wait(bar, parity, abort_word, p.error));
+  };
+
+  if (warp == 8) {
+    // ---- producer
+    const int nbox = kTreeBlock / p.box;
+    const int* table = kv.block_tables + (size_t)b * kv.max_blocks;
+    auto page_at = [&](int pos) {  // a page id outside the pool is reported and read as page 0
+      if (pos >= p1) return 0;
+      int page = table[pos / kv.ps];
+      if (page < 0 || page >= kv.num_pages) {
+        atomicExch(p.error, 1);
+        page = 0;
+      }
+      return page;
+    };
+    int issued = 0;
+    int next_box = page_at(p0 + lane * p.box), next_scale = kFp8 ? page_at(p0 + 4 * lane) : 0;
+    for (int j = 0; j < nblocks; ++j) {
+      const int st = j % L::kStages, c0 = p0 + j * kTreeBlock;
+      const int page = next_box, spage = next_scale;
+      next_box = lane < nbox ? page_at(c0 + kTreeBlock + lane * p.box) : 0;  // in flight during the wait
+      if (kFp8) next_scale = page_at(c0 + kTreeBlock + 4 * lane);
+      if (j >= L::kStages && !wait_all(empty(st), ((j / L::kStages) + 1) & 1)) break;
+      const uint32_t kdst = base + (kFp8 ? L::kRaw + st * 2 * kTreeRawBytes : L::kTiles + st * 2 * kTreeTileBytes);
+      const uint32_t vdst = kdst + (kFp8 ? kTreeRawBytes : kTreeTileBytes);
+      const int boxes = min(nbox, (p1 - c0 + p.box - 1) / p.box);
+      const uint32_t box_bytes = p.box * (kFp8 ? 64 : 128);
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(st)),
+                     "r"(2 * boxes * box_bytes)
+                     : "memory");
+      __syncwarp();
+      if (lane < boxes) {
+        const int pos = c0 + lane * p.box;
+        const int row = (page * kv.NKV + g) * kv.ps + pos % kv.ps;
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(kdst + lane * box_bytes),
+            "l"(&tp.tm_k), "r"(full(st)), "r"(0), "r"(row)
+            : "memory");
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(vdst + lane * box_bytes),
+            "l"(&tp.tm_v), "r"(full(st)), "r"(0), "r"(row)
+            : "memory");
+      }
+      if (kFp8) {
+        const int pos = c0 + 4 * lane;  // the page size is a multiple of 8: four scale bytes lie together
+        if (pos < p1) {
+          const size_t r = ((size_t)spage * kv.NKV + g) * kv.ps + pos % kv.ps;
+          const uint32_t sdst = base + L::kScales + st * 2 * kTreeBlock + 4 * lane;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sdst), "l"(kv.k_scales + r) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sdst + kTreeBlock), "l"(kv.v_scales + r)
+                       : "memory");
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(st)) : "memory");
+      }
+      ++issued;
+    }
+    // every box issued lands before the CTA may exit (bounded)
+    for (int j = max(0, issued - L::kStages); j < issued; ++j) {
+      const uint64_t t0 = global_ns();
+      while (!mbar_try_wait(reinterpret_cast<uint64_t*>(smem + L::kBars) + j % L::kStages, (j / L::kStages) & 1) &&
+             global_ns() - t0 < 4000000000ull) {
+      }
+    }
+  } else if (warp == 9) {
+    // ---- issuer
+    if (lane == 0) {
+      constexpr uint32_t id_s = tree_idesc(kTreeBlock, false), id_o = tree_idesc(64, true);
+      auto pv = [&](int j) {
+        const uint32_t v = base + L::kTiles + (j % L::kReady) * 2 * kTreeTileBytes + kTreeTileBytes;
+#pragma unroll
+        for (int kk = 0; kk < kTreeBlock / 16; ++kk) {
+          const uint64_t dv = tree_desc(v + kk * 2048);
+          asm volatile(
+              "{\n\t.reg .pred p;\n\t"
+              "setp.ne.b32 p, %4, 0;\n\t"
+              "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(t_o),
+              "r"(t_p + kk * 8), "l"(dv), "r"(id_o), "r"((j > 0 || kk > 0) ? 1u : 0u)
+              : "memory");
+        }
+        tree_commit(kFp8 ? free_(j % L::kReady) : empty(j % L::kStages));
+        tree_commit(b_o);
+      };
+      bool ok = wait(b_q, 0);
+      int done = 0;
+      for (int j = 0; j < nblocks && ok; ++j) {
+        ok = wait(ready(j % L::kReady), (j / L::kReady) & 1) && (j == 0 || wait(b_p, (j - 1) & 1));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t k = base + L::kTiles + (j % L::kReady) * 2 * kTreeTileBytes;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint64_t dq = tree_desc(base + L::kQ + kk * 32), dk = tree_desc(k + kk * 32);
+          asm volatile(
+              "{\n\t.reg .pred p;\n\t"
+              "setp.ne.b32 p, %4, 0;\n\t"
+              "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(t_s),
+              "l"(dq), "l"(dk), "r"(id_s), "r"(kk > 0 ? 1u : 0u)
+              : "memory");
+        }
+        tree_commit(b_s);
+        if (j > 0) pv(j - 1);
+        done = j;
+      }
+      if (ok && wait(b_p, done & 1)) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        pv(done);
+      }
+      // all MMAs issued finish before TMEM is released (bounded): one more commit
+      // on the Q barrier's next phase, which has as many arrivals as softmax warps
+      for (int i = 0; i < active; ++i) tree_commit(b_q);
+      const uint64_t t0 = global_ns();
+      while (!mbar_try_wait(reinterpret_cast<uint64_t*>(smem + L::kBars + 96), 1) && global_ns() - t0 < 4000000000ull) {
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---- block warps, one thread per position
+    const int r = threadIdx.x - 128;
+    for (int j = 0; j < nblocks; ++j) {
+      const int st = j % L::kStages, rd = j % L::kReady, c0 = p0 + j * kTreeBlock, pos = c0 + r;
+      const bool tail = c0 + kTreeBlock > prefix;
+      const bool drafted = pos >= prefix && pos < end;
+      uint8_t* vrow = smem + L::kTiles + rd * 2 * kTreeTileBytes + kTreeTileBytes + r * 128;
+      bool not_finite = false;
+      if (!wait_all(full(st), (j / L::kStages) & 1)) break;
+      if (kFp8) {
+        if (j >= L::kReady && !wait_all(free_(rd), ((j / L::kReady) + 1) & 1)) break;
+        const uint8_t* sc = smem + L::kScales + st * 2 * kTreeBlock;
+        const int ks = sc[r];
+        int vs = sc[kTreeBlock + r];
+        if (pos >= end) vs = -1;  // nothing there: V is 0
+        if (drafted && vs == kScaleNaN) {
+          not_finite = true;
+          vs = -1;
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {  // K, V
+          const int byte = x ? vs : ks;
+          // 2^120 * 2^(byte - 127); above bf16's range in two factors
+          const __nv_bfloat162 f = byte < 0 ? tree_pow2(0) : byte == kScaleNaN ? tree_nan2() : tree_pow2(min(byte + 120, 254));
+          const __nv_bfloat162 f2 = byte + 120 > 254 && byte != kScaleNaN ? tree_pow2(byte + 120 - 254 + 127) : tree_pow2(127);
+          const bool two = __any_sync(0xffffffffu, byte + 120 > 254 && byte != kScaleNaN);
+          const uint8_t* src = smem + L::kRaw + st * 2 * kTreeRawBytes + x * kTreeRawBytes + r * 64;
+          uint8_t* dst = smem + L::kTiles + rd * 2 * kTreeTileBytes + x * kTreeTileBytes + r * 128;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            // the codes came in with the 64-byte swizzle, the rows go out with the 128-byte one
+            const uint4 u = *reinterpret_cast<const uint4*>(src + ((c ^ ((r >> 1) & 3)) << 4));
+            uint2 w[4] = {tree_decode(u.x, f), tree_decode(u.y, f), tree_decode(u.z, f), tree_decode(u.w, f)};
+            if (two) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                __nv_bfloat162 a = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&w[e].x), f2);
+                __nv_bfloat162 d = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&w[e].y), f2);
+                w[e] = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&d));
+              }
+            }
+            *reinterpret_cast<uint4*>(dst + (((2 * c) ^ (r & 7)) << 4)) = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
+            *reinterpret_cast<uint4*>(dst + (((2 * c + 1) ^ (r & 7)) << 4)) = make_uint4(w[2].x, w[2].y, w[3].x, w[3].y);
+          }
+        }
+      } else if (tail) {
+        if (drafted) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint4 u = reinterpret_cast<const uint4*>(vrow)[c];
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              not_finite |= (w[e] & 0x7F800000u) == 0x7F800000u || (w[e] & 0x7F80u) == 0x7F80u;
+          }
+        }
+        if (pos >= end || not_finite) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(vrow)[c] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (tail) {
+        const uint32_t w = __ballot_sync(0xffffffffu, not_finite);
+        if (lane == 0) bad[rd * 4 + warp - 4] = w;
+      }
+      if (kFp8 || tail) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if (kFp8) tree_arrive(empty(st));
+        tree_arrive(ready(rd));
+      }
+    }
+  } else if (warp < active) {
+    // ---- softmax, one thread per row
+    const int r = threadIdx.x, pr = trow0 + r;
+    const bool real = r < trows;
+    const int node = real ? pr / p.group : 0, head = g * p.group + (real ? pr % p.group : 0);
+    const int row = row0 + node;
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + ((size_t)row * p.NQ + head) * 64);
+      uint8_t* dst = smem + L::kQ + r * 128;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint4 u = real ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        if (kFp8)  // the order of dims that tree_decode leaves: 0, 2, 1, 3
+          u = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632),
+                         __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
+        *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = u;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) tree_arrive(b_q);
+    }
+    const uint32_t tl = (uint32_t)(warp * 32) << 16;
+    const float c2 = p.scale * 1.4426950408889634f;  // scores in powers of two
+    const unsigned long long* mrow = p.mask + (size_t)row * p.words;
+    float m = -INFINITY, l = 0.f;  // m: the reference maximum, in powers of two
+    bool ok = true;
+    for (int j = 0; j < nblocks; ++j) {
+      const int c0 = p0 + j * kTreeBlock;
+      const bool tail = c0 + kTreeBlock > prefix;
+      unsigned long long vis0 = ~0ull, vis1 = ~0ull, bad0 = 0, bad1 = 0;
+      if (tail) {
+        vis0 = tree_bits(mrow, p.words, nodes, c0 - prefix);
+        vis1 = tree_bits(mrow, p.words, nodes, c0 + 64 - prefix);
+        ok = wait_all(ready(j % L::kReady), (j / L::kReady) & 1);
+        if (!ok) break;
+        const int rd = j % L::kReady;
+        bad0 = vis0 & (bad[rd * 4] | (unsigned long long)bad[rd * 4 + 1] << 32);
+        bad1 = vis1 & (bad[rd * 4 + 2] | (unsigned long long)bad[rd * 4 + 3] << 32);
+      }
+      ok = wait_all(b_s, j & 1);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      auto load = [&](int c, float (&v)[32]) {
+        tree_ld32(t_s + tl + 32 * c, v);
+        if (tail) {
+          const uint32_t vw = (uint32_t)((c & 2 ? vis1 : vis0) >> (32 * (c & 1)));
+          const uint32_t bw = (uint32_t)((c & 2 ? bad1 : bad0) >> (32 * (c & 1)));
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (!((vw >> i) & 1)) v[i] = -INFINITY;
+            if ((bw >> i) & 1) v[i] = __uint_as_float(0x7FFFFFFFu);
+          }
+        }
+      };
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float v[32];
+        load(c, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, v[i]);
+      }
+      mx *= c2;
+      // P V of the block before has read P and completed O
+      if (j > 0) {
+        ok = wait_all(b_o, (j - 1) & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      const bool grow = mx > m + 8.f;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float alpha = grow ? tree_exp2(m - mx) : 1.f;  // 0 for the first maximum
+        if (grow) m = mx;
+        l *= alpha;
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            float v[32];
+            uint32_t w[32];
+            tree_ld32(t_o + tl + 32 * c, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * alpha);
+            tree_st32(t_o + tl + 32 * c, w);
+          }
+        }
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float v[32];
+        load(c, v);
+        uint32_t w[16];
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float a = tree_exp2(fmaf(v[2 * i], c2, -mu)), d = tree_exp2(fmaf(v[2 * i + 1], c2, -mu));
+          s0 += a;
+          s1 += d;
+          __nv_bfloat162 h = __floats2bfloat162_rn(a, d);
+          w[i] = *reinterpret_cast<uint32_t*>(&h);
+        }
+        l += s0 + s1;
+        tree_st16(t_p + tl + 16 * c, w);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) tree_arrive(b_p);
+    }
+    if (ok) ok = wait_all(b_o, (nblocks - 1) & 1);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (ok) {
+      float o[64];
+      {
+        float v[32];
+        tree_ld32(t_o + tl, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[kFp8 && (i & 3) % 3 ? (i ^ 3) : i] = v[i];
+        tree_ld32(t_o + tl + 32, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[32 + (kFp8 && (i & 3) % 3 ? (i ^ 3) : i)] = v[i];
+      }
+      if (real && p.splits == 1) {
+        tree_store_row(p, row, head, o, l, m);
+      } else if (real) {
+        float* dst = p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
+        *reinterpret_cast<float2*>(dst) = make_float2(m, l);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) reinterpret_cast<float2*>(dst)[1 + i] = make_float2(o[2 * i], o[2 * i + 1]);
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 9) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTreeTmem) : "memory");
+  }
+}
+
+// One warp per (node, query head): the splits' partials joined, in split order.
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, g = blockIdx.y, b = blockIdx.z;
+  const int pr = blockIdx.x * 8 + (threadIdx.x >> 5);
+  int row0, nodes, prefix;
+  if (!tree_sequence(p, b, row0, nodes, prefix) || pr >= nodes * p.group) return;
+  const int splits = (prefix + nodes + p.split_len - 1) / p.split_len;
+  const size_t stride = (size_t)p.max_nodes * p.group * kTreePartial;
+  const float* src = p.work + ((size_t)b * p.kv.NKV + g) * p.splits * stride + (size_t)pr * kTreePartial;
+  float m = -INFINITY;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, src[s * stride]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float* q = src + s * stride;
+    const float a = tree_exp2(q[0] - mu);
+    const float2 v = *reinterpret_cast<const float2*>(q + 2 + 2 * lane);
+    l = fmaf(q[1], a, l);
+    o0 = fmaf(v.x, a, o0);
+    o1 = fmaf(v.y, a, o1);
+  }
+  const int row = row0 + pr / p.group, head = g * p.group + pr % p.group;
+  const bool any = l != 0.f;
   reinterpret_cast<__nv_bfloat162*>(p.out + ((size_t)row * p.NQ + head) * 64)[lane] =
       __floats2bfloat162_rn(any ? o0 / l : 0.f, any ? o1 / l : 0.f);
-  if (p.lse && lane == 0) p.lse[(size_t)row * p.NQ + head] = any ? m + logf(l) : -INFINITY;
+  if (p.lse && lane == 0) p.lse[(size_t)row * p.NQ + head] = any ? mu * 0.6931471805599453f + logf(l) : -INFINITY;
 }
 
 }  // namespace mk
