@@ -469,7 +469,7 @@ int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32
  * committed position and the nodes j of its sequence whose bit j % 64 of
  * mask[node][j / 64] is set (mask [rows][ceil(max_nodes / 64)], bits past the
  * sequence's nodes ignored). out [rows][num_q_heads][64] bf16 = softmax(scale
- * q K^T) V; lse [rows][num_q_heads] fp32 (may be NULL) the log of the
+ * q K^T) V, scale > 0; lse [rows][num_q_heads] fp32 (may be NULL) the log of the
  * normaliser. A node that attends nothing gets out 0, lse -inf; what masked
  * places and the pages behind the last node hold has no effect on a row. A
  * row that attends a node whose K or V is not finite is not finite.
@@ -477,7 +477,7 @@ int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32
  * bound every sequence's nodes and prefix + nodes. One node per sequence with
  * its own bit is a plain decode step. *error = 1: lengths or node ranges beyond
  * the bounds (that sequence is not computed) or a page id out of range (its
- * positions are skipped); 2: a device-side wait ran out (2 s). */
+ * sequence's rows mean nothing); 2: a device-side wait ran out (2 s). */
 int64_t mk_tree_attention_workspace(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                     int32_t max_nodes, int32_t max_len);
 int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_nodes,
@@ -489,7 +489,8 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
 /* Log probabilities from logits [rows][ld] (the first `vocab` columns; dtype
  * MK_F32 or MK_BF16): logprobs [rows][num_targets] of targets (int32; negative:
  * no token, 0 is written), entropy [rows] in nats, and the `top` (0..32) most
- * likely ids with their log probabilities, ties to the lower id. Logits of -inf
+ * likely ids with their log probabilities, ties to the lower id. vocab is at most
+ * 524,288. Logits of -inf
  * are forbidden tokens. A row of nothing else has log probabilities -inf and
  * entropy 0; one with a NaN or +inf has NaN for both. *error = 1: a target
  * >= vocab (its log probability is NaN). */

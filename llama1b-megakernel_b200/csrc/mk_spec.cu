@@ -3,6 +3,7 @@
 // (mk_tree.cuh), log probabilities of tokens (mk_logprobs.cuh).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "../../include/mk.h"
@@ -102,6 +103,47 @@ cudaError_t launch_tree(const mk::TreeTmaParams& tp, dim3 grid, cudaStream_t st)
   constexpr int smem = mk::TreeSmem<kFp8>::kBytes;
   if (cudaError_t e = allow_smem(mk::tree_attn_kernel<kFp8>, smem, done)) return e;
   return launch_pdl(mk::tree_attn_kernel<kFp8>, grid, dim3(mk::kTreeThreads), smem, st, tp);
+}
+
+// How a row is cut. Chunks of 16 logits a thread, or of one vector where the rows
+// have too few of those to give every SM work. A slice costs its chunks and about
+// kLpFixedChunks more (the choice of alternatives, the join); an SM's share is that
+// times the slices that fall to it, and the cut with the least is taken.
+constexpr int kLpMaxVocab = mk::kLpThreads * mk::kLpThreads * 8;  // the join takes a slice per thread
+constexpr int kLpFixedChunks = 2;
+struct LpCut {
+  int per, slices, len;
+};
+LpCut lp_cut(int rows, int vocab, int vector) {
+  const int sms = device_sms();
+  auto chunks = [&](int per) { return (vocab + mk::kLpThreads * per - 1) / (mk::kLpThreads * per); };
+  int per = 16;
+  if ((long long)rows * chunks(per) < 2LL * sms && chunks(vector) <= mk::kLpThreads) per = vector;
+  const int n = chunks(per);
+  int each = n, slices = 1;
+  long long least = -1;
+  for (int want = 1; want <= std::min(n, mk::kLpThreads); ++want) {
+    const int e = (n + want - 1) / want, k = (n + e - 1) / e;
+    const long long cost = (((long long)rows * k + sms - 1) / sms) * (e + kLpFixedChunks);
+    if (k <= mk::kLpThreads && (least < 0 || cost < least)) {
+      least = cost;
+      each = e;
+      slices = k;
+    }
+  }
+  return {per, slices, each * mk::kLpThreads * per};
+}
+
+template <typename T, int E>
+cudaError_t launch_logprobs_e(const mk::LogprobsParams& p, bool vec, cudaStream_t st) {
+  return launch_pdl(vec ? mk::logprobs_kernel<T, E, true> : mk::logprobs_kernel<T, E, false>, dim3(p.slices, p.rows),
+                    dim3(mk::kLpThreads), 0, st, p);
+}
+
+template <typename T>
+cudaError_t launch_logprobs(const mk::LogprobsParams& p, int per, bool vec, cudaStream_t st) {
+  constexpr int N = 16 / (int)sizeof(T);
+  return per == N ? launch_logprobs_e<T, N>(p, vec, st) : launch_logprobs_e<T, 16>(p, vec, st);
 }
 
 }  // namespace
@@ -228,8 +270,10 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
 }
 
 int64_t mk_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top) {
-  if (rows < 1 || vocab < 1 || top < 0 || top > mk::kLogprobsMaxTop) return 0;
-  return 0;
+  if (rows < 1 || vocab < 1 || vocab > kLpMaxVocab || top < 0 || top > mk::kLogprobsMaxTop) return 0;
+  // either type's slices
+  const int64_t slices = std::max(lp_cut(rows, vocab, 4).slices, lp_cut(rows, vocab, 8).slices);
+  return slices == 1 ? 0 : (int64_t)rows * slices * (16 + 8 * top);
 }
 
 int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t ld,
@@ -238,13 +282,15 @@ int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t v
                       float* top_logprobs, int32_t* error, void* stream) {
   if (!logits || !entropy || !error) return fail(MK_EINVAL, "NULL argument");
   if (dtype != MK_F32 && dtype != MK_BF16) return fail(MK_EINVAL, "logits type %d", dtype);
-  if (rows < 0 || vocab < 1 || ld < vocab) return fail(MK_EINVAL, "rows %d, vocab %d, ld %lld", rows, vocab, (long long)ld);
+  if (rows < 0 || vocab < 1 || vocab > kLpMaxVocab || ld < vocab) return fail(MK_EINVAL, "rows %d, vocab %d, ld %lld", rows, vocab, (long long)ld);
   if (num_targets < 0 || (num_targets && (!targets || !logprobs)))
     return fail(MK_EINVAL, "num_targets %d needs targets and logprobs", num_targets);
   if (top < 0 || top > mk::kLogprobsMaxTop || top > vocab || (top && (!top_ids || !top_logprobs)))
     return fail(MK_EINVAL, "top %d must be in [0, min(%d, vocab)] and needs top_ids and top_logprobs", top,
                 mk::kLogprobsMaxTop);
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == MK_F32 ? 4 : 2)) return fail(MK_EINVAL, "logits are not aligned to their type");
   const int64_t need = mk_token_logprobs_workspace(rows, vocab, top);
+  if (need > 0 && !aligned16(workspace)) return fail(MK_EINVAL, "the workspace must be 16-byte aligned");
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(MK_EINVAL, "workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   if (rows == 0) return MK_OK;
@@ -261,8 +307,30 @@ int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t v
   p.top_ids = top_ids;
   p.top_logprobs = top_logprobs;
   p.error = error;
-  MK_CUDA(launch_pdl(dtype == MK_F32 ? mk::logprobs_kernel<float> : mk::logprobs_kernel<__nv_bfloat16>, dim3(rows),
-                     dim3(256), 0, static_cast<cudaStream_t>(stream), p));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int size = dtype == MK_F32 ? 4 : 2;
+  const LpCut cut = lp_cut(rows, vocab, 16 / size);
+  p.slices = cut.slices;
+  p.slice_len = cut.len;
+  p.stats = static_cast<float*>(workspace);
+  p.lists = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(workspace) + (int64_t)rows * p.slices * 16);
+  const bool vec = aligned16(logits) && (rows == 1 || (ld * size) % 16 == 0);
+  // rows go in launches of at most 65,535 (the grid's second dimension)
+  for (int r0 = 0; r0 < rows; r0 += 65535) {
+    mk::LogprobsParams q = p;
+    const int64_t n = std::min(rows - r0, 65535);
+    q.logits = static_cast<const uint8_t*>(logits) + (int64_t)r0 * ld * size;
+    q.rows = (int)n;
+    q.targets += (int64_t)r0 * num_targets;
+    q.logprobs += (int64_t)r0 * num_targets;
+    q.entropy += r0;
+    q.top_ids += (int64_t)r0 * top;
+    q.top_logprobs += (int64_t)r0 * top;
+    MK_CUDA(dtype == MK_F32 ? launch_logprobs<float>(q, cut.per, vec, st) : launch_logprobs<__nv_bfloat16>(q, cut.per, vec, st));
+    if (p.slices > 1)
+      MK_CUDA(launch_pdl(dtype == MK_F32 ? mk::logprobs_join_kernel<float> : mk::logprobs_join_kernel<__nv_bfloat16>,
+                         dim3((unsigned)n), dim3(mk::kLpThreads), 0, st, q));
+  }
   return MK_OK;
 }
 
