@@ -22,12 +22,14 @@
 //    in P V would reach rows that do not see them), which are noted in a bit mask.
 //    8-bit: it turns codes into bf16 rows of the value code * 2^e, exactly (see
 //    tree_decode), and treats the last block's V in the same way;
-//  * one thread issues S = Q K^T (M 128, N 128, 64 dims) and O += P V (N 64, 128
-//    positions) with P read from TMEM and V taken MN-major as it lies;
-//  * four warps do the softmax, one thread per row (TMEM lane): S from TMEM, the
-//    exponentials, P as bf16 pairs back to TMEM. O is only rescaled when a row's
-//    maximum has grown by more than 8 powers of two since it was last set:
-//    until then p is at most 256, which costs bf16 and fp32 nothing.
+//  * one thread issues S = Q K^T (M 128, N 64, 64 dims) for half a block and O += P V
+//    (N 64, 64 positions) with P read from TMEM and V taken MN-major as it lies. S
+//    and P are double-buffered by halves: the next half's S is there before the
+//    softmax asks for it;
+//  * four warps do the softmax, one thread per row (TMEM lane): the 64 scores from
+//    TMEM into registers, the exponentials, P as bf16 pairs back to TMEM. O is only
+//    rescaled when a row's maximum has grown by more than 8 powers of two since it
+//    was last set: until then p is at most 256, which costs bf16 and fp32 nothing.
 // P is rounded to bf16 (relative 2^-8 at most, unbiased, as V is no more precise
 // itself); its sum is taken before the rounding. A range that is not the whole
 // sequence leaves (m, l, O) in the workspace for tree_merge_kernel.
@@ -45,9 +47,10 @@ namespace mk {
 constexpr int kTreeMaxNodes = 256;
 constexpr int kTreeRows = 128;     // rows of a tile (the MMA's M)
 constexpr int kTreeBlock = 128;    // positions of a block
+constexpr int kTreeHalf = 64;      // of a step of the softmax
 constexpr int kTreeThreads = 320;  // 4 softmax warps, 4 block warps, producer, issuer
 constexpr int kTreePartial = 66;   // m, l, o[64]
-constexpr uint32_t kTreeTmem = 256;  // columns: S 128, P 64, O 64
+constexpr uint32_t kTreeTmem = 256;  // columns: S 2 x 64, P 2 x 32, O 64
 constexpr uint32_t kTreeTileBytes = kTreeBlock * 128;  // a bf16 K or V block (and the Q tile)
 constexpr uint32_t kTreeRawBytes = kTreeBlock * 64;    // an 8-bit one
 
@@ -157,8 +160,8 @@ __device__ __forceinline__ constexpr uint32_t tree_idesc(int n, bool trans_b) {
          ((uint32_t)(kTreeRows >> 4) << 24);
 }
 
-__device__ __forceinline__ void tree_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns of the thread's TMEM lane; tree_ld_wait() before the values are used.
+__device__ __forceinline__ void tree_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
       "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -167,19 +170,30 @@ __device__ __forceinline__ void tree_ld32(uint32_t taddr, float (&v)[32]) {
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-__device__ __forceinline__ void tree_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+// The loads issued so far are complete; the values pass through, so that no use is
+// moved ahead of the wait.
+__device__ __forceinline__ void tree_ld_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+  asm volatile(""
+               : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void tree_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 
@@ -196,6 +210,23 @@ __device__ __forceinline__ float tree_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 tree_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<unsigned long long*>(&d))
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return d;
+}
+__device__ __forceinline__ float2 tree_add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<unsigned long long*>(&d))
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return d;
 }
 
 // Four e4m3 codes as bf16: {d0, d2} and {d1, d3}. A code s eeee mmm moved into
@@ -263,14 +294,17 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, g = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-  // barriers: full[3], empty[3], ready[3], free[3], q, s, pr, o; then words
+  // barriers: full[3], empty[3], ready[3], free[3], q, s[2], p[2], o[2]; then words
   const uint32_t bars = base + L::kBars;
   auto full = [&](int i) { return bars + 8 * i; };
   auto empty = [&](int i) { return bars + 24 + 8 * i; };
   auto ready = [&](int i) { return bars + 48 + 8 * i; };
   auto free_ = [&](int i) { return bars + 72 + 8 * i; };
-  const uint32_t b_q = bars + 96, b_s = bars + 104, b_p = bars + 112, b_o = bars + 120;
-  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 128);
+  const uint32_t b_q = bars + 96;
+  auto b_s = [&](int h) { return bars + 104 + 8 * (h & 1); };  // S of half h is in TMEM
+  auto b_p = [&](int h) { return bars + 120 + 8 * (h & 1); };  // P is, and S has been read
+  auto b_o = [&](int h) { return bars + 136 + 8 * (h & 1); };  // O has the half, P has been read
+  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 160);
   volatile uint32_t* abort_word = words;      // words[1]: TMEM base
   volatile uint32_t* bad = words + 4;         // [kReady][4] drafted positions whose V is not finite
 
@@ -287,6 +321,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int p0 = split * p.split_len, p1 = min(end, p0 + p.split_len);
   if (trows <= 0 || p0 >= p1) return;
   const int nblocks = (p1 - p0 + kTreeBlock - 1) / kTreeBlock;
+  const int halves = (p1 - p0 + kTreeHalf - 1) / kTreeHalf;
   const int active = (trows + 31) >> 5;  // softmax warps with a row
 
   if (threadIdx.x == 0) {
@@ -300,14 +335,16 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       init(free_(i), 1);
     }
     init(b_q, active);
-    init(b_s, 1);
-    init(b_p, active);
-    init(b_o, 1);
+    for (int i = 0; i < 2; ++i) {
+      init(b_s(i), 1);
+      init(b_p(i), active);
+      init(b_o(i), 1);
+    }
     *abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 132),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 164),
                  "r"(kTreeTmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -316,7 +353,9 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = words[1];
-  const uint32_t t_s = tmem, t_p = tmem + 128, t_o = tmem + 192;
+  const uint32_t t_o = tmem + 192;
+  auto t_s = [&](int h) { return tmem + 64 * (h & 1); };
+  auto t_p = [&](int h) { return tmem + 128 + 32 * (h & 1); };
   auto wait = [&](uint32_t bar, uint32_t parity) { return tree_wait(bar, parity, abort_word, p.error); };
   // the whole warp: the same answer in every lane, and all of them there again
   auto wait_all = [&](uint32_t bar, uint32_t parity) {
@@ -390,46 +429,44 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   } else if (warp == 9) {
     // ---- issuer
     if (lane == 0) {
-      constexpr uint32_t id_s = tree_idesc(kTreeBlock, false), id_o = tree_idesc(64, true);
-      auto pv = [&](int j) {
-        const uint32_t v = base + L::kTiles + (j % L::kReady) * 2 * kTreeTileBytes + kTreeTileBytes;
-#pragma unroll
-        for (int kk = 0; kk < kTreeBlock / 16; ++kk) {
-          const uint64_t dv = tree_desc(v + kk * 2048);
-          asm volatile(
-              "{\n\t.reg .pred p;\n\t"
-              "setp.ne.b32 p, %4, 0;\n\t"
-              "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(t_o),
-              "r"(t_p + kk * 8), "l"(dv), "r"(id_o), "r"((j > 0 || kk > 0) ? 1u : 0u)
-              : "memory");
-        }
-        tree_commit(kFp8 ? free_(j % L::kReady) : empty(j % L::kStages));
-        tree_commit(b_o);
-      };
-      bool ok = wait(b_q, 0);
-      int done = 0;
-      for (int j = 0; j < nblocks && ok; ++j) {
-        ok = wait(ready(j % L::kReady), (j / L::kReady) & 1) && (j == 0 || wait(b_p, (j - 1) & 1));
-        if (!ok) break;
+      constexpr uint32_t id_s = tree_idesc(kTreeHalf, false), id_o = tree_idesc(64, true);
+      auto tile_of = [&](int h) { return base + L::kTiles + (h / 2 % L::kReady) * 2 * kTreeTileBytes + (h & 1) * kTreeHalf * 128; };
+      auto scores = [&](int h) {
+        if (!(h & 1) && !wait(ready(h / 2 % L::kReady), (h / 2 / L::kReady) & 1)) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t k = base + L::kTiles + (j % L::kReady) * 2 * kTreeTileBytes;
+        const uint32_t k = tile_of(h);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           const uint64_t dq = tree_desc(base + L::kQ + kk * 32), dk = tree_desc(k + kk * 32);
           asm volatile(
               "{\n\t.reg .pred p;\n\t"
               "setp.ne.b32 p, %4, 0;\n\t"
-              "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(t_s),
+              "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(t_s(h)),
               "l"(dq), "l"(dk), "r"(id_s), "r"(kk > 0 ? 1u : 0u)
               : "memory");
         }
-        tree_commit(b_s);
-        if (j > 0) pv(j - 1);
-        done = j;
-      }
-      if (ok && wait(b_p, done & 1)) {
+        tree_commit(b_s(h));
+        return true;
+      };
+      bool ok = wait(b_q, 0) && scores(0) && (halves < 2 || scores(1));
+      for (int h = 0; h < halves && ok; ++h) {
+        ok = wait(b_p(h), (h >> 1) & 1);
+        if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        pv(done);
+        const uint32_t v = tile_of(h) + kTreeTileBytes;
+#pragma unroll
+        for (int kk = 0; kk < kTreeHalf / 16; ++kk) {
+          const uint64_t dv = tree_desc(v + kk * 2048);
+          asm volatile(
+              "{\n\t.reg .pred p;\n\t"
+              "setp.ne.b32 p, %4, 0;\n\t"
+              "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(t_o),
+              "r"(t_p(h) + kk * 8), "l"(dv), "r"(id_o), "r"((h > 0 || kk > 0) ? 1u : 0u)
+              : "memory");
+        }
+        if (h & 1) tree_commit(kFp8 ? free_(h / 2 % L::kReady) : empty(h / 2 % L::kStages));
+        tree_commit(b_o(h));
+        if (h + 2 < halves) ok = scores(h + 2);
       }
       // all MMAs issued finish before TMEM is released (bounded): one more commit
       // on the Q barrier's next phase, which has as many arrivals as softmax warps
@@ -538,101 +575,97 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     const unsigned long long* mrow = p.mask + (size_t)row * p.words;
     float m = -INFINITY, l = 0.f;  // m: the reference maximum, in powers of two
     bool ok = true;
-    for (int j = 0; j < nblocks; ++j) {
-      const int c0 = p0 + j * kTreeBlock;
-      const bool tail = c0 + kTreeBlock > prefix;
-      unsigned long long vis0 = ~0ull, vis1 = ~0ull, bad0 = 0, bad1 = 0;
+    for (int h = 0; h < halves; ++h) {
+      const int c0 = p0 + h * kTreeHalf, rd = h / 2 % L::kReady;
+      const bool tail = c0 + kTreeHalf > prefix;
+      unsigned long long vis = ~0ull, poison = 0;
       if (tail) {
-        vis0 = tree_bits(mrow, p.words, nodes, c0 - prefix);
-        vis1 = tree_bits(mrow, p.words, nodes, c0 + 64 - prefix);
-        ok = wait_all(ready(j % L::kReady), (j / L::kReady) & 1);
+        vis = tree_bits(mrow, p.words, nodes, c0 - prefix);
+        ok = wait_all(ready(rd), (h / 2 / L::kReady) & 1);
         if (!ok) break;
-        const int rd = j % L::kReady;
-        bad0 = vis0 & (bad[rd * 4] | (unsigned long long)bad[rd * 4 + 1] << 32);
-        bad1 = vis1 & (bad[rd * 4 + 2] | (unsigned long long)bad[rd * 4 + 3] << 32);
+        poison = vis & (bad[rd * 4 + 2 * (h & 1)] | (unsigned long long)bad[rd * 4 + 2 * (h & 1) + 1] << 32);
       }
-      ok = wait_all(b_s, j & 1);
+      ok = wait_all(b_s(h), (h >> 1) & 1);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      auto load = [&](int c, float (&v)[32]) {
-        tree_ld32(t_s + tl + 32 * c, v);
-        if (tail) {
-          const uint32_t vw = (uint32_t)((c & 2 ? vis1 : vis0) >> (32 * (c & 1)));
-          const uint32_t bw = (uint32_t)((c & 2 ? bad1 : bad0) >> (32 * (c & 1)));
+      uint32_t raw[64];
+      tree_ld32(t_s(h) + tl, raw);
+      tree_ld32(t_s(h) + tl + 32, raw + 32);
+      tree_ld_wait(raw);
+      tree_ld_wait(raw + 32);
+      if (tail) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (!((vw >> i) & 1)) v[i] = -INFINITY;
-            if ((bw >> i) & 1) v[i] = __uint_as_float(0x7FFFFFFFu);
-          }
+        for (int i = 0; i < 64; ++i) {
+          if (!((vis >> i) & 1)) raw[i] = 0xFF800000u;        // -inf
+          if ((poison >> i) & 1) raw[i] = 0x7FFFFFFFu;        // NaN
         }
-      };
+      }
       float mx = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float v[32];
-        load(c, v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, v[i]);
-      }
+      for (int i = 0; i < 64; i += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(raw[i]), __uint_as_float(raw[i + 1])));
       mx *= c2;
-      // P V of the block before has read P and completed O
-      if (j > 0) {
-        ok = wait_all(b_o, (j - 1) & 1);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      }
       const bool grow = mx > m + 8.f;
       if (__any_sync(0xffffffffu, grow)) {
         const float alpha = grow ? tree_exp2(m - mx) : 1.f;  // 0 for the first maximum
         if (grow) m = mx;
         l *= alpha;
-        if (j > 0) {
+        if (h > 0) {
+          ok = wait_all(b_o(h - 1), ((h - 1) >> 1) & 1);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            float v[32];
-            uint32_t w[32];
-            tree_ld32(t_o + tl + 32 * c, v);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[16];
+            tree_ld16(t_o + tl + 16 * c, w);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * alpha);
-            tree_st32(t_o + tl + 32 * c, w);
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
+            tree_st16(t_o + tl + 16 * c, w);
           }
         }
       }
+      if (h > 1) {  // P V of the half before last has read this P
+        ok = wait_all(b_o(h), ((h - 2) >> 1) & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
       const float mu = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float v[32];
-        load(c, v);
+      const float2 scale2 = make_float2(c2, c2), shift2 = make_float2(-mu, -mu);
+      float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
         uint32_t w[16];
-        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float a = tree_exp2(fmaf(v[2 * i], c2, -mu)), d = tree_exp2(fmaf(v[2 * i + 1], c2, -mu));
-          s0 += a;
-          s1 += d;
-          __nv_bfloat162 h = __floats2bfloat162_rn(a, d);
-          w[i] = *reinterpret_cast<uint32_t*>(&h);
+          float2 x = make_float2(__uint_as_float(raw[32 * c + 2 * i]), __uint_as_float(raw[32 * c + 2 * i + 1]));
+          x = tree_fma2(x, scale2, shift2);
+          x = make_float2(tree_exp2(x.x), tree_exp2(x.y));
+          if (i & 1) {
+            s1 = tree_add2(s1, x);
+          } else {
+            s0 = tree_add2(s0, x);
+          }
+          __nv_bfloat162 pr = __floats2bfloat162_rn(x.x, x.y);
+          w[i] = *reinterpret_cast<uint32_t*>(&pr);
         }
-        l += s0 + s1;
-        tree_st16(t_p + tl + 16 * c, w);
+        tree_st16(t_p(h) + tl + 16 * c, w);
       }
+      l += (s0.x + s0.y) + (s1.x + s1.y);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) tree_arrive(b_p);
+      if (lane == 0) tree_arrive(b_p(h));
     }
-    if (ok) ok = wait_all(b_o, (nblocks - 1) & 1);
+    if (ok) ok = wait_all(b_o(halves - 1), ((halves - 1) >> 1) & 1);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (ok) {
       float o[64];
-      {
-        float v[32];
-        tree_ld32(t_o + tl, v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[kFp8 && (i & 3) % 3 ? (i ^ 3) : i] = v[i];
-        tree_ld32(t_o + tl + 32, v);
+      for (int c = 0; c < 2; ++c) {
+        uint32_t raw[32];
+        tree_ld32(t_o + tl + 32 * c, raw);
+        tree_ld_wait(raw);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[32 + (kFp8 && (i & 3) % 3 ? (i ^ 3) : i)] = v[i];
+        for (int i = 0; i < 32; ++i) o[32 * c + (kFp8 && (i & 3) % 3 ? (i ^ 3) : i)] = __uint_as_float(raw[i]);
       }
       if (real && p.splits == 1) {
         tree_store_row(p, row, head, o, l, m);
