@@ -102,23 +102,31 @@ __device__ __forceinline__ bool tree_sequence(const TreeParams& p, int b, int& r
   return true;
 }
 
+__device__ __forceinline__ uint32_t tree_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+
 // Wait with a limit of 2 s. A wait that runs out reports error 2 and raises the
-// CTA's abort word, on which every other wait of the CTA gives up.
+// CTA's abort word, on which every other wait of the CTA gives up. The waiting is
+// kept out of the roles' loops, which have to stay in the instruction cache.
 __device__ __noinline__ bool tree_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_word, int* error) {
-  const uint64_t t0 = global_ns();
-  for (uint32_t it = 0;; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if ((it & 15) == 15) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (tree_try(bar, parity)) return true;
+    if ((it & 63) == 0) {
       if (*abort_word) return false;
-      if (global_ns() - t0 > 2000000000ull) {
+      const uint64_t now = global_ns();
+      if (!t0) {
+        t0 = now;
+      } else if (now - t0 > 2000000000ull) {
         *abort_word = 1;
         atomicCAS(error, 0, 2);
         return false;
@@ -128,23 +136,61 @@ __device__ __noinline__ bool tree_wait_slow(uint32_t bar, uint32_t parity, volat
 }
 
 __device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_word, int* error) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred q;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok ? true : tree_wait_slow(bar, parity, abort_word, error);
+  return tree_try(bar, parity) || tree_wait_slow(bar, parity, abort_word, error);
 }
 
 __device__ __forceinline__ void tree_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// The issuing warp runs converged and lets elect.sync pick the thread: descriptors
+// and addresses stay uniform over the warp. (Inside `if (lane == 0)` every MMA cost
+// about 100 cycles of moves into uniform registers, and the four of a product more
+// than the softmax of a half block.)
 __device__ __forceinline__ void tree_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+      : "memory");
+}
+
+// D = A B, four steps of 16 along K, A and B K-major in shared memory (a step is 32 bytes).
+__device__ __forceinline__ void tree_mma_scores(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred q, no, yes;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 no, 0, 0;\n\t"
+      "setp.eq.b32 yes, 0, 0;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, no;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, yes;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, yes;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, yes;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc)
+      : "memory");
+}
+
+// D (+)= A B, four steps of 16 along K, A in TMEM (a step is 8 columns), B MN-major
+// in shared memory (a step is 16 rows of 128 bytes).
+__device__ __forceinline__ void tree_mma_values(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred q, first, yes;\n\t"
+      ".reg .b64 b1, b2, b3;\n\t"
+      ".reg .b32 a1, a2, a3;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 first, %4, 0;\n\t"
+      "setp.eq.b32 yes, 0, 0;\n\t"
+      "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\t"
+      "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, first;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, yes;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, yes;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, yes;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
 }
 
 // A 128-byte-swizzled operand of 128-byte rows, groups of 8 rows 1024 bytes apart:
@@ -253,7 +299,7 @@ __device__ __forceinline__ __nv_bfloat162 tree_nan2() {
 }
 
 // 64 bits of row `mask` from bit j0 on (j0 may be negative: committed positions, all seen).
-__device__ __forceinline__ unsigned long long tree_bits(const unsigned long long* mask, int words, int nodes, int j0) {
+__device__ __noinline__ unsigned long long tree_bits(const unsigned long long* mask, int words, int nodes, int j0) {
   auto word = [&](int w) -> unsigned long long {
     if (w < 0) return ~0ull;
     if (w >= words || 64 * w >= nodes) return 0;
@@ -294,17 +340,19 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, g = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-  // barriers: full[3], empty[3], ready[3], free[3], q, s[2], p[2], o[2]; then words
+  // barriers: full[3], empty[3], ready[3], free[3], q, s[2], p[2], o[2], r[2]; then words
   const uint32_t bars = base + L::kBars;
   auto full = [&](int i) { return bars + 8 * i; };
   auto empty = [&](int i) { return bars + 24 + 8 * i; };
   auto ready = [&](int i) { return bars + 48 + 8 * i; };
   auto free_ = [&](int i) { return bars + 72 + 8 * i; };
   const uint32_t b_q = bars + 96;
-  auto b_s = [&](int h) { return bars + 104 + 8 * (h & 1); };  // S of half h is in TMEM
-  auto b_p = [&](int h) { return bars + 120 + 8 * (h & 1); };  // P is, and S has been read
-  auto b_o = [&](int h) { return bars + 136 + 8 * (h & 1); };  // O has the half, P has been read
-  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 160);
+  // of the first and second halves of the blocks, a phase per block
+  auto b_s = [&](int half) { return bars + 104 + 8 * half; };  // S is in TMEM
+  auto b_r = [&](int half) { return bars + 152 + 8 * half; };  // S has been read
+  auto b_p = [&](int half) { return bars + 120 + 8 * half; };  // P is in TMEM
+  auto b_o = [&](int half) { return bars + 136 + 8 * half; };  // O has the half, P has been read
+  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 176);
   volatile uint32_t* abort_word = words;      // words[1]: TMEM base
   volatile uint32_t* bad = words + 4;         // [kReady][4] drafted positions whose V is not finite
 
@@ -339,12 +387,13 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       init(b_s(i), 1);
       init(b_p(i), active);
       init(b_o(i), 1);
+      init(b_r(i), active);
     }
     *abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 164),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 180),
                  "r"(kTreeTmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -354,9 +403,10 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = words[1];
   const uint32_t t_o = tmem + 192;
-  auto t_s = [&](int h) { return tmem + 64 * (h & 1); };
-  auto t_p = [&](int h) { return tmem + 128 + 32 * (h & 1); };
-  auto wait = [&](uint32_t bar, uint32_t parity) { return tree_wait(bar, parity, abort_word, p.error); };
+  // the buffers of the two halves of a block
+  auto t_s = [&](int half) { return tmem + 64 * half; };
+  auto t_p = [&](int half) { return tmem + 128 + 32 * half; };
+  auto slot_at = [&](int slot) { return base + L::kTiles + slot * 2 * kTreeTileBytes; };
   // the whole warp: the same answer in every lane, and all of them there again
   auto wait_all = [&](uint32_t bar, uint32_t parity) {
     return (bool)__all_sync(0xffffffffu, tree_wait(bar, parity, abort_word, p.error));
@@ -427,67 +477,59 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       }
     }
   } else if (warp == 9) {
-    // ---- issuer
-    if (lane == 0) {
-      constexpr uint32_t id_s = tree_idesc(kTreeHalf, false), id_o = tree_idesc(64, true);
-      auto tile_of = [&](int h) { return base + L::kTiles + (h / 2 % L::kReady) * 2 * kTreeTileBytes + (h & 1) * kTreeHalf * 128; };
-      auto scores = [&](int h) {
-        if (!(h & 1) && !wait(ready(h / 2 % L::kReady), (h / 2 / L::kReady) & 1)) return false;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t k = tile_of(h);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const uint64_t dq = tree_desc(base + L::kQ + kk * 32), dk = tree_desc(k + kk * 32);
-          asm volatile(
-              "{\n\t.reg .pred p;\n\t"
-              "setp.ne.b32 p, %4, 0;\n\t"
-              "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(t_s(h)),
-              "l"(dq), "l"(dk), "r"(id_s), "r"(kk > 0 ? 1u : 0u)
-              : "memory");
-        }
-        tree_commit(b_s(h));
-        return true;
-      };
-      bool ok = wait(b_q, 0) && scores(0) && (halves < 2 || scores(1));
-      for (int h = 0; h < halves && ok; ++h) {
-        ok = wait(b_p(h), (h >> 1) & 1);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t v = tile_of(h) + kTreeTileBytes;
-#pragma unroll
-        for (int kk = 0; kk < kTreeHalf / 16; ++kk) {
-          const uint64_t dv = tree_desc(v + kk * 2048);
-          asm volatile(
-              "{\n\t.reg .pred p;\n\t"
-              "setp.ne.b32 p, %4, 0;\n\t"
-              "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(t_o),
-              "r"(t_p(h) + kk * 8), "l"(dv), "r"(id_o), "r"((h > 0 || kk > 0) ? 1u : 0u)
-              : "memory");
-        }
-        if (h & 1) tree_commit(kFp8 ? free_(h / 2 % L::kReady) : empty(h / 2 % L::kStages));
-        tree_commit(b_o(h));
-        if (h + 2 < halves) ok = scores(h + 2);
+    // ---- issuer, the whole warp converged
+    constexpr uint32_t id_s = tree_idesc(kTreeHalf, false), id_o = tree_idesc(64, true);
+    const uint64_t dq = tree_desc(base + L::kQ);
+    int ahead = 0;             // of the scores: half, ready slot and its phase
+    int slot_s = 0, phase_s = 0, slot_v = 0;
+    auto scores = [&] {
+      const int half = ahead & 1;
+      if (!half && !wait_all(ready(slot_s), phase_s)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      tree_mma_scores(t_s(half), dq, tree_desc(slot_at(slot_s) + half * (kTreeHalf * 128)), id_s);
+      tree_commit(b_s(half));
+      if (half && ++slot_s == L::kReady) {
+        slot_s = 0;
+        phase_s ^= 1;
       }
-      // all MMAs issued finish before TMEM is released (bounded): one more commit
-      // on the Q barrier's next phase, which has as many arrivals as softmax warps
-      for (int i = 0; i < active; ++i) tree_commit(b_q);
-      const uint64_t t0 = global_ns();
-      while (!mbar_try_wait(reinterpret_cast<uint64_t*>(smem + L::kBars + 96), 1) && global_ns() - t0 < 4000000000ull) {
+      ++ahead;
+      return true;
+    };
+    bool ok = wait_all(b_q, 0) && scores() && (halves < 2 || scores());
+    for (int h = 0; h < halves && ok; ++h) {
+      const int half = h & 1, phase = (h >> 1) & 1;
+      // the next S over the one just read, while the softmax is at work on that
+      ok = (h + 2 >= halves || (wait_all(b_r(half), phase) && scores())) && wait_all(b_p(half), phase);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      tree_mma_values(t_o, t_p(half), tree_desc(slot_at(slot_v) + kTreeTileBytes + half * (kTreeHalf * 128)), id_o, h > 0 ? 1u : 0u);
+      if (half) {
+        tree_commit(kFp8 ? free_(slot_v) : empty(slot_v));
+        if (++slot_v == L::kReady) slot_v = 0;
       }
+      tree_commit(b_o(half));
+    }
+    // all MMAs issued finish before TMEM is released (bounded): one more commit
+    // on the Q barrier's next phase, which has as many arrivals as softmax warps
+    for (int i = 0; i < active; ++i) tree_commit(b_q);
+    const uint64_t t0 = global_ns();
+    while (!mbar_try_wait(reinterpret_cast<uint64_t*>(smem + L::kBars + 96), 1) && global_ns() - t0 < 4000000000ull) {
     }
     __syncwarp();
   } else if (warp >= 4) {
     // ---- block warps, one thread per position
     const int r = threadIdx.x - 128;
+    static_assert(L::kStages == L::kReady, "one slot counter for both rings");
+    int rd = 0, phase = 0;
     for (int j = 0; j < nblocks; ++j) {
-      const int st = j % L::kStages, rd = j % L::kReady, c0 = p0 + j * kTreeBlock, pos = c0 + r;
+      const int st = rd, c0 = p0 + j * kTreeBlock, pos = c0 + r;
       const bool tail = c0 + kTreeBlock > prefix;
       const bool drafted = pos >= prefix && pos < end;
       uint8_t* vrow = smem + L::kTiles + rd * 2 * kTreeTileBytes + kTreeTileBytes + r * 128;
       bool not_finite = false;
-      if (!wait_all(full(st), (j / L::kStages) & 1)) break;
+      if (!wait_all(full(st), phase)) break;
       if (kFp8) {
-        if (j >= L::kReady && !wait_all(free_(rd), ((j / L::kReady) + 1) & 1)) break;
+        if (j >= L::kReady && !wait_all(free_(rd), phase ^ 1)) break;
         const uint8_t* sc = smem + L::kScales + st * 2 * kTreeBlock;
         const int ks = sc[r];
         int vs = sc[kTreeBlock + r];
@@ -548,6 +590,10 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
         if (kFp8) tree_arrive(empty(st));
         tree_arrive(ready(rd));
       }
+      if (++rd == L::kReady) {
+        rd = 0;
+        phase ^= 1;
+      }
     }
   } else if (warp < active) {
     // ---- softmax, one thread per row
@@ -575,42 +621,51 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     const unsigned long long* mrow = p.mask + (size_t)row * p.words;
     float m = -INFINITY, l = 0.f;  // m: the reference maximum, in powers of two
     bool ok = true;
+    int rd = 0, rd_phase = 0;  // the block's ready slot
     for (int h = 0; h < halves; ++h) {
-      const int c0 = p0 + h * kTreeHalf, rd = h / 2 % L::kReady;
+      const int c0 = p0 + h * kTreeHalf, half = h & 1, phase = (h >> 1) & 1;
       const bool tail = c0 + kTreeHalf > prefix;
-      unsigned long long vis = ~0ull, poison = 0;
-      if (tail) {
+      unsigned long long vis = ~0ull;
+      if (__builtin_expect(tail, 0)) {
         vis = tree_bits(mrow, p.words, nodes, c0 - prefix);
-        ok = wait_all(ready(rd), (h / 2 / L::kReady) & 1);
+        ok = wait_all(ready(rd), rd_phase);
         if (!ok) break;
-        poison = vis & (bad[rd * 4 + 2 * (h & 1)] | (unsigned long long)bad[rd * 4 + 2 * (h & 1) + 1] << 32);
+        // a row that sees a V that is not finite has no finite result
+        if (vis & (bad[rd * 4 + 2 * half] | (unsigned long long)bad[rd * 4 + 2 * half + 1] << 32))
+          l = __uint_as_float(0x7FFFFFFFu);
       }
-      ok = wait_all(b_s(h), (h >> 1) & 1);
+      if (half && ++rd == L::kReady) {
+        rd = 0;
+        rd_phase ^= 1;
+      }
+      ok = wait_all(b_s(half), phase);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       uint32_t raw[64];
-      tree_ld32(t_s(h) + tl, raw);
-      tree_ld32(t_s(h) + tl + 32, raw + 32);
+      tree_ld32(t_s(half) + tl, raw);
+      tree_ld32(t_s(half) + tl + 32, raw + 32);
       tree_ld_wait(raw);
       tree_ld_wait(raw + 32);
-      if (tail) {
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) tree_arrive(b_r(half));
+      if (__builtin_expect(tail, 0)) {
+        const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          if (!((vis >> i) & 1)) raw[i] = 0xFF800000u;        // -inf
-          if ((poison >> i) & 1) raw[i] = 0x7FFFFFFFu;        // NaN
-        }
+        for (int i = 0; i < 64; ++i)
+          if (!((i < 32 ? v0 : v1) & (1u << (i & 31)))) raw[i] = 0xFF800000u;  // -inf
       }
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 64; i += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(raw[i]), __uint_as_float(raw[i + 1])));
       mx *= c2;
       const bool grow = mx > m + 8.f;
-      if (__any_sync(0xffffffffu, grow)) {
+      if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
         const float alpha = grow ? tree_exp2(m - mx) : 1.f;  // 0 for the first maximum
         if (grow) m = mx;
         l *= alpha;
         if (h > 0) {
-          ok = wait_all(b_o(h - 1), ((h - 1) >> 1) & 1);
+          ok = wait_all(b_o(half ^ 1), ((h - 1) >> 1) & 1);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -624,7 +679,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
         }
       }
       if (h > 1) {  // P V of the half before last has read this P
-        ok = wait_all(b_o(h), ((h - 2) >> 1) & 1);
+        ok = wait_all(b_o(half), phase ^ 1);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
@@ -647,15 +702,15 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
           __nv_bfloat162 pr = __floats2bfloat162_rn(x.x, x.y);
           w[i] = *reinterpret_cast<uint32_t*>(&pr);
         }
-        tree_st16(t_p(h) + tl + 16 * c, w);
+        tree_st16(t_p(half) + tl + 16 * c, w);
       }
       l += (s0.x + s0.y) + (s1.x + s1.y);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) tree_arrive(b_p(h));
+      if (lane == 0) tree_arrive(b_p(half));
     }
-    if (ok) ok = wait_all(b_o(halves - 1), ((halves - 1) >> 1) & 1);
+    if (ok) ok = wait_all(b_o((halves - 1) & 1), ((halves - 1) >> 1) & 1);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (ok) {
       float o[64];
@@ -697,9 +752,11 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
   const size_t stride = (size_t)p.max_nodes * p.group * kTreePartial;
   const float* src = p.work + ((size_t)b * p.kv.NKV + g) * p.splits * stride + (size_t)pr * kTreePartial;
   float m = -INFINITY;
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) m = fmaxf(m, src[s * stride]);
   const float mu = m == -INFINITY ? 0.f : m;
   float l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     const float* q = src + s * stride;
     const float a = tree_exp2(q[0] - mu);
