@@ -23,13 +23,16 @@
 //    8-bit: it turns codes into bf16 rows of the value code * 2^e, exactly (see
 //    tree_decode), and treats the last block's V in the same way;
 //  * one thread issues S = Q K^T (M 128, N 64, 64 dims) for half a block and O += P V
-//    (N 64, 64 positions) with P read from TMEM and V taken MN-major as it lies. S
-//    and P are double-buffered by halves: the next half's S is there before the
-//    softmax asks for it;
-//  * four warps do the softmax, one thread per row (TMEM lane): the 64 scores from
-//    TMEM into registers, the exponentials, P as bf16 pairs back to TMEM. O is only
-//    rescaled when a row's maximum has grown by more than 8 powers of two since it
-//    was last set: until then p is at most 256, which costs bf16 and fp32 nothing.
+//    (N 64, 64 positions) with P read from TMEM and V taken MN-major as it lies;
+//  * two warpgroups do the softmax, one the first halves of the blocks and one the
+//    second, each with its own S, maximum, sum and O, which are joined at the end: a
+//    row's thread spends as long on waits, loads and bookkeeping as on its 64
+//    exponentials, so four warps (two CTAs) on each scheduler keep the special
+//    function unit busy where two did not (235 us to X for the chunk case). A thread
+//    has a row (TMEM lane): the 64 scores, the exponentials, P as bf16 pairs over S.
+//    O is only rescaled when a row's maximum has grown by more than 8 powers of two
+//    since it was last set: until then p is at most 256, which costs bf16 and fp32
+//    nothing.
 // P is rounded to bf16 (relative 2^-8 at most, unbiased, as V is no more precise
 // itself); its sum is taken before the rounding. A range that is not the whole
 // sequence leaves (m, l, O) in the workspace for tree_merge_kernel.
@@ -48,9 +51,9 @@ constexpr int kTreeMaxNodes = 256;
 constexpr int kTreeRows = 128;     // rows of a tile (the MMA's M)
 constexpr int kTreeBlock = 128;    // positions of a block
 constexpr int kTreeHalf = 64;      // of a step of the softmax
-constexpr int kTreeThreads = 320;  // 4 softmax warps, 4 block warps, producer, issuer
+constexpr int kTreeThreads = 448;  // 2 x 4 softmax warps, 4 block warps, producer, issuer
 constexpr int kTreePartial = 66;   // m, l, o[64]
-constexpr uint32_t kTreeTmem = 256;  // columns: S 2 x 64, P 2 x 32, O 64
+constexpr uint32_t kTreeTmem = 256;  // columns: S (and P over it) 2 x 64, O 2 x 64
 constexpr uint32_t kTreeTileBytes = kTreeBlock * 128;  // a bf16 K or V block (and the Q tile)
 constexpr uint32_t kTreeRawBytes = kTreeBlock * 64;    // an 8-bit one
 
@@ -63,7 +66,7 @@ struct TreeSmem {
   static constexpr uint32_t kRaw = kTiles + kReady * 2 * kTreeTileBytes;    // 8-bit: kStages x (K, V)
   static constexpr uint32_t kScales = kRaw + (kFp8 ? kStages * 2 * kTreeRawBytes : 0);  // kStages x 256
   static constexpr uint32_t kBars = kScales + (kFp8 ? kStages * 2 * kTreeBlock : 0);
-  static constexpr uint32_t kBytes = kBars + 256;
+  static constexpr uint32_t kBytes = kBars + 256;   // the (m, l) of the second softmax lie over Q at the end
 };
 
 struct TreeParams {
@@ -311,25 +314,6 @@ __device__ __noinline__ unsigned long long tree_bits(const unsigned long long* m
   return sh ? (lo >> sh) | (word(w + 1) << (64 - sh)) : lo;
 }
 
-// Where a row's result goes: the output, or this split's partial.
-__device__ __forceinline__ void tree_store_row(const TreeParams& p, int row, int head, const float (&o)[64], float l,
-                                               float m2) {
-  const bool any = l != 0.f;  // NaN counts as something
-  const float r = any ? 1.f / l : 0.f;
-  uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)row * p.NQ + head) * 64);
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      __nv_bfloat162 h = __floats2bfloat162_rn(any ? o[8 * c + 2 * e] * r : 0.f, any ? o[8 * c + 2 * e + 1] * r : 0.f);
-      w[e] = *reinterpret_cast<uint32_t*>(&h);
-    }
-    dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  if (p.lse) p.lse[(size_t)row * p.NQ + head] = any ? m2 * 0.6931471805599453f + logf(l) : -INFINITY;
-}
-
 template <bool kFp8>
 __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid_constant__ TreeTmaParams tp) {
   using L = TreeSmem<kFp8>;
@@ -340,19 +324,17 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, g = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-  // barriers: full[3], empty[3], ready[3], free[3], q, s[2], p[2], o[2], r[2]; then words
+  // barriers: full[3], empty[3], ready[3], free[3], q, s[2], p[2], o; then words
   const uint32_t bars = base + L::kBars;
   auto full = [&](int i) { return bars + 8 * i; };
   auto empty = [&](int i) { return bars + 24 + 8 * i; };
   auto ready = [&](int i) { return bars + 48 + 8 * i; };
   auto free_ = [&](int i) { return bars + 72 + 8 * i; };
-  const uint32_t b_q = bars + 96;
+  const uint32_t b_q = bars + 96, b_o = bars + 136;            // Q is in place; all O are complete
   // of the first and second halves of the blocks, a phase per block
-  auto b_s = [&](int half) { return bars + 104 + 8 * half; };  // S is in TMEM
-  auto b_r = [&](int half) { return bars + 152 + 8 * half; };  // S has been read
+  auto b_s = [&](int half) { return bars + 104 + 8 * half; };  // S is in TMEM (and O has the block before)
   auto b_p = [&](int half) { return bars + 120 + 8 * half; };  // P is in TMEM
-  auto b_o = [&](int half) { return bars + 136 + 8 * half; };  // O has the half, P has been read
-  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 176);
+  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 144);
   volatile uint32_t* abort_word = words;      // words[1]: TMEM base
   volatile uint32_t* bad = words + 4;         // [kReady][4] drafted positions whose V is not finite
 
@@ -386,14 +368,13 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     for (int i = 0; i < 2; ++i) {
       init(b_s(i), 1);
       init(b_p(i), active);
-      init(b_o(i), 1);
-      init(b_r(i), active);
     }
+    init(b_o, 1);
     *abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 180),
+  if (warp == 13) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 148),
                  "r"(kTreeTmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -402,17 +383,16 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = words[1];
-  const uint32_t t_o = tmem + 192;
-  // the buffers of the two halves of a block
-  auto t_s = [&](int half) { return tmem + 64 * half; };
-  auto t_p = [&](int half) { return tmem + 128 + 32 * half; };
+  // of the first and second halves of the blocks
+  auto t_s = [&](int half) { return tmem + 64 * half; };  // P lies over the first 32 columns of S
+  auto t_o = [&](int half) { return tmem + 128 + 64 * half; };
   auto slot_at = [&](int slot) { return base + L::kTiles + slot * 2 * kTreeTileBytes; };
   // the whole warp: the same answer in every lane, and all of them there again
   auto wait_all = [&](uint32_t bar, uint32_t parity) {
     return (bool)__all_sync(0xffffffffu, tree_wait(bar, parity, abort_word, p.error));
   };
 
-  if (warp == 8) {
+  if (warp == 12) {
     // ---- producer
     const int nbox = kTreeBlock / p.box;
     const int* table = kv.block_tables + (size_t)b * kv.max_blocks;
@@ -476,49 +456,45 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
              global_ns() - t0 < 4000000000ull) {
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 13) {
     // ---- issuer, the whole warp converged
     constexpr uint32_t id_s = tree_idesc(kTreeHalf, false), id_o = tree_idesc(64, true);
     const uint64_t dq = tree_desc(base + L::kQ);
-    int ahead = 0;             // of the scores: half, ready slot and its phase
-    int slot_s = 0, phase_s = 0, slot_v = 0;
-    auto scores = [&] {
-      const int half = ahead & 1;
-      if (!half && !wait_all(ready(slot_s), phase_s)) return false;
+    int slot = 0, next = 0, next_phase = 0;  // the block's slot; the next one's, and its phase
+    auto scores = [&](int half) {
+      if (!half && !wait_all(ready(next), next_phase)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      tree_mma_scores(t_s(half), dq, tree_desc(slot_at(slot_s) + half * (kTreeHalf * 128)), id_s);
+      tree_mma_scores(t_s(half), dq, tree_desc(slot_at(next) + half * (kTreeHalf * 128)), id_s);
       tree_commit(b_s(half));
-      if (half && ++slot_s == L::kReady) {
-        slot_s = 0;
-        phase_s ^= 1;
-      }
-      ++ahead;
       return true;
     };
-    bool ok = wait_all(b_q, 0) && scores() && (halves < 2 || scores());
-    for (int h = 0; h < halves && ok; ++h) {
-      const int half = h & 1, phase = (h >> 1) & 1;
-      // the next S over the one just read, while the softmax is at work on that
-      ok = (h + 2 >= halves || (wait_all(b_r(half), phase) && scores())) && wait_all(b_p(half), phase);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      tree_mma_values(t_o, t_p(half), tree_desc(slot_at(slot_v) + kTreeTileBytes + half * (kTreeHalf * 128)), id_o, h > 0 ? 1u : 0u);
-      if (half) {
-        tree_commit(kFp8 ? free_(slot_v) : empty(slot_v));
-        if (++slot_v == L::kReady) slot_v = 0;
+    bool ok = wait_all(b_q, 0) && scores(0) && (halves < 2 || scores(1));
+    for (int j = 0; j < nblocks && ok; ++j) {
+      if (++next == L::kReady) {
+        next = 0;
+        next_phase ^= 1;
       }
-      tree_commit(b_o(half));
+      for (int half = 0; half < 2; ++half) {
+        const int h = 2 * j + half;
+        if (h >= halves) break;
+        ok = wait_all(b_p(half), j & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tree_mma_values(t_o(half), t_s(half), tree_desc(slot_at(slot) + kTreeTileBytes + half * (kTreeHalf * 128)), id_o,
+                        j > 0 ? 1u : 0u);
+        if (half) tree_commit(kFp8 ? free_(slot) : empty(slot));
+        // the next S over the P just used: MMAs of one thread run in order
+        if (h + 2 < halves) ok = scores(half);
+        if (!ok) break;
+      }
+      slot = next;
     }
-    // all MMAs issued finish before TMEM is released (bounded): one more commit
-    // on the Q barrier's next phase, which has as many arrivals as softmax warps
-    for (int i = 0; i < active; ++i) tree_commit(b_q);
-    const uint64_t t0 = global_ns();
-    while (!mbar_try_wait(reinterpret_cast<uint64_t*>(smem + L::kBars + 96), 1) && global_ns() - t0 < 4000000000ull) {
-    }
-    __syncwarp();
-  } else if (warp >= 4) {
+    // what was issued finishes before the results are read and TMEM is released
+    tree_commit(b_o);
+    wait_all(b_o, 0);
+  } else if (warp >= 8) {
     // ---- block warps, one thread per position
-    const int r = threadIdx.x - 128;
+    const int r = threadIdx.x - 256;
     static_assert(L::kStages == L::kReady, "one slot counter for both rings");
     int rd = 0, phase = 0;
     for (int j = 0; j < nblocks; ++j) {
@@ -582,7 +558,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       }
       if (tail) {
         const uint32_t w = __ballot_sync(0xffffffffu, not_finite);
-        if (lane == 0) bad[rd * 4 + warp - 4] = w;
+        if (lane == 0) bad[rd * 4 + warp - 8] = w;
       }
       if (kFp8 || tail) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -595,13 +571,13 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
         phase ^= 1;
       }
     }
-  } else if (warp < active) {
-    // ---- softmax, one thread per row
-    const int r = threadIdx.x, pr = trow0 + r;
+  } else if ((warp & 3) < active) {
+    // ---- softmax, one thread per row; warps 0-3 the first halves, 4-7 the second
+    const int half = warp >> 2, r = threadIdx.x & 127, pr = trow0 + r;
     const bool real = r < trows;
     const int node = real ? pr / p.group : 0, head = g * p.group + (real ? pr % p.group : 0);
     const int row = row0 + node;
-    {
+    if (half == 0) {
       const uint4* src = reinterpret_cast<const uint4*>(p.q + ((size_t)row * p.NQ + head) * 64);
       uint8_t* dst = smem + L::kQ + r * 128;
 #pragma unroll
@@ -616,82 +592,81 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       __syncwarp();
       if (lane == 0) tree_arrive(b_q);
     }
-    const uint32_t tl = (uint32_t)(warp * 32) << 16;
+    const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = t_s(half) + tl, o_at = t_o(half) + tl;
     const float c2 = p.scale * 1.4426950408889634f;  // scores in powers of two
-    const unsigned long long* mrow = p.mask + (size_t)row * p.words;
     float m = -INFINITY, l = 0.f;  // m: the reference maximum, in powers of two
+    int rd = 0, rd_phase = 0;      // the block's ready slot
+    const int mine = (halves + 1 - half) >> 1;
     bool ok = true;
-    int rd = 0, rd_phase = 0;  // the block's ready slot
-    for (int h = 0; h < halves; ++h) {
-      const int c0 = p0 + h * kTreeHalf, half = h & 1, phase = (h >> 1) & 1;
+    for (int j = 0; j < mine; ++j) {
+      const int c0 = p0 + j * kTreeBlock + half * kTreeHalf;
       const bool tail = c0 + kTreeHalf > prefix;
       unsigned long long vis = ~0ull;
       if (__builtin_expect(tail, 0)) {
-        vis = tree_bits(mrow, p.words, nodes, c0 - prefix);
+        vis = tree_bits(p.mask + (size_t)row * p.words, p.words, nodes, c0 - prefix);
         ok = wait_all(ready(rd), rd_phase);
         if (!ok) break;
         // a row that sees a V that is not finite has no finite result
         if (vis & (bad[rd * 4 + 2 * half] | (unsigned long long)bad[rd * 4 + 2 * half + 1] << 32))
           l = __uint_as_float(0x7FFFFFFFu);
       }
-      if (half && ++rd == L::kReady) {
+      if (++rd == L::kReady) {
         rd = 0;
         rd_phase ^= 1;
       }
-      ok = wait_all(b_s(half), phase);
+      ok = wait_all(b_s(half), j & 1);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      uint32_t raw[64];
-      tree_ld32(t_s(half) + tl, raw);
-      tree_ld32(t_s(half) + tl + 32, raw + 32);
-      tree_ld_wait(raw);
-      tree_ld_wait(raw + 32);
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) tree_arrive(b_r(half));
-      if (__builtin_expect(tail, 0)) {
-        const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
+      auto load = [&](int c, uint32_t (&raw)[32]) {
+        tree_ld32(s_at + 32 * c, raw);
+        tree_ld_wait(raw);
+        if (__builtin_expect(tail, 0)) {
+          const uint32_t v = (uint32_t)(vis >> (32 * c));
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (!((i < 32 ? v0 : v1) & (1u << (i & 31)))) raw[i] = 0xFF800000u;  // -inf
-      }
+          for (int i = 0; i < 32; ++i)
+            if (!(v & (1u << i))) raw[i] = 0xFF800000u;  // -inf
+        }
+      };
       float mx = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t raw[32];
+        load(c, raw);
+        float x[4];
 #pragma unroll
-      for (int i = 0; i < 64; i += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(raw[i]), __uint_as_float(raw[i + 1])));
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(raw[i]);
+#pragma unroll
+        for (int i = 4; i < 32; ++i) x[i & 3] = fmaxf(x[i & 3], __uint_as_float(raw[i]));
+        mx = fmaxf(fmaxf(mx, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+      }
       mx *= c2;
       const bool grow = mx > m + 8.f;
       if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
         const float alpha = grow ? tree_exp2(m - mx) : 1.f;  // 0 for the first maximum
         if (grow) m = mx;
         l *= alpha;
-        if (h > 0) {
-          ok = wait_all(b_o(half ^ 1), ((h - 1) >> 1) & 1);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (j > 0) {
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t w[16];
-            tree_ld16(t_o + tl + 16 * c, w);
+            tree_ld16(o_at + 16 * c, w);
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
-            tree_st16(t_o + tl + 16 * c, w);
+            tree_st16(o_at + 16 * c, w);
           }
         }
-      }
-      if (h > 1) {  // P V of the half before last has read this P
-        ok = wait_all(b_o(half), phase ^ 1);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
       const float mu = m == -INFINITY ? 0.f : m;
       const float2 scale2 = make_float2(c2, c2), shift2 = make_float2(-mu, -mu);
       float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[16];
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {  // P of the first 32 scores goes over scores already used, and so on
+        uint32_t raw[32], w[16];
+        load(c, raw);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float2 x = make_float2(__uint_as_float(raw[32 * c + 2 * i]), __uint_as_float(raw[32 * c + 2 * i + 1]));
+          float2 x = make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
           x = tree_fma2(x, scale2, shift2);
           x = make_float2(tree_exp2(x.x), tree_exp2(x.y));
           if (i & 1) {
@@ -699,10 +674,10 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
           } else {
             s0 = tree_add2(s0, x);
           }
-          __nv_bfloat162 pr = __floats2bfloat162_rn(x.x, x.y);
-          w[i] = *reinterpret_cast<uint32_t*>(&pr);
+          __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+          w[i] = *reinterpret_cast<uint32_t*>(&h);
         }
-        tree_st16(t_p(half) + tl + 16 * c, w);
+        tree_st16(s_at + 16 * c, w);
       }
       l += (s0.x + s0.y) + (s1.x + s1.y);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -710,31 +685,59 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       __syncwarp();
       if (lane == 0) tree_arrive(b_p(half));
     }
-    if (ok) ok = wait_all(b_o((halves - 1) & 1), ((halves - 1) >> 1) & 1);
+    // ---- the two softmaxes joined: the second's (m, l) by way of shared memory
+    if (ok) ok = wait_all(b_o, 0);  // no MMA reads Q any more
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (ok) {
-      float o[64];
+    float2* ml = reinterpret_cast<float2*>(smem + L::kQ);
+    if (half) ml[r] = make_float2(m, l);
+    asm volatile("bar.sync 1, %0;" ::"r"(64 * active) : "memory");
+    if (ok && !half) {
+      const float2 other = ml[r];
+      const bool two = halves > 1;
+      const float m1 = two ? other.x : -INFINITY;
+      const float top = fmaxf(m, m1), mu = top == -INFINITY ? 0.f : top;
+      const float a = tree_exp2(m - mu), a1 = tree_exp2(m1 - mu);
+      const float sum = two ? l * a + other.y * a1 : l * a;
+      const bool whole = p.splits == 1, any = sum != 0.f;  // NaN counts as something
+      const float f = !whole ? a : any ? a / sum : 0.f, f1 = !whole ? a1 : any ? a1 / sum : 0.f;
+      float* part = p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
+      if (real && !whole) *reinterpret_cast<float2*>(part) = make_float2(top, sum);
+      if (real && whole && p.lse)
+        p.lse[(size_t)row * p.NQ + head] = any ? mu * 0.6931471805599453f + logf(sum) : -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16], w1[16];
+        float o[16];
+        __syncwarp();
+        tree_ld16(o_at + 16 * c, w);
+        if (two) tree_ld16(t_o(1) + tl + 16 * c, w1);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t raw[32];
-        tree_ld32(t_o + tl + 32 * c, raw);
-        tree_ld_wait(raw);
+        for (int i = 0; i < 16; ++i) {
+          const float x = __uint_as_float(w[i]) * f;
+          o[kFp8 && (i & 3) % 3 ? (i ^ 3) : i] = two ? fmaf(__uint_as_float(w1[i]), f1, x) : x;
+        }
+        if (real && whole) {
+          uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)row * p.NQ + head) * 64 + 16 * c);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[32 * c + (kFp8 && (i & 3) % 3 ? (i ^ 3) : i)] = __uint_as_float(raw[i]);
-      }
-      if (real && p.splits == 1) {
-        tree_store_row(p, row, head, o, l, m);
-      } else if (real) {
-        float* dst = p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
-        *reinterpret_cast<float2*>(dst) = make_float2(m, l);
+          for (int q = 0; q < 2; ++q) {
+            uint32_t v[4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) reinterpret_cast<float2*>(dst)[1 + i] = make_float2(o[2 * i], o[2 * i + 1]);
+            for (int e = 0; e < 4; ++e) {
+              __nv_bfloat162 h = __floats2bfloat162_rn(any ? o[8 * q + 2 * e] : 0.f, any ? o[8 * q + 2 * e + 1] : 0.f);
+              v[e] = *reinterpret_cast<uint32_t*>(&h);
+            }
+            dst[q] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        } else if (real) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) reinterpret_cast<float2*>(part + 2 + 16 * c)[i] = make_float2(o[2 * i], o[2 * i + 1]);
+        }
       }
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 13) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTreeTmem) : "memory");
   }
