@@ -122,18 +122,25 @@ __device__ __forceinline__ uint32_t tree_try(uint32_t bar, uint32_t parity) {
 // kept out of the roles' loops, which have to stay in the instruction cache.
 __device__ __noinline__ bool tree_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_word, int* error) {
   uint64_t t0 = 0;
-  for (uint32_t it = 1;; ++it) {
-    if (tree_try(bar, parity)) return true;
-    if ((it & 63) == 0) {
-      if (*abort_word) return false;
-      const uint64_t now = global_ns();
-      if (!t0) {
-        t0 = now;
-      } else if (now - t0 > 2000000000ull) {
-        *abort_word = 1;
-        atomicCAS(error, 0, 2);
-        return false;
-      }
+  for (;;) {
+    // asleep until the phase ends, 1 ms at most: warps that poll take issue slots from the softmax
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2, 1000000;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (*abort_word) return false;
+    const uint64_t now = global_ns();
+    if (!t0) {
+      t0 = now;
+    } else if (now - t0 > 2000000000ull) {
+      *abort_word = 1;
+      atomicCAS(error, 0, 2);
+      return false;
     }
   }
 }
@@ -209,31 +216,24 @@ __device__ __forceinline__ constexpr uint32_t tree_idesc(int n, bool trans_b) {
          ((uint32_t)(kTreeRows >> 4) << 24);
 }
 
-// 32 columns of the thread's TMEM lane; tree_ld_wait() before the values are used.
-__device__ __forceinline__ void tree_ld32(uint32_t taddr, uint32_t* r) {
+// 32 columns of the thread's TMEM lane.
+__device__ __forceinline__ void tree_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
+      : "r"(taddr)
+      : "memory");
 }
 
-// The loads issued so far are complete; the values pass through, so that no use is
-// moved ahead of the wait.
-__device__ __forceinline__ void tree_ld_wait(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-  asm volatile(""
-               : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
+__device__ __forceinline__ float tree_max3(float a, float b, float c) {  // NaN is nobody's largest
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 __device__ __forceinline__ void tree_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -620,7 +620,6 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       auto load = [&](int c, uint32_t (&raw)[32]) {
         tree_ld32(s_at + 32 * c, raw);
-        tree_ld_wait(raw);
         if (__builtin_expect(tail, 0)) {
           const uint32_t v = (uint32_t)(vis >> (32 * c));
 #pragma unroll
@@ -633,12 +632,11 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       for (int c = 0; c < 2; ++c) {
         uint32_t raw[32];
         load(c, raw);
-        float x[4];
+        float x[4] = {mx, __uint_as_float(raw[0]), __uint_as_float(raw[1]), -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(raw[i]);
-#pragma unroll
-        for (int i = 4; i < 32; ++i) x[i & 3] = fmaxf(x[i & 3], __uint_as_float(raw[i]));
-        mx = fmaxf(fmaxf(mx, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+        for (int i = 2; i < 32; i += 2)
+          x[(i >> 1) & 3] = tree_max3(x[(i >> 1) & 3], __uint_as_float(raw[i]), __uint_as_float(raw[i + 1]));
+        mx = tree_max3(tree_max3(x[0], x[1], x[2]), x[3], -INFINITY);
       }
       mx *= c2;
       const bool grow = mx > m + 8.f;
