@@ -11,6 +11,7 @@
 #include "mk_kv8.cuh"
 #include "mk_logprobs.cuh"
 #include "mk_tree.cuh"
+#include "mk_tree_few.cuh"
 
 using namespace mk::host;
 
@@ -42,31 +43,37 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
   return MK_OK;
 }
 
-// How the positions of a sequence are split over CTAs. Two CTAs fit an SM, so a
-// launch of n CTAs takes about ceil(n / (2 SMs)) waves of one range each; a
-// range costs its blocks and a fixed part (launch, first bytes, the store),
-// taken as kTreeFixedBlocks blocks, and joining the ranges kTreeJoinBlocks more.
-struct TreeSplit {
-  int splits, len;
+// Which kernel a call takes and how the positions of a sequence are split over its
+// CTAs. Up to kTreeFewRows rows (nodes x query heads of a K/V head) go to the
+// mma.sync kernel, in one tile of 16 or 32; more to the tcgen05 kernel in tiles of
+// 128. A launch of n CTAs, c to an SM, takes about ceil(n / (c SMs)) waves of one
+// range each; a range costs its length and a fixed part (launch, first bytes, the
+// store), and joining ranges a little more; the cheapest length is taken.
+constexpr int kTreeFewRows = 32;
+struct TreePlan {
+  int few;  // row tiles of 16 of the mma.sync kernel, 0: tcgen05
+  int tiles, splits, len;
 };
-constexpr int kTreeFixedBlocks = 3;
-constexpr int kTreeJoinBlocks = 2;
-TreeSplit tree_split(int batch, int num_kv_heads, int rows, int max_len) {
-  const int tiles = (rows + mk::kTreeRows - 1) / mk::kTreeRows;
-  const int blocks = (max_len + mk::kTreeBlock - 1) / mk::kTreeBlock;
-  const long long ctas = (long long)batch * num_kv_heads * tiles, slots = 2LL * device_sms();
-  TreeSplit best{1, blocks * mk::kTreeBlock};
-  long long best_cost = -1;
-  for (int per = blocks; per >= 1; --per) {
-    const int splits = (blocks + per - 1) / per;
+TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
+  TreePlan t{};
+  t.few = rows <= 16 ? 1 : rows <= kTreeFewRows ? 2 : 0;
+  const int tile_rows = t.few ? 16 * t.few : mk::kTreeRows;
+  t.tiles = (rows + tile_rows - 1) / tile_rows;
+  const int unit = mk::kTreeBlock, units = (max_len + unit - 1) / unit;
+  const int fixed = t.few ? 2 : 3, join = t.few ? 1 : 2;  // in units
+  const long long ctas = (long long)batch * num_kv_heads * t.tiles, slots = (t.few == 1 ? 3LL : 2LL) * device_sms();
+  long long best = -1;
+  for (int per = units; per >= 1; --per) {
+    const int splits = (units + per - 1) / per;
     const long long waves = (ctas * splits + slots - 1) / slots;
-    const long long cost = waves * (per + kTreeFixedBlocks) + (splits > 1 ? kTreeJoinBlocks : 0);
-    if (best_cost < 0 || cost < best_cost) {
-      best_cost = cost;
-      best = {splits, per * mk::kTreeBlock};
+    const long long cost = waves * (per + fixed) + (splits > 1 ? join : 0);
+    if (best < 0 || cost < best) {
+      best = cost;
+      t.splits = splits;
+      t.len = per * unit;
     }
   }
-  return best;
+  return t;
 }
 
 // A page pool as rows of 64 values, boxes of `box` whole rows: bf16 rows with the
@@ -97,8 +104,18 @@ cudaError_t allow_smem(K kernel, int bytes, bool (&done)[64]) {
   return e;
 }
 
+template <bool kFp8, int MT>
+cudaError_t launch_few(const mk::TreeTmaParams& tp, dim3 grid, cudaStream_t st) {
+  static bool done[64];
+  constexpr int smem = mk::FewShape<kFp8>::kBytes;
+  if (cudaError_t e = allow_smem(mk::tree_few_kernel<kFp8, MT>, smem, done)) return e;
+  return launch_pdl(mk::tree_few_kernel<kFp8, MT>, grid, dim3((mk::kFewWarps + 1) * 32), smem, st, tp);
+}
+
 template <bool kFp8>
-cudaError_t launch_tree(const mk::TreeTmaParams& tp, dim3 grid, cudaStream_t st) {
+cudaError_t launch_tree(const mk::TreeTmaParams& tp, int few, dim3 grid, cudaStream_t st) {
+  if (few == 1) return launch_few<kFp8, 1>(tp, grid, st);
+  if (few == 2) return launch_few<kFp8, 2>(tp, grid, st);
   static bool done[64];
   constexpr int smem = mk::TreeSmem<kFp8>::kBytes;
   if (cudaError_t e = allow_smem(mk::tree_attn_kernel<kFp8>, smem, done)) return e;
@@ -206,7 +223,7 @@ int64_t mk_tree_attention_workspace(int32_t batch, int32_t num_q_heads, int32_t 
                                     int32_t max_nodes, int32_t max_len) {
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_nodes < 1 || max_len < 1) return 0;
   const int group = num_q_heads / num_kv_heads;
-  const TreeSplit sp = tree_split(batch, num_kv_heads, max_nodes * group, max_len);
+  const TreePlan sp = tree_plan(batch, num_kv_heads, max_nodes * group, max_len);
   if (sp.splits == 1) return 0;
   return (int64_t)batch * num_kv_heads * sp.splits * max_nodes * group * mk::kTreePartial * 4;
 }
@@ -251,19 +268,19 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   p.error = error;
-  const TreeSplit sp = tree_split(batch, nkv, max_nodes * group, max_len);
-  p.tiles = (max_nodes * group + mk::kTreeRows - 1) / mk::kTreeRows;
-  p.splits = sp.splits;
-  p.split_len = sp.len;
+  const TreePlan plan = tree_plan(batch, nkv, max_nodes * group, max_len);
+  p.tiles = plan.tiles;
+  p.splits = plan.splits;
+  p.split_len = plan.len;
   p.work = static_cast<float*>(workspace);
-  p.box = 128;
-  while (kv->page_size % p.box) p.box /= 2;
   const bool fp8 = kv->format == MK_KV_E4M3;
+  p.box = !plan.few ? mk::kTreeBlock : fp8 ? mk::FewShape<true>::kChunk : mk::FewShape<false>::kChunk;
+  while (kv->page_size % p.box) p.box /= 2;
   if (int rc = encode_rows(&tp.tm_k, kv->k_pages, pool_rows, p.box, fp8)) return rc;
   if (int rc = encode_rows(&tp.tm_v, kv->v_pages, pool_rows, p.box, fp8)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(p.tiles * p.splits, nkv, batch);
-  MK_CUDA(fp8 ? launch_tree<true>(tp, grid, st) : launch_tree<false>(tp, grid, st));
+  MK_CUDA(fp8 ? launch_tree<true>(tp, plan.few, grid, st) : launch_tree<false>(tp, plan.few, grid, st));
   if (p.splits > 1)
     MK_CUDA(launch_pdl(mk::tree_merge_kernel, dim3((max_nodes * group + 7) / 8, nkv, batch), dim3(256), 0, st, p));
   return MK_OK;

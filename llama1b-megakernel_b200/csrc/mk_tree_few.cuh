@@ -1,0 +1,508 @@
+// Attention of few drafted rows per K/V head (mk_tree.cuh has the definition, the
+// parameters and the join of split ranges): decode steps and small trees.
+//
+// With at most 32 rows (nodes x query heads of a K/V head) a 128-row tensor tile
+// would be mostly empty and its softmax would run on a quarter of the SM, while the
+// work is to stream K and V once. So a tile is MT x 16 rows (MT 1 or 2) on
+// mma.sync.m16n8k16, whose B operand comes straight from registers:
+//  * four consumer warps take turns at the chunks of the range (32 positions of
+//    bf16, 64 of 8-bit codes: 8 KB either way), each with its own maximum, sum and O,
+//    joined in shared memory at the end; a producer warp keeps eight chunks in
+//    flight by TMA;
+//  * bf16: fragments by ldmatrix from the 128-byte-swizzled rows, P bf16;
+//  * 8-bit: a thread's K fragment is 16 consecutive codes of a position (one 128-bit
+//    load; the order of dims in a sum is free, so Q is laid out to match), turned
+//    into f16, where every code is exact, by one conversion a pair. Q goes to f16
+//    under a power of two for each row that brings its largest value to 2^14: what
+//    is lost lies below 2^-38 of it. The row's K scale multiplies the score. V
+//    fragments pair two positions of a dim, so their bytes are gathered and moved
+//    into bf16's place (tree_decode); V's scale multiplies P before its rounding.
+//    The positions of a block of 8 are permuted between fragment columns and rows
+//    in memory (few_place) so that both loads are free of bank conflicts under the
+//    64-byte swizzle.
+// O is rescaled when a maximum grew by more than 8 powers of two, as in mk_tree.cuh.
+#pragma once
+
+#include "mk_tree.cuh"
+
+namespace mk {
+
+constexpr int kFewWarps = 4;
+constexpr int kFewStages = 8;
+constexpr int kFewStageBytes = 8192;  // K rows, then V rows
+
+template <bool kFp8>
+struct FewShape {
+  static constexpr int kChunk = kFp8 ? 64 : 32;
+  static constexpr uint32_t kScales = kFewStages * kFewStageBytes;
+  static constexpr uint32_t kBars = kScales + (kFp8 ? kFewStages * 2 * kChunk : 0);
+  static constexpr uint32_t kBytes = kBars + 256;
+};
+
+// The row within its 8 that fragment column c reads (8-bit): bits (c1 ^ c0, c0, c2).
+__device__ __forceinline__ int few_place(int c) { return (((c >> 1) ^ c) & 1) | ((c & 1) << 1) | (c & 4); }
+
+__device__ __forceinline__ void few_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void few_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+template <bool kHalf>
+__device__ __forceinline__ void few_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kHalf) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+// Two e4m3 codes (the low or the high half of w) as f16, exactly.
+__device__ __forceinline__ uint32_t few_half2(uint32_t w, bool high) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(high ? w >> 16 : w)));
+  return h;
+}
+
+template <bool kFp8, int MT>
+__global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
+    tree_few_kernel(const __grid_constant__ TreeTmaParams tp) {
+  using L = FewShape<kFp8>;
+  constexpr int C = L::kChunk, R = 16 * MT;
+  const TreeParams& p = tp.p;
+  const KVLayer& kv = p.kv;
+  pdl_trigger();
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, g = blockIdx.y, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
+  auto full = [&](int i) { return base + L::kBars + 8 * i; };
+  auto empty = [&](int i) { return base + L::kBars + 64 + 8 * i; };
+  volatile uint32_t* abort_word = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 128);
+
+  pdl_wait();
+  int row0, nodes, prefix;
+  if (!tree_sequence(p, b, row0, nodes, prefix)) return;
+  if (base & 1023) {
+    atomicCAS(p.error, 0, 2);
+    return;
+  }
+  const int trow0 = tile * R;
+  const int trows = min(R, nodes * p.group - trow0);
+  const int end = prefix + nodes;
+  const int p0 = split * p.split_len, p1 = min(end, p0 + p.split_len);
+  if (trows <= 0 || p0 >= p1) return;
+  const int nchunks = (p1 - p0 + C - 1) / C;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kFewStages; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(i)), "r"(kFp8 ? 33 : 1) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty(i)) : "memory");
+    }
+    *abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  auto wait_all = [&](uint32_t bar, uint32_t parity) {
+    return (bool)__all_sync(0xffffffffu, tree_wait(bar, parity, abort_word, p.error));
+  };
+
+  if (warp == kFewWarps) {
+    // ---- producer
+    const int box = min(p.box, C), nbox = C / box;
+    const int* table = kv.block_tables + (size_t)b * kv.max_blocks;
+    auto page_at = [&](int pos) {  // a page id outside the pool is reported and read as page 0
+      if (pos >= p1) return 0;
+      int page = table[pos / kv.ps];
+      if (page < 0 || page >= kv.num_pages) {
+        atomicExch(p.error, 1);
+        page = 0;
+      }
+      return page;
+    };
+    int issued = 0;
+    int next_box = lane < nbox ? page_at(p0 + lane * box) : 0, next_scale = kFp8 ? page_at(p0 + 4 * (lane & 15)) : 0;
+    for (int j = 0; j < nchunks; ++j) {
+      const int st = j % kFewStages, c0 = p0 + j * C;
+      const int page = next_box, spage = next_scale;
+      next_box = lane < nbox ? page_at(c0 + C + lane * box) : 0;  // in flight during the wait
+      if (kFp8) next_scale = page_at(c0 + C + 4 * (lane & 15));
+      if (j >= kFewStages && !wait_all(empty(st), ((j / kFewStages) + 1) & 1)) break;
+      const uint32_t kdst = base + st * kFewStageBytes, vdst = kdst + kFewStageBytes / 2;
+      const int boxes = min(nbox, (p1 - c0 + box - 1) / box);
+      const uint32_t box_bytes = box * (kFp8 ? 64 : 128);
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(st)),
+                     "r"(2 * boxes * box_bytes)
+                     : "memory");
+      __syncwarp();
+      if (lane < boxes) {
+        const int row = (page * kv.NKV + g) * kv.ps + (c0 + lane * box) % kv.ps;
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(kdst + lane * box_bytes),
+            "l"(&tp.tm_k), "r"(full(st)), "r"(0), "r"(row)
+            : "memory");
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4}], [%2];" ::"r"(vdst + lane * box_bytes),
+            "l"(&tp.tm_v), "r"(full(st)), "r"(0), "r"(row)
+            : "memory");
+      }
+      if (kFp8) {  // lanes 0-15 the K scales of four positions each, 16-31 the V scales
+        const int pos = c0 + 4 * (lane & 15);
+        if (pos < p1) {
+          const size_t r = ((size_t)spage * kv.NKV + g) * kv.ps + pos % kv.ps;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + L::kScales + st * 2 * C + 4 * lane),
+                       "l"((lane < 16 ? kv.k_scales : kv.v_scales) + r)
+                       : "memory");
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(st)) : "memory");
+      }
+      ++issued;
+    }
+    // every box issued lands before the CTA may exit (bounded)
+    for (int j = max(0, issued - kFewStages); j < issued; ++j) {
+      const uint64_t t0 = global_ns();
+      while (!mbar_try_wait(reinterpret_cast<uint64_t*>(smem + L::kBars) + j % kFewStages, (j / kFewStages) & 1) &&
+             global_ns() - t0 < 4000000000ull) {
+      }
+    }
+    return;
+  }
+
+  // ---- consumers. Fragment rows of thread (g8, t4): g8 and g8 + 8 of each 16.
+  const int g8 = lane >> 2, t4 = lane & 3;
+  uint32_t qa[MT][4][4];
+  float fac[MT][2];  // scores in powers of two: times this (and, 8-bit, the K scale)
+  const float c2 = p.scale * 1.4426950408889634f;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = mt * 16 + x * 8 + g8, pr = trow0 + r;
+      const bool real = r < trows;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(
+          p.q + ((size_t)(row0 + (real ? pr / p.group : 0)) * p.NQ + g * p.group + (real ? pr % p.group : 0)) * 64);
+      if (!kFp8) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {  // dims 16 kk + 2 t4 (+ 1), and 8 more
+          qa[mt][kk][x] = real ? __ldg(q + 8 * kk + t4) : 0u;
+          qa[mt][kk][2 + x] = real ? __ldg(q + 8 * kk + 4 + t4) : 0u;
+        }
+        fac[mt][x] = c2;
+      } else {
+        // dims 16 t4 + 4 kk (+ 1), and 2 more
+        uint32_t w[8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          w[i] = real ? __ldg(q + 8 * t4 + i) : 0u;
+          top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the largest exponent becomes 14 (an infinity or NaN stays one; a row of zeros may take any factor)
+        const int e = min(max((int)(top >> 7), 30), 254);  // biased
+        const float f = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
+        fac[mt][x] = fmaxf(c2 / f, 1.2e-38f);  // never 0: it meets masked scores of -inf
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t u = w[2 * kk + y];
+            __half2 h = __floats2half2_rn(bf_lo(u) * f, bf_hi(u) * f);
+            qa[mt][kk][2 * y + x] = *reinterpret_cast<uint32_t*>(&h);
+          }
+        }
+      }
+    }
+  }
+  float m[MT][2], l[MT][2], o[MT][8][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt][0] = m[mt][1] = -INFINITY;
+    l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
+  }
+  bool ok = true;
+  for (int j = warp; j < nchunks; j += kFewWarps) {
+    const int st = j % kFewStages;
+    ok = wait_all(full(st), (j / kFewStages) & 1);
+    if (!ok) break;
+#pragma unroll 1
+    for (int sub = 0; sub < C / 32; ++sub) {
+      const int c0 = p0 + j * C + sub * 32;
+      if (c0 >= p1) break;
+      const bool tail = c0 + 32 > prefix;
+      const uint32_t kb = base + st * kFewStageBytes + sub * 32 * (kFp8 ? 64 : 128), vb = kb + kFewStageBytes / 2;
+      const uint8_t* sc = smem + L::kScales + st * 2 * C + sub * 32;  // K scales; V's are C further
+      uint32_t vis[MT][2], dead = 0;  // seen positions; positions without a finite V
+      bool special = tail;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) vis[mt][0] = vis[mt][1] = 0xffffffffu;
+      if (kFp8) special = special || __any_sync(0xffffffffu, sc[lane] == kScaleNaN || sc[C + lane] == kScaleNaN);
+      if (__builtin_expect(tail, 0)) {
+        const int pos = c0 + lane;
+        bool bad = false;
+        if (kFp8) {
+          bad = sc[C + lane] == kScaleNaN;
+        } else if (pos >= prefix && pos < end) {
+          const uint4* v = reinterpret_cast<const uint4*>(smem + (vb - base) + lane * 128);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint4 u = v[c];
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              bad |= (w[e] & 0x7F800000u) == 0x7F800000u || (w[e] & 0x7F80u) == 0x7F80u;
+          }
+        }
+        if (!kFp8 && (pos >= end || bad)) {  // V becomes 0: a masked P of 0 must not meet a NaN
+          uint4* v = reinterpret_cast<uint4*>(smem + (vb - base) + lane * 128);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        bad = bad && pos >= prefix && pos < end;
+        const uint32_t poison = __ballot_sync(0xffffffffu, bad);
+        dead = poison | __ballot_sync(0xffffffffu, pos >= end);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int r = mt * 16 + x * 8 + g8;
+            vis[mt][x] = 0;
+            if (r < trows)
+              vis[mt][x] = (uint32_t)tree_bits(p.mask + (size_t)(row0 + (trow0 + r) / p.group) * p.words, p.words,
+                                               nodes, c0 - prefix);
+            // a row that sees a V that is not finite has no finite result
+            if (vis[mt][x] & poison) l[mt][x] = __uint_as_float(0x7FFFFFFFu);
+          }
+        }
+        __syncwarp();
+      }
+      // ---- scores: four blocks of 8 positions
+      float s[MT][4][4];
+      float sv[4][2];  // 8-bit: V's scales of this thread's columns
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][nb][0] = s[mt][nb][1] = s[mt][nb][2] = s[mt][nb][3] = 0.f;
+        if (!kFp8) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t kf[4];
+            const int r = nb * 8 + (lane & 7), c = hf * 4 + (lane >> 3);
+            few_ldmatrix(kf, kb + r * 128 + ((c ^ (r & 7)) << 4));
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) few_mma<false>(s[mt][nb], qa[mt][hf * 2 + u], kf[2 * u], kf[2 * u + 1]);
+          }
+        } else {
+          const int r = nb * 8 + few_place(g8);
+          const uint4 u = lds128(kb + r * 64 + ((t4 ^ ((r >> 1) & 3)) << 4));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint32_t b0 = few_half2(w[kk], false), b1 = few_half2(w[kk], true);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) few_mma<true>(s[mt][nb], qa[mt][kk], b0, b1);
+          }
+          // the scales of this thread's two columns, out of four neighbouring bytes
+          const uint32_t ks = *reinterpret_cast<const uint32_t*>(sc + nb * 8 + (t4 >> 1) * 4);
+          const uint32_t vs = *reinterpret_cast<const uint32_t*>(sc + C + nb * 8 + (t4 >> 1) * 4);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int byte = e ? 2 + ((t4 & 1) ^ 1) : (t4 & 1);
+            const uint32_t kb8 = (ks >> (8 * byte)) & 255u, vb8 = (vs >> (8 * byte)) & 255u;
+            float kf = __uint_as_float(kb8 << 23), vf = __uint_as_float(vb8 << 23);
+            if (__builtin_expect(special, 0)) {
+              if (kb8 == kScaleNaN) kf = __uint_as_float(0x7FFFFFFFu);
+              if (vb8 == kScaleNaN) vf = __uint_as_float(0x7FFFFFFFu);
+              if ((dead >> (nb * 8 + (t4 >> 1) * 4 + byte)) & 1) vf = 0.f;
+            }
+            sv[nb][e] = vf;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              s[mt][nb][e] *= kf;
+              s[mt][nb][2 + e] *= kf;
+            }
+          }
+        }
+      }
+      if (__builtin_expect(tail, 0)) {
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at = nb * 8 + (kFp8 ? few_place(2 * t4 + e) : 2 * t4 + e);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              if (!((vis[mt][0] >> at) & 1)) s[mt][nb][e] = -INFINITY;
+              if (!((vis[mt][1] >> at) & 1)) s[mt][nb][2 + e] = -INFINITY;
+            }
+          }
+      }
+      // ---- maxima
+      float mx[MT][2];
+      bool grow = false;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float t = -INFINITY;
+#pragma unroll
+          for (int nb = 0; nb < 4; ++nb) t = tree_max3(t, s[mt][nb][2 * x], s[mt][nb][2 * x + 1]);
+          mx[mt][x] = t * fac[mt][x];
+          grow |= mx[mt][x] > m[mt][x] + 8.f;
+        }
+      if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float t = mx[mt][x];  // the row's four lanes agree
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            if (t > m[mt][x] + 8.f) {
+              const float alpha = tree_exp2(m[mt][x] - t);  // 0 for the first maximum
+              m[mt][x] = t;
+              l[mt][x] *= alpha;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                o[mt][i][2 * x] *= alpha;
+                o[mt][i][2 * x + 1] *= alpha;
+              }
+            }
+          }
+      }
+      // ---- probabilities, as the A fragments of P V
+      uint32_t pa[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float mu = m[mt][x] == -INFINITY ? 0.f : m[mt][x];
+#pragma unroll
+          for (int nb = 0; nb < 4; ++nb) {
+            const float e0 = tree_exp2(fmaf(s[mt][nb][2 * x], fac[mt][x], -mu));
+            const float e1 = tree_exp2(fmaf(s[mt][nb][2 * x + 1], fac[mt][x], -mu));
+            l[mt][x] += e0 + e1;
+            __nv_bfloat162 h = kFp8 ? __floats2bfloat162_rn(e0 * sv[nb][0], e1 * sv[nb][1]) : __floats2bfloat162_rn(e0, e1);
+            pa[mt][nb >> 1][(nb & 1) * 2 + x] = *reinterpret_cast<uint32_t*>(&h);
+          }
+        }
+      }
+      // ---- P . V: two steps of 16 positions, eight blocks of 8 dims
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (!kFp8) {
+#pragma unroll
+          for (int dp = 0; dp < 4; ++dp) {
+            uint32_t vf[4];
+            const int r = ks * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), c = dp * 2 + (lane >> 4);
+            few_ldmatrix_t(vf, vb + r * 128 + ((c ^ (r & 7)) << 4));
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][dp * 2 + u], pa[mt][ks], vf[2 * u], vf[2 * u + 1]);
+          }
+        } else {
+          uint2 v[2][2];  // [8 positions][column e]: dims 8 g8 .. 8 g8 + 7 of a position
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = ks * 16 + q * 8 + few_place(2 * t4 + e);
+              const uint32_t at = vb + r * 64 + (((g8 >> 1) ^ ((r >> 1) & 3)) << 4) + (g8 & 1) * 8;
+              asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[q][e].x), "=r"(v[q][e].y) : "r"(at));
+            }
+          const __nv_bfloat162 f = tree_pow2(247);  // 2^120
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            uint32_t bf[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint32_t lo = d < 4 ? v[q][0].x : v[q][0].y, hi = d < 4 ? v[q][1].x : v[q][1].y;
+              const uint32_t w = __byte_perm(lo, hi, (d & 3) << 4 | (4 + (d & 3)) << 12);
+              const uint32_t z = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);
+              const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&z), f);
+              bf[q] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][d], pa[mt][ks], bf[0], bf[1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) tree_arrive(empty(st));
+  }
+
+  // ---- the four warps joined; their states lie over the ring, which nobody reads any more
+  float* state = reinterpret_cast<float*>(smem);  // [warp][R][66]
+  asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float t = l[mt][x];
+      t += __shfl_xor_sync(0xffffffffu, t, 1);
+      t += __shfl_xor_sync(0xffffffffu, t, 2);
+      float* d = state + (warp * R + mt * 16 + x * 8 + g8) * kTreePartial;
+      if (t4 == 0) *reinterpret_cast<float2*>(d) = make_float2(m[mt][x], t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (!kFp8) {  // dims 8 i + 2 t4 (+ 1)
+          *reinterpret_cast<float2*>(d + 2 + 8 * i + 2 * t4) = make_float2(o[mt][i][2 * x], o[mt][i][2 * x + 1]);
+        } else {      // dims 16 t4 + i and 8 more
+          d[2 + 16 * t4 + i] = o[mt][i][2 * x];
+          d[2 + 16 * t4 + 8 + i] = o[mt][i][2 * x + 1];
+        }
+      }
+    }
+  asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
+  if (!ok) return;
+  for (int r = warp; r < trows; r += kFewWarps) {  // a lane has two dims
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, state[(w * R + r) * kTreePartial]);
+    const float mu = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float* d = state + (w * R + r) * kTreePartial;
+      const float a = tree_exp2(d[0] - mu);
+      const float2 v = *reinterpret_cast<const float2*>(d + 2 + 2 * lane);
+      sum = fmaf(d[1], a, sum);
+      o0 = fmaf(v.x, a, o0);
+      o1 = fmaf(v.y, a, o1);
+    }
+    const int pr = trow0 + r;
+    if (p.splits > 1) {
+      float* dst = p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
+      if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(top, sum);
+      *reinterpret_cast<float2*>(dst + 2 + 2 * lane) = make_float2(o0, o1);
+      continue;
+    }
+    const int row = row0 + pr / p.group, head = g * p.group + pr % p.group;
+    const bool any = sum != 0.f;  // NaN counts as something
+    reinterpret_cast<__nv_bfloat162*>(p.out + ((size_t)row * p.NQ + head) * 64)[lane] =
+        __floats2bfloat162_rn(any ? o0 / sum : 0.f, any ? o1 / sum : 0.f);
+    if (p.lse && lane == 0) p.lse[(size_t)row * p.NQ + head] = any ? mu * 0.6931471805599453f + logf(sum) : -INFINITY;
+  }
+}
+
+}  // namespace mk
