@@ -45,23 +45,23 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 
 // Which kernel a call takes and how the positions of a sequence are split over its
 // CTAs. Up to kTreeFewRows rows (nodes x query heads of a K/V head) go to the
-// mma.sync kernel, in one tile of 16 or 32; more to the tcgen05 kernel in tiles of
+// mma.sync kernel, in one tile of 8, 16 or 32; more to the tcgen05 kernel in tiles of
 // 128. A launch of n CTAs, c to an SM, takes about ceil(n / (c SMs)) waves of one
 // range each; a range costs its length and a fixed part (launch, first bytes, the
 // store), and joining ranges a little more; the cheapest length is taken.
 constexpr int kTreeFewRows = 32;
 struct TreePlan {
-  int few;  // row tiles of 16 of the mma.sync kernel, 0: tcgen05
+  int few;  // eights of rows in a tile of the mma.sync kernel (1, 2, 4), 0: tcgen05
   int tiles, splits, len;
 };
 TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
   TreePlan t{};
-  t.few = rows <= 16 ? 1 : rows <= kTreeFewRows ? 2 : 0;
-  const int tile_rows = t.few ? 16 * t.few : mk::kTreeRows;
+  t.few = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= kTreeFewRows ? 4 : 0;
+  const int tile_rows = t.few ? 8 * t.few : mk::kTreeRows;
   t.tiles = (rows + tile_rows - 1) / tile_rows;
   const int unit = mk::kTreeBlock, units = (max_len + unit - 1) / unit;
   const int fixed = t.few ? 2 : 3, join = t.few ? 1 : 2;  // in units
-  const long long ctas = (long long)batch * num_kv_heads * t.tiles, slots = (t.few == 1 ? 3LL : 2LL) * device_sms();
+  const long long ctas = (long long)batch * num_kv_heads * t.tiles, slots = (t.few == 1 ? 4LL : t.few == 2 ? 3LL : 2LL) * device_sms();
   long long best = -1;
   for (int per = units; per >= 1; --per) {
     const int splits = (units + per - 1) / per;
@@ -104,18 +104,19 @@ cudaError_t allow_smem(K kernel, int bytes, bool (&done)[64]) {
   return e;
 }
 
-template <bool kFp8, int MT>
+template <bool kFp8, int RT>
 cudaError_t launch_few(const mk::TreeTmaParams& tp, dim3 grid, cudaStream_t st) {
   static bool done[64];
   constexpr int smem = mk::FewShape<kFp8>::kBytes;
-  if (cudaError_t e = allow_smem(mk::tree_few_kernel<kFp8, MT>, smem, done)) return e;
-  return launch_pdl(mk::tree_few_kernel<kFp8, MT>, grid, dim3((mk::kFewWarps + 1) * 32), smem, st, tp);
+  if (cudaError_t e = allow_smem(mk::tree_few_kernel<kFp8, RT>, smem, done)) return e;
+  return launch_pdl(mk::tree_few_kernel<kFp8, RT>, grid, dim3((mk::kFewWarps + 1) * 32), smem, st, tp);
 }
 
 template <bool kFp8>
 cudaError_t launch_tree(const mk::TreeTmaParams& tp, int few, dim3 grid, cudaStream_t st) {
   if (few == 1) return launch_few<kFp8, 1>(tp, grid, st);
   if (few == 2) return launch_few<kFp8, 2>(tp, grid, st);
+  if (few == 4) return launch_few<kFp8, 4>(tp, grid, st);
   static bool done[64];
   constexpr int smem = mk::TreeSmem<kFp8>::kBytes;
   if (cudaError_t e = allow_smem(mk::tree_attn_kernel<kFp8>, smem, done)) return e;

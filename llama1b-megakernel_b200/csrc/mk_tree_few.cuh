@@ -3,20 +3,23 @@
 //
 // With at most 32 rows (nodes x query heads of a K/V head) a 128-row tensor tile
 // would be mostly empty and its softmax would run on a quarter of the SM, while the
-// work is to stream K and V once. So a tile is MT x 16 rows (MT 1 or 2) on
+// work is to stream K and V once. So a tile is 8, 16 or 32 rows (RT eights) on
 // mma.sync.m16n8k16, whose B operand comes straight from registers:
 //  * four consumer warps take turns at the chunks of the range (32 positions of
 //    bf16, 64 of 8-bit codes: 8 KB either way), each with its own maximum, sum and O,
-//    joined in shared memory at the end; a producer warp keeps eight chunks in
+//    joined in shared memory at the end; a producer warp keeps six chunks in
 //    flight by TMA;
 //  * bf16: fragments by ldmatrix from the 128-byte-swizzled rows, P bf16;
-//  * 8-bit: a thread's K fragment is 16 consecutive codes of a position (one 128-bit
-//    load; the order of dims in a sum is free, so Q is laid out to match), turned
-//    into f16, where every code is exact, by one conversion a pair. Q goes to f16
-//    under a power of two for each row that brings its largest value to 2^14: what
-//    is lost lies below 2^-38 of it. The row's K scale multiplies the score. V
-//    fragments pair two positions of a dim, so their bytes are gathered and moved
-//    into bf16's place (tree_decode); V's scale multiplies P before its rounding.
+//  * 8-bit: all products in f16, where every code is exact and one conversion makes
+//    two of them. A thread's K fragment is 16 consecutive codes of a position (one
+//    128-bit load; the order of dims in a sum is free, so Q is laid out to match);
+//    Q goes to f16 under a power of two for each row that brings its largest value
+//    to 2^14: what is lost lies below 2^-38 of it. The row's K scale multiplies the
+//    score. A V fragment pairs two positions of a dim. V's scales multiply P, relative
+//    to the largest one so far (2^E; O is in units of it, and rescaled when it grows),
+//    so P fits f16, with 2^-12 of rounding. Where some V scale of 32 positions is
+//    below 2^(E - 10), f16 could lose P's low bits: those positions take P and V as
+//    bf16 instead (tree_decode's way), whose range holds everything.
 //    The positions of a block of 8 are permuted between fragment columns and rows
 //    in memory (few_place) so that both loads are free of bank conflicts under the
 //    64-byte swizzle.
@@ -28,7 +31,7 @@
 namespace mk {
 
 constexpr int kFewWarps = 4;
-constexpr int kFewStages = 8;
+constexpr int kFewStages = 6;
 constexpr int kFewStageBytes = 8192;  // K rows, then V rows
 
 template <bool kFp8>
@@ -74,11 +77,13 @@ __device__ __forceinline__ uint32_t few_half2(uint32_t w, bool high) {
   return h;
 }
 
-template <bool kFp8, int MT>
-__global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
+template <bool kFp8, int RT>
+__global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 3 : 2)
     tree_few_kernel(const __grid_constant__ TreeTmaParams tp) {
   using L = FewShape<kFp8>;
-  constexpr int C = L::kChunk, R = 16 * MT;
+  constexpr int C = L::kChunk, R = 8 * RT;
+  constexpr int MT = RT == 4 ? 2 : 1;  // tiles of 16
+  constexpr int X = RT == 1 ? 1 : 2;   // their upper and lower eight rows
   const TreeParams& p = tp.p;
   const KVLayer& kv = p.kv;
   pdl_trigger();
@@ -182,13 +187,14 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
 
   // ---- consumers. Fragment rows of thread (g8, t4): g8 and g8 + 8 of each 16.
   const int g8 = lane >> 2, t4 = lane & 3;
-  uint32_t qa[MT][4][4];
+  const uint32_t pick0 = 0x0444u | (uint32_t)few_place(2 * t4 & 3) << 12, pick1 = 0x0444u | (uint32_t)(few_place((2 * t4 & 3) + 1) & 3) << 12;
+  uint32_t qa[MT][4][4] = {};
   float fac[MT][2];  // scores in powers of two: times this (and, 8-bit, the K scale)
   const float c2 = p.scale * 1.4426950408889634f;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < X; ++x) {
       const int r = mt * 16 + x * 8 + g8, pr = trow0 + r;
       const bool real = r < trows;
       const uint32_t* q = reinterpret_cast<const uint32_t*>(
@@ -235,6 +241,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
   }
+  int top_v = 0;  // 8-bit: O's unit is 2^(top_v - 127)
   bool ok = true;
   for (int j = warp; j < nchunks; j += kFewWarps) {
     const int st = j % kFewStages;
@@ -251,7 +258,25 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
       bool special = tail;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) vis[mt][0] = vis[mt][1] = 0xffffffffu;
-      if (kFp8) special = special || __any_sync(0xffffffffu, sc[lane] == kScaleNaN || sc[C + lane] == kScaleNaN);
+      bool wide = false;  // V's scales span more than f16 holds
+      if (kFp8) {
+        const int vb8 = sc[C + lane];
+        special = special || __any_sync(0xffffffffu, sc[lane] == kScaleNaN || vb8 == kScaleNaN);
+        // positions behind the end, and NaN, do not count
+        const bool counts = c0 + lane < end && vb8 != kScaleNaN;
+        const int most = __reduce_max_sync(0xffffffffu, counts ? vb8 : 0);
+        if (most > top_v) {
+          const float f = top_v ? e8m0_value(max(127 + top_v - most, 1)) : 1.f;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 2 * X; ++e) o[mt][i][e] *= f;
+          top_v = most;
+        }
+        wide = __reduce_min_sync(0xffffffffu, counts ? vb8 : 255) < top_v - 10;
+      }
       if (__builtin_expect(tail, 0)) {
         const int pos = c0 + lane;
         bool bad = false;
@@ -268,10 +293,10 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
               bad |= (w[e] & 0x7F800000u) == 0x7F800000u || (w[e] & 0x7F80u) == 0x7F80u;
           }
         }
-        if (!kFp8 && (pos >= end || bad)) {  // V becomes 0: a masked P of 0 must not meet a NaN
-          uint4* v = reinterpret_cast<uint4*>(smem + (vb - base) + lane * 128);
+        if (pos >= end || bad) {  // V becomes 0: a masked P of 0 must not meet a NaN
+          uint4* v = reinterpret_cast<uint4*>(smem + (vb - base) + lane * (kFp8 ? 64 : 128));
 #pragma unroll
-          for (int c = 0; c < 8; ++c) v[c] = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < (kFp8 ? 4 : 8); ++c) v[c] = make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         bad = bad && pos >= prefix && pos < end;
@@ -280,7 +305,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
+          for (int x = 0; x < X; ++x) {
             const int r = mt * 16 + x * 8 + g8;
             vis[mt][x] = 0;
             if (r < trows)
@@ -293,6 +318,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
         __syncwarp();
       }
       // ---- scores: four blocks of 8 positions
+      const float v_unit = kFp8 ? e8m0_value(max(254 - top_v, 1)) : 1.f;  // 2^(127 - top_v)
       float s[MT][4][4];
       float sv[4][2];  // 8-bit: V's scales of this thread's columns
 #pragma unroll
@@ -325,20 +351,19 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
           const uint32_t vs = *reinterpret_cast<const uint32_t*>(sc + C + nb * 8 + (t4 >> 1) * 4);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int byte = e ? 2 + ((t4 & 1) ^ 1) : (t4 & 1);
-            const uint32_t kb8 = (ks >> (8 * byte)) & 255u, vb8 = (vs >> (8 * byte)) & 255u;
-            float kf = __uint_as_float(kb8 << 23), vf = __uint_as_float(vb8 << 23);
+            // the byte on top, then down by one: a float's exponent
+            const uint32_t kx = __byte_perm(ks, 0, e ? pick1 : pick0) >> 1, vx = __byte_perm(vs, 0, e ? pick1 : pick0) >> 1;
+            float kf = __uint_as_float(kx), vf = __uint_as_float(vx) * v_unit;
             if (__builtin_expect(special, 0)) {
-              if (kb8 == kScaleNaN) kf = __uint_as_float(0x7FFFFFFFu);
-              if (vb8 == kScaleNaN) vf = __uint_as_float(0x7FFFFFFFu);
-              if ((dead >> (nb * 8 + (t4 >> 1) * 4 + byte)) & 1) vf = 0.f;
+              if (kx == 0x7F800000u) kf = __uint_as_float(0x7FFFFFFFu);
+              if (vx == 0x7F800000u) vf = __uint_as_float(0x7FFFFFFFu);
+              if ((dead >> (nb * 8 + few_place(2 * t4 + e))) & 1) vf = 0.f;
             }
             sv[nb][e] = vf;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              s[mt][nb][e] *= kf;
-              s[mt][nb][2 + e] *= kf;
-            }
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int x = 0; x < X; ++x) s[mt][nb][2 * x + e] *= kf;
           }
         }
       }
@@ -350,8 +375,9 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
             const int at = nb * 8 + (kFp8 ? few_place(2 * t4 + e) : 2 * t4 + e);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              if (!((vis[mt][0] >> at) & 1)) s[mt][nb][e] = -INFINITY;
-              if (!((vis[mt][1] >> at) & 1)) s[mt][nb][2 + e] = -INFINITY;
+#pragma unroll
+              for (int x = 0; x < X; ++x)
+                if (!((vis[mt][x] >> at) & 1)) s[mt][nb][2 * x + e] = -INFINITY;
             }
           }
       }
@@ -361,7 +387,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < X; ++x) {
           float t = -INFINITY;
 #pragma unroll
           for (int nb = 0; nb < 4; ++nb) t = tree_max3(t, s[mt][nb][2 * x], s[mt][nb][2 * x + 1]);
@@ -372,7 +398,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
+          for (int x = 0; x < X; ++x) {
             float t = mx[mt][x];  // the row's four lanes agree
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
@@ -389,19 +415,29 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
           }
       }
       // ---- probabilities, as the A fragments of P V
-      uint32_t pa[MT][2][4];
+      uint32_t pa[MT][2][4] = {};
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < X; ++x) {
           const float mu = m[mt][x] == -INFINITY ? 0.f : m[mt][x];
 #pragma unroll
           for (int nb = 0; nb < 4; ++nb) {
-            const float e0 = tree_exp2(fmaf(s[mt][nb][2 * x], fac[mt][x], -mu));
-            const float e1 = tree_exp2(fmaf(s[mt][nb][2 * x + 1], fac[mt][x], -mu));
+            float e0 = tree_exp2(fmaf(s[mt][nb][2 * x], fac[mt][x], -mu));
+            float e1 = tree_exp2(fmaf(s[mt][nb][2 * x + 1], fac[mt][x], -mu));
             l[mt][x] += e0 + e1;
-            __nv_bfloat162 h = kFp8 ? __floats2bfloat162_rn(e0 * sv[nb][0], e1 * sv[nb][1]) : __floats2bfloat162_rn(e0, e1);
-            pa[mt][nb >> 1][(nb & 1) * 2 + x] = *reinterpret_cast<uint32_t*>(&h);
+            uint32_t& a = pa[mt][nb >> 1][(nb & 1) * 2 + x];
+            if (kFp8) {
+              e0 *= sv[nb][0];
+              e1 *= sv[nb][1];
+            }
+            if (!kFp8 || __builtin_expect(wide, 0)) {
+              __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
+              a = *reinterpret_cast<uint32_t*>(&h);
+            } else {
+              __half2 h = __floats2half2_rn(e0, e1);
+              a = *reinterpret_cast<uint32_t*>(&h);
+            }
           }
         }
       }
@@ -429,20 +465,39 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
               const uint32_t at = vb + r * 64 + (((g8 >> 1) ^ ((r >> 1) & 3)) << 4) + (g8 & 1) * 8;
               asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[q][e].x), "=r"(v[q][e].y) : "r"(at));
             }
-          const __nv_bfloat162 f = tree_pow2(247);  // 2^120
+          if (!__builtin_expect(wide, 0)) {
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            uint32_t bf[2];
+            for (int d = 0; d < 8; d += 2) {
+              uint32_t bf[2][2];  // [dim][8 positions]
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const uint32_t lo = d < 4 ? v[q][0].x : v[q][0].y, hi = d < 4 ? v[q][1].x : v[q][1].y;
-              const uint32_t w = __byte_perm(lo, hi, (d & 3) << 4 | (4 + (d & 3)) << 12);
-              const uint32_t z = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);
-              const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&z), f);
-              bf[q] = *reinterpret_cast<const uint32_t*>(&y);
+              for (int q = 0; q < 2; ++q) {
+                const uint32_t lo = d < 4 ? v[q][0].x : v[q][0].y, hi = d < 4 ? v[q][1].x : v[q][1].y;
+                const uint32_t w = __byte_perm(lo, hi, (d & 2) ? 0x7362 : 0x5140);
+                bf[0][q] = few_half2(w, false);
+                bf[1][q] = few_half2(w, true);
+              }
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                few_mma<true>(o[mt][d], pa[mt][ks], bf[0][0], bf[0][1]);
+                few_mma<true>(o[mt][d + 1], pa[mt][ks], bf[1][0], bf[1][1]);
+              }
             }
+          } else {
+            const __nv_bfloat162 f = tree_pow2(247);  // 2^120
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][d], pa[mt][ks], bf[0], bf[1]);
+            for (int d = 0; d < 8; ++d) {
+              uint32_t bf[2];
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const uint32_t lo = d < 4 ? v[q][0].x : v[q][0].y, hi = d < 4 ? v[q][1].x : v[q][1].y;
+                const uint32_t w = __byte_perm(lo, hi, (d & 3) << 4 | (4 + (d & 3)) << 12);
+                const uint32_t z = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);
+                const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&z), f);
+                bf[q] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][d], pa[mt][ks], bf[0], bf[1]);
+            }
           }
         }
       }
@@ -453,11 +508,12 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
 
   // ---- the four warps joined; their states lie over the ring, which nobody reads any more
   float* state = reinterpret_cast<float*>(smem);  // [warp][R][66]
+  const float unit = kFp8 && top_v ? e8m0_value(top_v) : 1.f;
   asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < X; ++x) {
       float t = l[mt][x];
       t += __shfl_xor_sync(0xffffffffu, t, 1);
       t += __shfl_xor_sync(0xffffffffu, t, 2);
@@ -467,9 +523,9 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, MT == 1 ? 3 : 2)
       for (int i = 0; i < 8; ++i) {
         if (!kFp8) {  // dims 8 i + 2 t4 (+ 1)
           *reinterpret_cast<float2*>(d + 2 + 8 * i + 2 * t4) = make_float2(o[mt][i][2 * x], o[mt][i][2 * x + 1]);
-        } else {      // dims 16 t4 + i and 8 more
-          d[2 + 16 * t4 + i] = o[mt][i][2 * x];
-          d[2 + 16 * t4 + 8 + i] = o[mt][i][2 * x + 1];
+        } else {  // in units of V's largest scale; dims 16 t4 + i and 8 more
+          d[2 + 16 * t4 + i] = o[mt][i][2 * x] * unit;
+          d[2 + 16 * t4 + 8 + i] = o[mt][i][2 * x + 1] * unit;
         }
       }
     }
