@@ -123,55 +123,44 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
 
   if (warp == kFewWarps) {
     // ---- producer
-    const int box = min(p.box, C), nbox = C / box;
-    const int* table = kv.block_tables + (size_t)b * kv.max_blocks;
-    auto page_at = [&](int pos) {  // a page id outside the pool is reported and read as page 0
-      if (pos >= p1) return 0;
-      int page = table[pos / kv.ps];
-      if (page < 0 || page >= kv.num_pages) {
-        atomicExch(p.error, 1);
-        page = 0;
-      }
-      return page;
-    };
-    int issued = 0;
-    int next_box = lane < nbox ? page_at(p0 + lane * box) : 0, next_scale = kFp8 ? page_at(p0 + 4 * (lane & 15)) : 0;
+    const int ps = kv.ps, nbox = C / p.box, blks = C / ps, offs = C % ps;
+    TreePages pages(kv, kv.block_tables + (size_t)b * kv.max_blocks, p0, p1, lane, p.error);
+    // the chunk's place, this lane's box's, and its four scales': lanes 0-15 K's, 16-31 V's
+    TreePlace first(p0, ps), box(p0 + lane * p.box, ps), four(p0 + 4 * (lane & 15), ps);
+    const uint32_t box_bytes = p.box * (kFp8 ? 64 : 128);
+    const uint8_t* scale_pool = lane < 16 ? kv.k_scales : kv.v_scales;
+    int issued = 0, st = 0, phase = 1;
     for (int j = 0; j < nchunks; ++j) {
-      const int st = j % kFewStages, c0 = p0 + j * C;
-      const int page = next_box, spage = next_scale;
-      next_box = lane < nbox ? page_at(c0 + C + lane * box) : 0;  // in flight during the wait
-      if (kFp8) next_scale = page_at(c0 + C + 4 * (lane & 15));
-      if (j >= kFewStages && !wait_all(empty(st), ((j / kFewStages) + 1) & 1)) break;
+      const int c0 = p0 + j * C;
+      const int boxes = min(nbox, (p1 - c0 + p.box - 1) / p.box);
+      pages.reach(first.blk);
+      const int row = (pages.page(box.blk, lane < boxes) * kv.NKV + g) * ps + box.off;
+      const bool scales = kFp8 && c0 + 4 * (lane & 15) < p1;
+      const int64_t srow = kFp8 ? ((int64_t)pages.page(four.blk, scales) * kv.NKV + g) * ps + four.off : 0;
+      if (j >= kFewStages && !wait_all(empty(st), phase)) break;
       const uint32_t kdst = base + st * kFewStageBytes, vdst = kdst + kFewStageBytes / 2;
-      const int boxes = min(nbox, (p1 - c0 + box - 1) / box);
-      const uint32_t box_bytes = box * (kFp8 ? 64 : 128);
       if (lane == 0)
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(st)),
                      "r"(2 * boxes * box_bytes)
                      : "memory");
       __syncwarp();
       if (lane < boxes) {
-        const int row = (page * kv.NKV + g) * kv.ps + (c0 + lane * box) % kv.ps;
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-            " [%0], [%1, {%3, %4}], [%2];" ::"r"(kdst + lane * box_bytes),
-            "l"(&tp.tm_k), "r"(full(st)), "r"(0), "r"(row)
-            : "memory");
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-            " [%0], [%1, {%3, %4}], [%2];" ::"r"(vdst + lane * box_bytes),
-            "l"(&tp.tm_v), "r"(full(st)), "r"(0), "r"(row)
-            : "memory");
+        tree_tma(kdst + lane * box_bytes, &tp.tm_k, full(st), row);
+        tree_tma(vdst + lane * box_bytes, &tp.tm_v, full(st), row);
       }
-      if (kFp8) {  // lanes 0-15 the K scales of four positions each, 16-31 the V scales
-        const int pos = c0 + 4 * (lane & 15);
-        if (pos < p1) {
-          const size_t r = ((size_t)spage * kv.NKV + g) * kv.ps + pos % kv.ps;
+      if (kFp8) {
+        if (scales)
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + L::kScales + st * 2 * C + 4 * lane),
-                       "l"((lane < 16 ? kv.k_scales : kv.v_scales) + r)
+                       "l"(scale_pool + srow)
                        : "memory");
-        }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(st)) : "memory");
+        four.advance(blks, offs, ps);
+      }
+      first.advance(blks, offs, ps);
+      box.advance(blks, offs, ps);
+      if (++st == kFewStages) {
+        st = 0;
+        phase ^= 1;
       }
       ++issued;
     }
