@@ -26,6 +26,8 @@
 // O is rescaled when a maximum grew by more than 8 powers of two, as in mk_tree.cuh.
 #pragma once
 
+#include <type_traits>
+
 #include "mk_tree.cuh"
 
 namespace mk {
@@ -45,6 +47,12 @@ struct FewShape {
 // The row within its 8 that fragment column c reads (8-bit): bits (c1 ^ c0, c0, c2).
 __device__ __forceinline__ int few_place(int c) { return (((c >> 1) ^ c) & 1) | ((c & 1) << 1) | (c & 4); }
 
+// Where, in 8-bit V rows, the thread of dims 8 g8 .. 8 g8 + 7 finds the position of column c.
+__device__ __forceinline__ uint32_t few_v_at(int c, int g8) {
+  const int r = few_place(c);
+  return r * 64 + (((g8 >> 1) ^ ((r >> 1) & 3)) << 4) + (g8 & 1) * 8;
+}
+
 __device__ __forceinline__ void few_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -55,18 +63,20 @@ __device__ __forceinline__ void few_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) 
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
+// c = a b + (first ? 0 : c)
 template <bool kHalf>
-__device__ __forceinline__ void few_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void few_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first = false) {
+  const float z0 = first ? 0.f : c[0], z1 = first ? 0.f : c[1], z2 = first ? 0.f : c[2], z3 = first ? 0.f : c[3];
   if constexpr (kHalf) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
   } else {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(z0), "f"(z1), "f"(z2), "f"(z3));
   }
 }
 
@@ -232,41 +242,49 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
   }
   int top_v = 0;  // 8-bit: O's unit is 2^(top_v - 127)
   bool ok = true;
+  // this thread's places in 32 rows of a chunk
+  const uint32_t k_at = kFp8 ? few_place(g8) * 64 + ((t4 ^ ((few_place(g8) >> 1) & 3)) << 4) : (lane & 7) * 128;
+  const uint32_t v_at[2] = {few_v_at(2 * t4, g8), few_v_at(2 * t4 + 1, g8)};
+  const int scale_at = (t4 >> 1) * 4;
+  int st = warp, phase = 0;
+  static_assert(kFewWarps <= kFewStages, "a warp's first chunk is in the ring's first round");
   for (int j = warp; j < nchunks; j += kFewWarps) {
-    const int st = j % kFewStages;
-    ok = wait_all(full(st), (j / kFewStages) & 1);
+    ok = wait_all(full(st), phase);
     if (!ok) break;
-#pragma unroll 1
-    for (int sub = 0; sub < C / 32; ++sub) {
+    bool odd = false, wide = false;  // 8-bit: the chunk has a NaN scale; V's scales span more than f16 holds
+    if (kFp8) {
+      // the scales of positions 2 lane and 2 lane + 1; those behind the end, and NaN, do not count
+      const uint8_t* sc = smem + L::kScales + st * 2 * C;
+      const uint32_t k2 = reinterpret_cast<const uint16_t*>(sc)[lane], v2 = reinterpret_cast<const uint16_t*>(sc + C)[lane];
+      const int v0 = v2 & 255, v1 = v2 >> 8, pos = p0 + j * C + 2 * lane;
+      odd = __any_sync(0xffffffffu, (k2 & 255) == kScaleNaN || (k2 >> 8) == kScaleNaN || v0 == kScaleNaN || v1 == kScaleNaN);
+      const bool in0 = pos < end && v0 != kScaleNaN, in1 = pos + 1 < end && v1 != kScaleNaN;
+      const int most = __reduce_max_sync(0xffffffffu, max(in0 ? v0 : 0, in1 ? v1 : 0));
+      if (most > top_v) {
+        const float f = top_v ? e8m0_value(max(127 + top_v - most, 1)) : 1.f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 2 * X; ++e) o[mt][i][e] *= f;
+        top_v = most;
+      }
+      wide = __reduce_min_sync(0xffffffffu, min(in0 ? v0 : 255, in1 ? v1 : 255)) < top_v - 10;
+    }
+    const float v_unit = kFp8 ? e8m0_value(max(254 - top_v, 1)) : 1.f;  // 2^(127 - top_v)
+    // 32 positions; kPlain: all committed, every scale a number and V's within f16's reach
+    auto step = [&](auto plain, const int sub) {
+      constexpr bool kPlain = decltype(plain)::value;
       const int c0 = p0 + j * C + sub * 32;
-      if (c0 >= p1) break;
-      const bool tail = c0 + 32 > prefix;
+      const bool tail = !kPlain && c0 + 32 > prefix;
       const uint32_t kb = base + st * kFewStageBytes + sub * 32 * (kFp8 ? 64 : 128), vb = kb + kFewStageBytes / 2;
+      const uint8_t* krow = smem + (kb - base);
       const uint8_t* sc = smem + L::kScales + st * 2 * C + sub * 32;  // K scales; V's are C further
       uint32_t vis[MT][2], dead = 0;  // seen positions; positions without a finite V
-      bool special = tail;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) vis[mt][0] = vis[mt][1] = 0xffffffffu;
-      bool wide = false;  // V's scales span more than f16 holds
-      if (kFp8) {
-        const int vb8 = sc[C + lane];
-        special = special || __any_sync(0xffffffffu, sc[lane] == kScaleNaN || vb8 == kScaleNaN);
-        // positions behind the end, and NaN, do not count
-        const bool counts = c0 + lane < end && vb8 != kScaleNaN;
-        const int most = __reduce_max_sync(0xffffffffu, counts ? vb8 : 0);
-        if (most > top_v) {
-          const float f = top_v ? e8m0_value(max(127 + top_v - most, 1)) : 1.f;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-              for (int e = 0; e < 2 * X; ++e) o[mt][i][e] *= f;
-          top_v = most;
-        }
-        wide = __reduce_min_sync(0xffffffffu, counts ? vb8 : 255) < top_v - 10;
-      }
-      if (__builtin_expect(tail, 0)) {
+      if (tail) {
         const int pos = c0 + lane;
         bool bad = false;
         if (kFp8) {
@@ -307,43 +325,38 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
         __syncwarp();
       }
       // ---- scores: four blocks of 8 positions
-      const float v_unit = kFp8 ? e8m0_value(max(254 - top_v, 1)) : 1.f;  // 2^(127 - top_v)
       float s[MT][4][4];
       float sv[4][2];  // 8-bit: V's scales of this thread's columns
 #pragma unroll
       for (int nb = 0; nb < 4; ++nb) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[mt][nb][0] = s[mt][nb][1] = s[mt][nb][2] = s[mt][nb][3] = 0.f;
         if (!kFp8) {
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t kf[4];
-            const int r = nb * 8 + (lane & 7), c = hf * 4 + (lane >> 3);
-            few_ldmatrix(kf, kb + r * 128 + ((c ^ (r & 7)) << 4));
+            few_ldmatrix(kf, kb + k_at + nb * 1024 + (((hf * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) few_mma<false>(s[mt][nb], qa[mt][hf * 2 + u], kf[2 * u], kf[2 * u + 1]);
+              for (int mt = 0; mt < MT; ++mt) few_mma<false>(s[mt][nb], qa[mt][hf * 2 + u], kf[2 * u], kf[2 * u + 1], hf == 0 && u == 0);
           }
         } else {
-          const int r = nb * 8 + few_place(g8);
-          const uint4 u = lds128(kb + r * 64 + ((t4 ^ ((r >> 1) & 3)) << 4));
+          const uint4 u = *reinterpret_cast<const uint4*>(krow + k_at + nb * 512);
           const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
             const uint32_t b0 = few_half2(w[kk], false), b1 = few_half2(w[kk], true);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) few_mma<true>(s[mt][nb], qa[mt][kk], b0, b1);
+            for (int mt = 0; mt < MT; ++mt) few_mma<true>(s[mt][nb], qa[mt][kk], b0, b1, kk == 0);
           }
           // the scales of this thread's two columns, out of four neighbouring bytes
-          const uint32_t ks = *reinterpret_cast<const uint32_t*>(sc + nb * 8 + (t4 >> 1) * 4);
-          const uint32_t vs = *reinterpret_cast<const uint32_t*>(sc + C + nb * 8 + (t4 >> 1) * 4);
+          const uint32_t ks = *reinterpret_cast<const uint32_t*>(sc + scale_at + nb * 8);
+          const uint32_t vs = *reinterpret_cast<const uint32_t*>(sc + scale_at + C + nb * 8);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             // the byte on top, then down by one: a float's exponent
             const uint32_t kx = __byte_perm(ks, 0, e ? pick1 : pick0) >> 1, vx = __byte_perm(vs, 0, e ? pick1 : pick0) >> 1;
             float kf = __uint_as_float(kx), vf = __uint_as_float(vx) * v_unit;
-            if (__builtin_expect(special, 0)) {
+            if (!kPlain && (tail || odd)) {
               if (kx == 0x7F800000u) kf = __uint_as_float(0x7FFFFFFFu);
               if (vx == 0x7F800000u) vf = __uint_as_float(0x7FFFFFFFu);
               if ((dead >> (nb * 8 + few_place(2 * t4 + e))) & 1) vf = 0.f;
@@ -356,7 +369,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
           }
         }
       }
-      if (__builtin_expect(tail, 0)) {
+      if (tail) {
 #pragma unroll
         for (int nb = 0; nb < 4; ++nb)
 #pragma unroll
@@ -383,7 +396,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
           mx[mt][x] = t * fac[mt][x];
           grow |= mx[mt][x] > m[mt][x] + 8.f;
         }
-      if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -420,7 +433,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
               e0 *= sv[nb][0];
               e1 *= sv[nb][1];
             }
-            if (!kFp8 || __builtin_expect(wide, 0)) {
+            if (!kFp8 || (!kPlain && wide)) {
               __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
               a = *reinterpret_cast<uint32_t*>(&h);
             } else {
@@ -450,11 +463,9 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
           for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int r = ks * 16 + q * 8 + few_place(2 * t4 + e);
-              const uint32_t at = vb + r * 64 + (((g8 >> 1) ^ ((r >> 1) & 3)) << 4) + (g8 & 1) * 8;
-              asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[q][e].x), "=r"(v[q][e].y) : "r"(at));
+              v[q][e] = *reinterpret_cast<const uint2*>(krow + kFewStageBytes / 2 + v_at[e] + (ks * 16 + q * 8) * 64);
             }
-          if (!__builtin_expect(wide, 0)) {
+          if (kPlain || !wide) {
 #pragma unroll
             for (int d = 0; d < 8; d += 2) {
               uint32_t bf[2][2];  // [dim][8 positions]
@@ -490,9 +501,23 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
           }
         }
       }
+    };
+#pragma unroll 1
+    for (int sub = 0; sub < C / 32; ++sub) {
+      const int c0 = p0 + j * C + sub * 32;
+      if (c0 >= p1) break;
+      if (c0 + 32 > prefix || odd || wide)
+        step(std::false_type{}, sub);
+      else
+        step(std::true_type{}, sub);
     }
     __syncwarp();
     if (lane == 0) tree_arrive(empty(st));
+    st += kFewWarps;
+    if (st >= kFewStages) {
+      st -= kFewStages;
+      phase ^= 1;
+    }
   }
 
   // ---- the four warps joined; their states lie over the ring, which nobody reads any more
