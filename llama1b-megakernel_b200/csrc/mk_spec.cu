@@ -48,11 +48,14 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 // mma.sync kernel, in one tile of 8, 16 or 32; more to the tcgen05 kernel in tiles of
 // 128. A launch of n CTAs, c to an SM, takes about ceil(n / (c SMs)) waves of one
 // range each; a range costs its length and a fixed part (launch, first bytes, the
-// store), and joining ranges a little more; the cheapest length is taken.
+// store). Joining ranges costs a little in a cluster (up to eight ranges) and a
+// launch and a trip through the workspace otherwise. The cheapest cut is taken.
 constexpr int kTreeFewRows = 32;
+constexpr int kTreeCluster = 8;  // the portable size
 struct TreePlan {
   int few;  // eights of rows in a tile of the mma.sync kernel (1, 2, 4), 0: tcgen05
   int tiles, splits, len;
+  bool cluster() const { return splits > 1 && splits <= kTreeCluster; }
 };
 TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
   TreePlan t{};
@@ -60,13 +63,18 @@ TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
   const int tile_rows = t.few ? 8 * t.few : mk::kTreeRows;
   t.tiles = (rows + tile_rows - 1) / tile_rows;
   const int unit = mk::kTreeBlock, units = (max_len + unit - 1) / unit;
-  const int fixed = t.few ? 2 : 3, join = t.few ? 1 : 2;  // in units
-  const long long ctas = (long long)batch * num_kv_heads * t.tiles, slots = (t.few == 1 ? 4LL : t.few == 2 ? 3LL : 2LL) * device_sms();
+  const int fixed = t.few ? 2 : 3;  // in units, like the costs of a join: 1 and 3
+  const long long ctas = (long long)batch * num_kv_heads * t.tiles;
+  const long long slots = (t.few == 1 ? 4LL : t.few == 2 ? 3LL : 2LL) * device_sms();
   long long best = -1;
-  for (int per = units; per >= 1; --per) {
-    const int splits = (units + per - 1) / per;
+  int last = 0;
+  for (int want = 1; want <= units; ++want) {
+    const int per = (units + want - 1) / want, splits = (units + per - 1) / per;
+    if (splits == last) continue;
+    last = splits;
     const long long waves = (ctas * splits + slots - 1) / slots;
-    const long long cost = waves * (per + fixed) + (splits > 1 ? join : 0);
+    if (best >= 0 && waves > 1 && splits > 4 * kTreeCluster) break;  // finer cuts only add waves
+    const long long cost = waves * (per + fixed) + (splits == 1 ? 0 : splits <= kTreeCluster ? 1 : 3);
     if (best < 0 || cost < best) {
       best = cost;
       t.splits = splits;
@@ -104,12 +112,32 @@ cudaError_t allow_smem(K kernel, int bytes, bool (&done)[64]) {
   return e;
 }
 
+// With programmatic stream serialization, and the ranges of a tile as a cluster where they are one.
+template <typename K>
+cudaError_t launch_ranges(K kernel, const mk::TreeTmaParams& tp, dim3 grid, int threads, int smem, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = tp.p.splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = tp.p.cluster ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, tp);
+}
+
 template <bool kFp8, int RT>
 cudaError_t launch_few(const mk::TreeTmaParams& tp, dim3 grid, cudaStream_t st) {
   static bool done[64];
   constexpr int smem = mk::FewShape<kFp8>::kBytes;
   if (cudaError_t e = allow_smem(mk::tree_few_kernel<kFp8, RT>, smem, done)) return e;
-  return launch_pdl(mk::tree_few_kernel<kFp8, RT>, grid, dim3((mk::kFewWarps + 1) * 32), smem, st, tp);
+  return launch_ranges(mk::tree_few_kernel<kFp8, RT>, tp, grid, (mk::kFewWarps + 1) * 32, smem, st);
 }
 
 template <bool kFp8>
@@ -120,7 +148,7 @@ cudaError_t launch_tree(const mk::TreeTmaParams& tp, int few, dim3 grid, cudaStr
   static bool done[64];
   constexpr int smem = mk::TreeSmem<kFp8>::kBytes;
   if (cudaError_t e = allow_smem(mk::tree_attn_kernel<kFp8>, smem, done)) return e;
-  return launch_pdl(mk::tree_attn_kernel<kFp8>, grid, dim3(mk::kTreeThreads), smem, st, tp);
+  return launch_ranges(mk::tree_attn_kernel<kFp8>, tp, grid, mk::kTreeThreads, smem, st);
 }
 
 // How a row is cut. Chunks of 16 logits a thread, or of one vector where the rows
@@ -225,7 +253,7 @@ int64_t mk_tree_attention_workspace(int32_t batch, int32_t num_q_heads, int32_t 
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_nodes < 1 || max_len < 1) return 0;
   const int group = num_q_heads / num_kv_heads;
   const TreePlan sp = tree_plan(batch, num_kv_heads, max_nodes * group, max_len);
-  if (sp.splits == 1) return 0;
+  if (sp.splits == 1 || sp.cluster()) return 0;
   return (int64_t)batch * num_kv_heads * sp.splits * max_nodes * group * mk::kTreePartial * 4;
 }
 
@@ -273,6 +301,7 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   p.tiles = plan.tiles;
   p.splits = plan.splits;
   p.split_len = plan.len;
+  p.cluster = plan.cluster();
   p.work = static_cast<float*>(workspace);
   const bool fp8 = kv->format == MK_KV_E4M3;
   p.box = !plan.few ? mk::kTreeBlock : fp8 ? mk::FewShape<true>::kChunk : mk::FewShape<false>::kChunk;
@@ -282,7 +311,7 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(p.tiles * p.splits, nkv, batch);
   MK_CUDA(fp8 ? launch_tree<true>(tp, plan.few, grid, st) : launch_tree<false>(tp, plan.few, grid, st));
-  if (p.splits > 1)
+  if (p.splits > 1 && !p.cluster)
     MK_CUDA(launch_pdl(mk::tree_merge_kernel, dim3((max_nodes * group + 7) / 8, nkv, batch), dim3(256), 0, st, p));
   return MK_OK;
 }

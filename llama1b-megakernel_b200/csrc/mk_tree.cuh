@@ -34,8 +34,10 @@
 //    since it was last set: until then p is at most 256, which costs bf16 and fp32
 //    nothing.
 // P is rounded to bf16 (relative 2^-8 at most, unbiased, as V is no more precise
-// itself); its sum is taken before the rounding. A range that is not the whole
-// sequence leaves (m, l, O) in the workspace for tree_merge_kernel.
+// itself); its sum is taken before the rounding. The ranges of a sequence that is
+// split into at most eight are one thread-block cluster, whose CTAs leave (m, l, O)
+// in shared memory and join them there, a share of the rows each (tree_join); more
+// ranges go through the workspace and tree_merge_kernel.
 #pragma once
 
 #include <cuda.h>
@@ -78,6 +80,7 @@ struct TreeParams {
   int rows, words, max_nodes, max_len, NQ, group;
   int box;                          // rows of a TMA box
   int tiles, splits, split_len;     // split_len: a multiple of kTreeBlock
+  int cluster;                      // the ranges of a tile are a cluster (else: partials in work)
   float scale;
   float* work;                      // [batch][NKV][splits][max_nodes * group][kTreePartial]
   __nv_bfloat16* out;               // [rows][NQ][64]
@@ -374,6 +377,65 @@ __device__ __noinline__ unsigned long long tree_bits(const unsigned long long* m
   return sh ? (lo >> sh) | (word(w + 1) << (64 - sh)) : lo;
 }
 
+// The CTA's row tile and range.
+__device__ __forceinline__ void tree_item(const TreeParams& p, int& tile, int& split) {
+  if (p.cluster) {  // a tile's ranges side by side
+    split = blockIdx.x % p.splits;
+    tile = blockIdx.x / p.splits;
+  } else {          // the tiles that read the same positions side by side
+    tile = blockIdx.x % p.tiles;
+    split = blockIdx.x / p.tiles;
+  }
+}
+
+// One row's result, two dims a lane: o not yet divided by the sum.
+__device__ __forceinline__ void tree_write(const TreeParams& p, int row, int head, int lane, float m, float sum, float o0, float o1) {
+  const bool any = sum != 0.f;  // NaN counts as something
+  reinterpret_cast<__nv_bfloat162*>(p.out + ((size_t)row * p.NQ + head) * 64)[lane] =
+      __floats2bfloat162_rn(any ? o0 / sum : 0.f, any ? o1 / sum : 0.f);
+  if (p.lse && lane == 0)
+    p.lse[(size_t)row * p.NQ + head] = any ? (m == -INFINITY ? 0.f : m) * 0.6931471805599453f + logf(sum) : -INFINITY;
+}
+
+// Join the ranges of a cluster: every CTA with a range has its partials
+// [rows][kTreePartial] at shared address `part` (the same in each) and comes here with
+// all its threads; warp `warp` of `warps` takes rows of its own. A CTA without a
+// range, or a warp that has nothing to do, may have left: the barrier only counts
+// threads that have not.
+__device__ __forceinline__ void tree_join(const TreeParams& p, uint32_t part, int ranges, int split, int warp, int warps,
+                                          int lane, int row0, int trow0, int trows, int g) {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  for (int r = split * warps + warp; r < trows; r += ranges * warps) {
+    auto remote = [&](int q) {
+      uint32_t a;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(part + r * kTreePartial * 4), "r"(q));
+      return a;
+    };
+    auto load = [](uint32_t a) {
+      float2 v;
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+      return v;
+    };
+    float m = -INFINITY;
+    for (int q = 0; q < ranges; ++q) m = fmaxf(m, load(remote(q)).x);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int q = 0; q < ranges; ++q) {
+      const uint32_t a = remote(q);
+      const float2 ml = load(a), v = load(a + 8 + 8 * lane);
+      const float f = tree_exp2(ml.x - mu);
+      sum = fmaf(ml.y, f, sum);
+      o0 = fmaf(v.x, f, o0);
+      o1 = fmaf(v.y, f, o1);
+    }
+    const int pr = trow0 + r;
+    tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, m, sum, o0, o1);
+  }
+  __syncwarp();  // nobody leaves while another may still read its partials
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 template <bool kFp8>
 __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid_constant__ TreeTmaParams tp) {
   using L = TreeSmem<kFp8>;
@@ -381,7 +443,9 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const KVLayer& kv = p.kv;
   pdl_trigger();
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, g = blockIdx.y, b = blockIdx.z;
+  const int g = blockIdx.y, b = blockIdx.z;
+  int tile, split;
+  tree_item(p, tile, split);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
   // barriers: full[3], empty[3], ready[3], free[3], q, s[2], p[2], o; then words
@@ -745,7 +809,9 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       const float sum = two ? l * a + other.y * a1 : l * a;
       const bool whole = p.splits == 1, any = sum != 0.f;  // NaN counts as something
       const float f = !whole ? a : any ? a / sum : 0.f, f1 = !whole ? a1 : any ? a1 / sum : 0.f;
-      float* part = p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
+      // in a cluster the partials lie over the blocks, which no copy and no MMA needs any more
+      float* part = p.cluster ? reinterpret_cast<float*>(smem + L::kTiles) + r * kTreePartial
+                              : p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
       if (real && !whole) *reinterpret_cast<float2*>(part) = make_float2(top, sum);
       if (real && whole && p.lse)
         p.lse[(size_t)row * p.NQ + head] = any ? mu * 0.6931471805599453f + logf(sum) : -INFINITY;
@@ -786,6 +852,9 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTreeTmem) : "memory");
   }
+  if (p.cluster)
+    tree_join(p, base + L::kTiles, (end + p.split_len - 1) / p.split_len, split, warp, kTreeThreads / 32, lane, row0, trow0,
+              trows, g);
 }
 
 // One warp per (node, query head): the splits' partials joined, in split order.
@@ -813,11 +882,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     o0 = fmaf(v.x, a, o0);
     o1 = fmaf(v.y, a, o1);
   }
-  const int row = row0 + pr / p.group, head = g * p.group + pr % p.group;
-  const bool any = l != 0.f;
-  reinterpret_cast<__nv_bfloat162*>(p.out + ((size_t)row * p.NQ + head) * 64)[lane] =
-      __floats2bfloat162_rn(any ? o0 / l : 0.f, any ? o1 / l : 0.f);
-  if (p.lse && lane == 0) p.lse[(size_t)row * p.NQ + head] = any ? mu * 0.6931471805599453f + logf(l) : -INFINITY;
+  tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, m, l, o0, o1);
 }
 
 }  // namespace mk

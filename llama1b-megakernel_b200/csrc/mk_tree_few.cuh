@@ -98,7 +98,9 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
   const KVLayer& kv = p.kv;
   pdl_trigger();
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, g = blockIdx.y, b = blockIdx.z;
+  const int g = blockIdx.y, b = blockIdx.z;
+  int tile, split;
+  tree_item(p, tile, split);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
   auto full = [&](int i) { return base + L::kBars + 8 * i; };
@@ -544,8 +546,9 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
       }
     }
   asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
-  if (!ok) return;
-  for (int r = warp; r < trows; r += kFewWarps) {  // a lane has two dims
+  float* joined = state + kFewWarps * R * kTreePartial;  // in a cluster: [R][66], for its other CTAs
+  static_assert((kFewWarps + 1) * R * kTreePartial * 4 <= kFewStages * kFewStageBytes, "the states fit over the ring");
+  for (int r = warp; ok && r < trows; r += kFewWarps) {  // a lane has two dims
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, state[(w * R + r) * kTreePartial]);
@@ -562,17 +565,17 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
     }
     const int pr = trow0 + r;
     if (p.splits > 1) {
-      float* dst = p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
+      float* dst = p.cluster ? joined + r * kTreePartial
+                             : p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
       if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(top, sum);
       *reinterpret_cast<float2*>(dst + 2 + 2 * lane) = make_float2(o0, o1);
-      continue;
+    } else {
+      tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, top, sum, o0, o1);
     }
-    const int row = row0 + pr / p.group, head = g * p.group + pr % p.group;
-    const bool any = sum != 0.f;  // NaN counts as something
-    reinterpret_cast<__nv_bfloat162*>(p.out + ((size_t)row * p.NQ + head) * 64)[lane] =
-        __floats2bfloat162_rn(any ? o0 / sum : 0.f, any ? o1 / sum : 0.f);
-    if (p.lse && lane == 0) p.lse[(size_t)row * p.NQ + head] = any ? mu * 0.6931471805599453f + logf(sum) : -INFINITY;
   }
+  if (p.cluster)
+    tree_join(p, base + kFewWarps * R * kTreePartial * 4, (end + p.split_len - 1) / p.split_len, split, warp, kFewWarps, lane,
+              row0, trow0, trows, g);
 }
 
 }  // namespace mk
