@@ -16,6 +16,10 @@ per-sequence S_MAX:
 
 The kernel writes each new K/V row in place at its position and reads
 positions [0, pos) for attention.
+
+``QuantizedPagedKVCache`` keeps e4m3 codes and a power-of-two scale byte for
+each (position, kv head) instead, 65 bytes a row where bf16 takes 128; the
+operators of ``speculative.py`` read and write both.
 """
 from __future__ import annotations
 
@@ -38,9 +42,7 @@ class PagedKVCache:
             num_pages = max_batch * self.max_blocks
         self.num_pages = num_pages
         self.device = torch.device(device)
-        shape = (cfg.num_layers, num_pages, cfg.num_kv_heads, page_size, cfg.head_dim)
-        self.k_pages = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
-        self.v_pages = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+        self._allocate((cfg.num_layers, num_pages, cfg.num_kv_heads, page_size, cfg.head_dim))
         self.block_tables = torch.full((max_batch, self.max_blocks), -1, dtype=torch.int32,
                                        device=self.device)
         self._host_tables = [[] for _ in range(max_batch)]
@@ -48,6 +50,17 @@ class PagedKVCache:
         self.seq_lens = [0] * max_batch
 
     # ------------------------------------------------------------ allocation
+    def _allocate(self, shape) -> None:
+        self.k_pages = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+        self.v_pages = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+
+    def layer(self, index: int):
+        """Layer ``index`` as the operators of ``speculative.py`` take it (the pools
+        never move, so it stays valid)."""
+        from .speculative import KVLayer
+
+        return KVLayer(self.k_pages[index], self.v_pages[index], self.block_tables)
+
     def reserve(self, seq: int, length: int) -> None:
         """Make positions [0, length) of sequence ``seq`` addressable."""
         if length > self.max_blocks * self.page_size:
@@ -109,3 +122,75 @@ class PagedKVCache:
 
     def nbytes(self) -> int:
         return 2 * self.k_pages.numel() * 2
+
+
+def encode_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows [..., head_dim] as ``mk_kv_write`` stores them in an 8-bit cache: e4m3 codes
+    and the scale bytes [...] (exponent + 127 of the smallest power of two, at
+    least 2^-110, with max|x| <= 448 times it; 255 for a row that is not finite)."""
+    x = x.float()
+    amax = x.abs().amax(-1)
+    finite = torch.isfinite(x).all(-1)
+    amax = torch.where(finite, amax, torch.ones_like(amax))
+    frac, e2 = torch.frexp(amax)
+    e = torch.where(amax > 0, e2 - 9 + (frac > 0.875).to(e2.dtype), torch.full_like(e2, -110)).clamp(min=-110)
+    inv = ((127 - e.to(torch.int32)) << 23).view(torch.float32)  # 2^-e from its bits
+    y = torch.where(finite[..., None], x * inv[..., None], torch.zeros_like(x))
+    byte = torch.where(finite, e.to(torch.int32) + 127, torch.full_like(e, 255, dtype=torch.int32))
+    return y.to(torch.float8_e4m3fn), byte.to(torch.uint8)
+
+
+def decode_rows(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """What codes and scale bytes stand for, in bf16 (exact)."""
+    byte = scales.to(torch.int32)
+    f = (byte << 23).view(torch.float32)
+    f = torch.where(byte == 255, torch.full_like(f, float("nan")), f)
+    return (codes.float() * f[..., None]).to(torch.bfloat16)
+
+
+class QuantizedPagedKVCache(PagedKVCache):
+    """A paged cache of 8-bit rows: ``k_pages`` / ``v_pages`` hold e4m3 codes and
+    ``k_scales`` / ``v_scales`` [num_layers, num_pages, num_kv_heads, page_size] one
+    E8M0 byte per row. No counterpart in the reference, whose cache is bf16
+    (llama_with_megakernel.py:134-139). Read and written by the operators of
+    ``speculative.py``; the persistent kernel and the batched step take the bf16
+    cache."""
+
+    def _allocate(self, shape) -> None:
+        self.k_pages = torch.zeros(shape, dtype=torch.float8_e4m3fn, device=self.device)
+        self.v_pages = torch.zeros(shape, dtype=torch.float8_e4m3fn, device=self.device)
+        self.k_scales = torch.full(shape[:-1], 17, dtype=torch.uint8, device=self.device)
+        self.v_scales = torch.full(shape[:-1], 17, dtype=torch.uint8, device=self.device)
+
+    def layer(self, index: int):
+        from .speculative import KVLayer
+
+        return KVLayer(self.k_pages[index], self.v_pages[index], self.block_tables, self.k_scales[index],
+                       self.v_scales[index])
+
+    def fill(self, seq: int, k_rows: torch.Tensor, v_rows: torch.Tensor) -> None:
+        n = k_rows.shape[2]
+        self.reserve(seq, n)
+        ps, table = self.page_size, self._host_tables[seq]
+        for pool, scales, rows in ((self.k_pages, self.k_scales, k_rows), (self.v_pages, self.v_scales, v_rows)):
+            codes, byte = encode_rows(rows.to(self.device))
+            for blk in range((n + ps - 1) // ps):
+                p0, p1 = blk * ps, min(n, (blk + 1) * ps)
+                pool.view(torch.uint8)[:, table[blk], :, : p1 - p0] = codes.view(torch.uint8)[:, :, p0:p1]
+                scales[:, table[blk], :, : p1 - p0] = byte[:, :, p0:p1]
+        self.seq_lens[seq] = max(self.seq_lens[seq], n)
+
+    def gather(self, seq: int, n: int) -> tuple[torch.Tensor, torch.Tensor]:
+        ps = self.page_size
+        nb = (n + ps - 1) // ps
+        pages = torch.tensor(self._host_tables[seq][:nb], dtype=torch.long, device=self.device)
+        L, _, nkv, _, hd = self.k_pages.shape
+        out = []
+        for pool, scales in ((self.k_pages, self.k_scales), (self.v_pages, self.v_scales)):
+            codes = pool.view(torch.uint8)[:, pages].view(torch.float8_e4m3fn)
+            x = decode_rows(codes, scales[:, pages])
+            out.append(x.permute(0, 2, 1, 3, 4).reshape(L, nkv, nb * ps, hd)[:, :, :n].contiguous())
+        return out[0], out[1]
+
+    def nbytes(self) -> int:
+        return 2 * (self.k_pages.numel() + self.k_scales.numel())

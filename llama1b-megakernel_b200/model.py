@@ -139,6 +139,8 @@ class MegakernelLlamaForCausalLM(torch.nn.Module):
         if kv.num_pages > self.kv.num_pages or kv.max_blocks != self.kv.max_blocks \
                 or kv.page_size != self.page_size:
             raise ValueError("cache geometry differs from the one the model was initialised with")
+        if kv.k_pages.dtype != torch.bfloat16:
+            raise ValueError("this path takes the bf16 cache; 8-bit rows go through speculative.py")
         s = _lib.MkKVCache(k_pages=kv.k_pages.data_ptr(), v_pages=kv.v_pages.data_ptr(),
                            block_tables=kv.block_tables.data_ptr())
         kv._mk_struct = (self, s)  # the pool tensors never move, so the struct stays valid

@@ -53,6 +53,8 @@ def prefill(model, input_ids, past_key_values: PagedKVCache | None = None):
     if getattr(model, "tp_world", 1) != 1:
         raise NotImplementedError("prefill runs on a single-GPU model")
     kv = past_key_values if past_key_values is not None else model.kv
+    if kv.k_pages.dtype != torch.bfloat16:
+        raise ValueError("prefill takes the bf16 cache; 8-bit rows go through speculative.py")
     if isinstance(input_ids, (list, tuple)):
         rows = [torch.as_tensor(r).reshape(-1) for r in input_ids]
     else:

@@ -14,6 +14,10 @@ each one C entry point of ``include/mk.h``:
 * ``token_logprobs``: log probabilities of given tokens, entropy and the most
   likely alternatives of rows of logits.
 
+``SpeculativeDecoder`` runs them together: prompts and drafted trees go through a
+model's layers (the projections, norms and SwiGLU are the batched step's kernels),
+every node is scored for its children, and accepted nodes stay in the cache.
+
 All run asynchronously on the current stream of their tensors' device, allocate
 outputs and workspaces that are not passed in from PyTorch's allocator, and raise
 ``ValueError`` on arguments that do not fit. What only the device can see (a page
@@ -23,10 +27,12 @@ tensor of one zero that the caller reads when it synchronises.
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 
 import torch
 
 from . import _lib
+from .kv_cache import PagedKVCache, QuantizedPagedKVCache
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device index, as a number
@@ -232,3 +238,313 @@ def token_logprobs(logits, targets=None, top: int = 0, logprobs=None, entropy=No
           _check(top_logprobs, _F32, "top_logprobs", index, (rows, top)) if top else None,
           _check(error, _I32, "error", index))
     return logprobs, entropy, top_ids, top_logprobs
+
+
+# ---------------------------------------------------------------- drafts
+class DraftTree:
+    """Drafted tokens of one sequence: ``tokens[i]`` continues ``tokens[parents[i]]``, or
+    the committed sequence where the parent is -1; a parent comes before its
+    children. ``DraftTree.chain(tokens)`` is a plain continuation."""
+
+    def __init__(self, tokens, parents):
+        self.tokens = [int(t) for t in tokens]
+        self.parents = [int(p) for p in parents]
+        if len(self.tokens) != len(self.parents):
+            raise ValueError(f"{len(self.tokens)} tokens, {len(self.parents)} parents")
+        for i, p in enumerate(self.parents):
+            if not -1 <= p < i:
+                raise ValueError(f"node {i}: parent {p} is neither -1 nor a node before it")
+
+    @classmethod
+    def chain(cls, tokens) -> "DraftTree":
+        tokens = list(tokens)
+        return cls(tokens, range(-1, len(tokens) - 1))
+
+    def __len__(self) -> int:
+        return len(self.tokens)
+
+    def depths(self) -> list[int]:
+        out: list[int] = []
+        for p in self.parents:
+            out.append(0 if p < 0 else out[p] + 1)
+        return out
+
+    def masks(self) -> list[int]:
+        """Bit j of node i's mask: j is i or an ancestor of it."""
+        out: list[int] = []
+        for i, p in enumerate(self.parents):
+            out.append((out[p] if p >= 0 else 0) | 1 << i)
+        return out
+
+    def children(self) -> list[list[int]]:
+        """The children of every node, and of the committed sequence at the end of the list."""
+        out: list[list[int]] = [[] for _ in range(len(self) + 1)]
+        for i, p in enumerate(self.parents):
+            out[p].append(i)
+        return out
+
+
+def mask_words(masks: list[int], max_nodes: int) -> torch.Tensor:
+    """Masks as ``tree_attention`` takes them: [nodes, ceil(max_nodes / 64)] int64 (CPU)."""
+    words = (max_nodes + 63) // 64
+    rows = []
+    for m in masks:
+        row = [(m >> (64 * w)) & 0xFFFFFFFFFFFFFFFF for w in range(words)]
+        rows.append([x - (1 << 64) if x >> 63 else x for x in row])
+    return torch.tensor(rows, dtype=torch.int64).reshape(len(masks), words)
+
+
+@dataclass
+class TreeScores:
+    """What a pass over drafted trees gives, a row per node, sequences one after the
+    other (``first[b]`` is sequence b's first row)."""
+
+    first: list[int]
+    logits: torch.Tensor         # [rows, vocab] fp32, after each node
+    child_logprobs: torch.Tensor  # [rows, most children] of the node's children, in order (0: none)
+    entropy: torch.Tensor        # [rows]
+    top_ids: torch.Tensor        # [rows, top]
+    top_logprobs: torch.Tensor   # [rows, top]
+
+
+class SpeculativeDecoder:
+    """Decoding several drafted tokens per pass with the weights of ``model`` (a
+    single-GPU ``MegakernelLlamaForCausalLM``), over a cache of its own: 8-bit rows
+    (``cache="e4m3"``) or bf16.
+
+    ``score`` takes one tree of at most ``max_nodes`` nodes per sequence (128 nodes
+    over all sequences), runs them through the model and returns every node's
+    logits, the log probabilities of its children, its entropy and ``top``
+    alternatives; the nodes' K/V rows then lie behind the committed ones.
+    ``commit`` keeps an accepted path of them, ``accept_greedy`` finds the longest
+    one the model itself would have taken. ``prefill`` runs prompts as causal
+    chains, ``generate`` is greedy decoding with a drafting function."""
+
+    MAX_ROWS = 128  # the GEMM's largest padded row count
+
+    def __init__(self, model, max_batch: int, max_seq_len: int, max_nodes: int = 64, page_size: int = 64,
+                 num_pages: int | None = None, cache: str = "e4m3", top: int = 4):
+        if getattr(model, "tp_world", 1) != 1:
+            raise NotImplementedError("SpeculativeDecoder runs on a single-GPU model")
+        if not 1 <= max_nodes <= self.MAX_ROWS:
+            raise ValueError(f"max_nodes {max_nodes} outside [1, {self.MAX_ROWS}]")
+        if not 1 <= top <= 32:
+            raise ValueError(f"top {top} outside [1, 32]")
+        if max_seq_len > model.rope_len:
+            raise ValueError(f"max_seq_len {max_seq_len} exceeds the model's RoPE table ({model.rope_len} positions)")
+        kinds = {"e4m3": QuantizedPagedKVCache, "bf16": PagedKVCache}
+        if cache not in kinds:
+            raise ValueError(f"cache must be one of {sorted(kinds)}, got {cache!r}")
+        self.m, self.cfg, self.lib, self.dev = model, model.cfg, model.lib, model.device
+        self.max_batch, self.max_seq_len, self.max_nodes, self.top = max_batch, max_seq_len, max_nodes, top
+        self.kv = kinds[cache](self.cfg, max_batch, max_seq_len, page_size, num_pages, device=self.dev)
+        self.layers = [self.kv.layer(i) for i in range(self.cfg.num_layers)]
+        self.err = torch.zeros(1, dtype=torch.int32, device=self.dev)
+        c, z = self.cfg, lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=self.dev)  # noqa: E731
+        R, nh = self.MAX_ROWS, c.num_q_heads + 2 * c.num_kv_heads
+        # the first three feed GEMMs, whose padded rows have to be finite: they start as zeros
+        self._h, self._attn, self._act = z(R, c.hidden), z(R, c.num_q_heads * 64), z(R, c.intermediate)
+        self._qkv, self._q, self._gu = z(R, nh * 64), z(R, c.num_q_heads, 64), z(R, 2 * c.intermediate)
+        self._pending: list[DraftTree | None] = [None] * max_batch
+
+    # ------------------------------------------------------------------ one pass
+    def _gemm(self, w, x, rows, out=None, out_f32=None, residual=None):
+        n, k = w.shape
+        pad = 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128
+        _lib.check(self.lib.mk_gemm_bf16(
+            w.data_ptr(), n, k, x.data_ptr(), rows, pad, residual.data_ptr() if residual is not None else None,
+            out.data_ptr() if out is not None else None, out_f32.data_ptr() if out_f32 is not None else None,
+            None, 0, self.err.data_ptr(), torch.cuda.current_stream(self.dev).cuda_stream))
+
+    @torch.no_grad()
+    def _forward(self, trees: list[DraftTree]) -> torch.Tensor:
+        """The nodes of one tree per sequence through the layers, their K/V behind the
+        committed positions; the residual stream [rows, hidden] after the last."""
+        c, pw, lib, kv, dev = self.cfg, self.m.packed, self.lib, self.kv, self.dev
+        sizes = [len(t) for t in trees]
+        rows = sum(sizes)
+        base = [kv.seq_lens[b] for b in range(len(trees))]
+        for b, n in enumerate(sizes):
+            if base[b] + n > self.max_seq_len:
+                raise ValueError(f"sequence {b}: {base[b]} + {n} positions exceed max_seq_len {self.max_seq_len}")
+            kv.reserve(b, base[b] + n)
+        T = max(sizes)
+        max_len = max(p + n for p, n in zip(base, sizes))
+        seqs = [b for b, n in enumerate(sizes) for _ in range(n)]
+        slots = [base[b] + i for b, n in enumerate(sizes) for i in range(n)]
+        positions = [base[b] + d for b, t in enumerate(trees) for d in t.depths()]
+        tokens = [x for t in trees for x in t.tokens]
+        if min(tokens) < 0 or max(tokens) >= c.vocab:
+            raise ValueError("token id outside the vocabulary")
+        cu = [sum(sizes[:b]) for b in range(len(sizes) + 1)]
+        ints = torch.tensor(tokens + seqs + slots + positions + cu + base, dtype=torch.int32).to(dev)
+        tokens, seqs, slots, positions = (ints[i * rows:(i + 1) * rows] for i in range(4))
+        cu, prefix = ints[4 * rows:4 * rows + len(cu)], ints[4 * rows + len(cu):]
+        mask = mask_words([m for t in trees for m in t.masks()], T).to(dev)
+        st = torch.cuda.current_stream(dev).cuda_stream
+        H, I, eps = c.hidden, c.intermediate, ctypes.c_float(c.rms_eps)
+        x = pw.embed[tokens.long()].contiguous()
+        qkv, q, attn = self._qkv[:rows], self._q[:rows], self._attn[:rows].view(rows, c.num_q_heads, 64)
+        nbytes = lib.mk_tree_attention_workspace(len(trees), c.num_q_heads, c.num_kv_heads, T, max_len)
+        work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        lse = torch.empty(rows, c.num_q_heads, dtype=torch.float32, device=dev)
+        for i, layer in enumerate(self.layers):
+            _lib.check(lib.mk_rmsnorm_rows(x.data_ptr(), pw.norm_attn[i].data_ptr(), eps, rows, H,
+                                           self._h.data_ptr(), st))
+            self._gemm(pw.w_qkv[i].view(-1, H), self._h, rows, out=qkv)
+            kv_write(layer, qkv, pw.rope_cos, pw.rope_sin, seqs, slots, positions, q, error=self.err)
+            tree_attention(q, layer, cu, mask, prefix, T, max_len, scale=c.head_dim ** -0.5, out=attn, lse=lse,
+                           workspace=work, error=self.err)
+            self._gemm(pw.w_o[i], self._attn, rows, out=x, residual=x)
+            _lib.check(lib.mk_rmsnorm_rows(x.data_ptr(), pw.norm_mlp[i].data_ptr(), eps, rows, H,
+                                           self._h.data_ptr(), st))
+            self._gemm(pw.w_gate_up[i].view(2 * I, H), self._h, rows, out=self._gu)
+            _lib.check(lib.mk_swiglu(self._gu.data_ptr(), rows * I, self._act.data_ptr(), st))
+            self._gemm(pw.w_down[i], self._act, rows, out=x, residual=x)
+        return x
+
+    def _logits(self, x: torch.Tensor) -> torch.Tensor:
+        c, pw, rows = self.cfg, self.m.packed, x.shape[0]
+        _lib.check(self.lib.mk_rmsnorm_rows(
+            x.data_ptr(), pw.norm_final.data_ptr(), ctypes.c_float(c.rms_eps), rows, c.hidden, self._h.data_ptr(),
+            torch.cuda.current_stream(self.dev).cuda_stream))
+        logits = torch.empty(rows, c.vocab, dtype=torch.float32, device=self.dev)
+        self._gemm(pw.embed, self._h, rows, out_f32=logits)
+        return logits
+
+    # ------------------------------------------------------------------ API
+    def prefill(self, prompts) -> torch.Tensor:
+        """Commit one prompt per sequence (a list of 1-D token tensors or lists, any
+        lengths), continuing from what each has; returns the fp32 logits [B, vocab]
+        after each prompt's last token."""
+        prompts = [torch.as_tensor(p).reshape(-1).tolist() for p in prompts]
+        if not 1 <= len(prompts) <= self.max_batch or not all(prompts):
+            raise ValueError(f"prefill takes 1 to {self.max_batch} prompts with at least one token each")
+        if any(self._pending):
+            raise ValueError("commit or drop the scored trees first")
+        done = [0] * len(prompts)
+        last = torch.empty(len(prompts), self.cfg.hidden, dtype=torch.bfloat16, device=self.dev)
+        while any(d < len(p) for d, p in zip(done, prompts)):
+            room, trees = self.MAX_ROWS, []
+            for p, d in zip(prompts, done):  # as many rows as the GEMM takes
+                n = min(room, len(p) - d)
+                trees.append(DraftTree.chain(p[d:d + n]))
+                room -= n
+            x = self._forward(trees)
+            at = 0
+            for b, t in enumerate(trees):
+                at += len(t)
+                done[b] += len(t)
+                self.kv.seq_lens[b] += len(t)
+                if len(t) and done[b] == len(prompts[b]):
+                    last[b] = x[at - 1]
+        return self._logits(last)
+
+    def score(self, trees: list[DraftTree]) -> TreeScores:
+        """Run one tree per sequence (at least one node each; usually node 0 is the
+        last accepted token and the rest are drafts) and score it."""
+        if not 1 <= len(trees) <= self.max_batch:
+            raise ValueError(f"{len(trees)} trees for a cache of {self.max_batch} sequences")
+        sizes = [len(t) for t in trees]
+        if min(sizes) < 1 or max(sizes) > self.max_nodes or sum(sizes) > self.MAX_ROWS:
+            raise ValueError(f"trees of {sizes} nodes: 1 to {self.max_nodes} each, {self.MAX_ROWS} together")
+        logits = self._logits(self._forward(trees))
+        kids = [t.children() for t in trees]
+        most = max(1, max(len(k) for ks in kids for k in ks[:-1]))
+        targets = [[t.tokens[j] for j in ks[i]] + [-1] * (most - len(ks[i]))
+                   for t, ks in zip(trees, kids) for i in range(len(t))]
+        targets = torch.tensor(targets, dtype=torch.int32).to(self.dev)
+        lp, ent, ids, top = token_logprobs(logits, targets, min(self.top, self.cfg.vocab), error=self.err)
+        self._pending[:len(trees)] = trees
+        return TreeScores([sum(sizes[:b]) for b in range(len(sizes))], logits, lp, ent, ids, top)
+
+    def commit(self, seq: int, path: list[int]) -> None:
+        """Keep the nodes ``path`` (root first, each the parent of the next) of the tree
+        scored for sequence ``seq``: their rows move to the next positions of the
+        sequence. An empty path drops the tree."""
+        tree = self._pending[seq]
+        if tree is None:
+            raise ValueError(f"sequence {seq} has no scored tree")
+        for i, (node, parent) in enumerate(zip(path, [-1, *path])):
+            if not 0 <= node < len(tree) or tree.parents[node] != parent:
+                raise ValueError(f"path {path}: {node} is not a child of {parent}")
+        kv, ps, base = self.kv, self.kv.page_size, self.kv.seq_lens[seq]
+        moved = [(base + n, base + i) for i, n in enumerate(path) if n != i]
+        if moved:
+            table = kv.pages_of(seq)
+            index = torch.tensor([[table[s // ps], s % ps, table[d // ps], d % ps] for s, d in moved]).to(self.dev)
+            sp, so, dp, do = index.unbind(1)
+            pools = [kv.k_pages, kv.v_pages]
+            if isinstance(kv, QuantizedPagedKVCache):
+                pools = [kv.k_pages.view(torch.uint8), kv.v_pages.view(torch.uint8), kv.k_scales, kv.v_scales]
+            for pool in pools:  # the right side is a copy, so the moves do not meet
+                pool[:, dp, :, do] = pool[:, sp, :, so]
+        kv.seq_lens[seq] += len(path)
+        self._pending[seq] = None
+
+    def accept_greedy(self, scores: TreeScores, seq: int) -> tuple[list[int], int]:
+        """The path of the tree scored for ``seq`` that greedy decoding takes, its first
+        root included, and the token that follows it."""
+        tree = self._pending[seq]
+        if tree is None:
+            raise ValueError(f"sequence {seq} has no scored tree")
+        first = scores.first[seq]
+        best = scores.top_ids[first:first + len(tree), 0].tolist()
+        kids = tree.children()
+        path = [0]
+        while True:
+            nxt = next((j for j in kids[path[-1]] if tree.tokens[j] == best[path[-1]]), None)
+            if nxt is None:
+                return path, best[path[-1]]
+            path.append(nxt)
+
+    def generate(self, prompt, max_new_tokens: int, draft=None) -> tuple[list[int], int]:
+        """Greedy tokens after ``prompt`` (sequence 0, from an empty cache):
+        ``draft(tokens)`` proposes a ``DraftTree`` of continuations of the tokens so
+        far (None or empty: no draft). Returns (tokens, passes)."""
+        if self.kv.seq_lens[0]:
+            raise ValueError("sequence 0 is not empty: release it first")
+        tokens = torch.as_tensor(prompt).reshape(-1).tolist()
+        start = len(tokens)
+        tokens.append(int(self.prefill([tokens])[0].argmax()))
+        passes = 1
+        while len(tokens) - start < max_new_tokens:
+            room = min(self.max_nodes - 1, self.max_seq_len - self.kv.seq_lens[0] - 1)
+            proposal = draft(tokens) if draft is not None else None
+            if proposal is not None and len(proposal) and room > 0:
+                n = min(len(proposal), room)  # parents come first, so a cut tree is a tree
+                tree = DraftTree([tokens[-1], *proposal.tokens[:n]], [-1, *(p + 1 for p in proposal.parents[:n])])
+            else:
+                tree = DraftTree.chain(tokens[-1:])
+            path, following = self.accept_greedy(self.score([tree]), 0)
+            passes += 1
+            tokens += [tree.tokens[i] for i in path[1:]] + [following]
+            self.commit(0, path)
+        self.check()
+        return tokens[start:start + max_new_tokens], passes
+
+    def release(self, seq: int) -> None:
+        """Forget a sequence."""
+        self.kv.release(seq)
+        self._pending[seq] = None
+
+    def check(self) -> None:
+        """Wait for the device and raise ``MkError`` if it reported a failure."""
+        torch.cuda.synchronize(self.dev)
+        code = int(self.err[0])
+        if code:
+            self.err.zero_()
+            what = ("a page id, length or token is out of range" if code == 1 else
+                    f"a device-side wait ran out (code {code})")
+            raise _lib.MkError(_lib.MK_EDEVICE, f"speculative pass: {what}")
+
+
+def lookup_draft(tokens: list[int], longest: int = 3, count: int = 8) -> DraftTree | None:
+    """Draft by looking the last tokens up in what came before: the continuation of
+    the latest earlier occurrence of the last ``longest`` (or fewer) tokens."""
+    for n in range(min(longest, len(tokens) - 1), 0, -1):
+        tail = tokens[-n:]
+        for i in range(len(tokens) - n - 1, -1, -1):
+            if tokens[i:i + n] == tail:
+                return DraftTree.chain(tokens[i + n:i + n + count])
+    return None

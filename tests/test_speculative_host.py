@@ -107,3 +107,51 @@ def test_workspaces_cover_the_call(lib):
         if need:
             assert _logprobs(lib, rows=args[0], vocab=args[1], ld=args[1], top=args[2],
                              ws_bytes=need - 1) == _lib.MK_EINVAL
+
+
+# ------------------------------------------------------------------ host-side parts
+def test_draft_tree():
+    from llama1b_megakernel_b200.speculative import DraftTree, lookup_draft, mask_words
+
+    t = DraftTree([5, 6, 7, 8], [-1, 0, 0, 2])
+    assert t.depths() == [0, 1, 1, 2]
+    assert t.masks() == [1, 0b11, 0b101, 0b1101]
+    assert t.children() == [[1, 2], [], [3], [], [0]]
+    assert DraftTree.chain([4, 4, 4]).parents == [-1, 0, 1] and len(DraftTree.chain([])) == 0
+    for tokens, parents in (([1], [0]), ([1, 2], [-1, 1]), ([1, 2], [-1]), ([1], [-2])):
+        with pytest.raises(ValueError):
+            DraftTree(tokens, parents)
+    w = mask_words([1 << 63, 1 << 64 | 1], 70)
+    assert w.tolist() == [[-(1 << 63), 0], [1, 1]]
+    assert lookup_draft([1, 2, 3, 9, 1, 2, 3]).tokens == [9, 1, 2, 3]
+    assert lookup_draft([1, 2, 3]) is None
+
+
+def test_quantised_cache_rows():
+    """What the 8-bit cache holds of rows: half a code step from them, exact on the way back."""
+    import torch
+
+    from llama1b_megakernel_b200.config import TINY
+    from llama1b_megakernel_b200.kv_cache import QuantizedPagedKVCache, decode_rows, encode_rows
+
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(50, 64, generator=g) * torch.exp(3 * torch.randn(50, 1, generator=g))
+    x[0] = 0
+    x[1, 3] = float("nan")
+    x[2, 5] = float("inf")
+    x[3] = 448.0
+    codes, byte = encode_rows(x)
+    y = decode_rows(codes, byte).double()
+    assert (byte[1:3] == 255).all() and y[1:3].isnan().all() and not y[0].any() and (y[3] == 448).all()
+    amax = x[3:].abs().amax(1).double()
+    scale = 2.0 ** (byte[3:].double() - 127)
+    assert (amax <= 448 * scale).all() and (amax > 224 * scale).all()
+    step = torch.maximum(2.0 ** torch.floor(torch.log2(x[3:].abs().double() / scale[:, None])), torch.tensor(2.0 ** -6)) / 8
+    assert ((y[3:] - x[3:].double()).abs() <= step * scale[:, None] / 2).all()
+    kv = QuantizedPagedKVCache(TINY, max_batch=2, max_seq_len=64, page_size=8, device="cpu")
+    kv.shuffle_free_pages(1)
+    rows = torch.randn(TINY.num_layers, TINY.num_kv_heads, 21, 64, generator=g)
+    kv.fill(1, rows, 2 * rows)
+    k, v = kv.gather(1, 21)
+    assert torch.equal(k, decode_rows(*encode_rows(rows))) and torch.equal(v, decode_rows(*encode_rows(2 * rows)))
+    assert kv.nbytes() == 2 * TINY.num_layers * kv.num_pages * TINY.num_kv_heads * 8 * 65
