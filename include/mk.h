@@ -490,12 +490,12 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
  * MK_F32 or MK_BF16): logprobs [rows][num_targets] of targets (int32; negative:
  * no token, 0 is written), entropy [rows] in nats, and the `top` (0..32) most
  * likely ids with their log probabilities, ties to the lower id. vocab is at most
- * 524,288. Logits of -inf
- * are forbidden tokens. A row of nothing else has log probabilities -inf and
+ * 2^30. Logits of -inf are forbidden tokens. A row of nothing else has log probabilities -inf and
  * entropy 0; one with a NaN or +inf has NaN for both. *error = 1: a target
  * >= vocab (its log probability is NaN). */
 #define MK_F32 0
 #define MK_BF16 1
+/* No workspace is needed (0; `workspace` may be NULL). */
 int64_t mk_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top);
 int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t ld,
                       const int32_t* targets, int32_t num_targets, int32_t top, void* workspace,

@@ -39,6 +39,8 @@ namespace mk {
 constexpr int kLogprobsMaxTop = 32;
 constexpr int kLpThreads = 256;
 constexpr int kLpCandidates = 512;
+constexpr int kLpMaxSlices = 16;  // CTAs of a cluster
+static_assert(kLpMaxSlices * kLogprobsMaxTop <= kLpCandidates, "a cluster's lists fit the candidates");
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct LogprobsParams {
@@ -51,8 +53,6 @@ struct LogprobsParams {
   float* entropy;       // [rows]
   int* top_ids;         // [rows][top]
   float* top_logprobs;  // [rows][top]
-  float* stats;                  // [rows][slices][4] m, s, w (several slices)
-  unsigned long long* lists;     // [rows][slices][top] keys
   int* error;
 };
 
@@ -69,13 +69,8 @@ __device__ __forceinline__ float lp_value(unsigned long long key) {
 }
 __device__ __forceinline__ int lp_id(unsigned long long key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
 
-__device__ __forceinline__ float lp_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 struct LpShared {
+  float4 stats;  // of the CTA's slice, for the first CTA of its cluster
   unsigned long long cand[kLpCandidates];
   unsigned long long list[kLogprobsMaxTop];
   unsigned long long best[8];
@@ -218,7 +213,7 @@ __device__ __forceinline__ void lp_finish(const LogprobsParams& p, const LpShare
 // One slice of a row. Thread t holds E logits of a chunk, in vectors of 16 bytes
 // that neighbouring threads read side by side (kVec: every row starts on 16 bytes).
 template <typename T, int E, bool kVec>
-__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_constant__ LogprobsParams p) {
+__global__ void __launch_bounds__(kLpThreads, sizeof(T) * E >= 64 || (!kVec && E == 16) ? 3 : 4) logprobs_kernel(const __grid_constant__ LogprobsParams p) {
   pdl_trigger();
   pdl_wait();
   __shared__ LpShared sh;
@@ -310,21 +305,26 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
     if (c + 1 < chunks) fetch(c0 + C);
     const float best = largest();
     if (best > m) {
-      const float a = m == -INFINITY ? 0.f : lp_exp2((m - best) * kLog2e);
+      const float a = m == -INFINITY ? 0.f : exp2_approx((m - best) * kLog2e);
       w = m == -INFINITY ? 0.f * s : a * fmaf(m - best, s, w);  // 0 * s: a NaN stays
       s *= a;
       m = best;
     }
     const float mu = m == -INFINITY ? 0.f : m;  // exp(-inf - 0) is 0, and a NaN stays one
-    float sx[4] = {s, 0.f, 0.f, 0.f}, wx[4] = {w, 0.f, 0.f, 0.f};  // chains of their own
+    const float2 shift = make_float2(-mu, -mu), base2 = make_float2(kLog2e, kLog2e);
+    float2 sx[2] = {make_float2(s, 0.f), make_float2(0.f, 0.f)}, wx[2] = {make_float2(w, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float d = v[e] - mu, a = lp_exp2(d * kLog2e);
-      sx[e & 3] += a;
-      wx[e & 3] = fmaf(a, fmaxf(d, -1e30f), wx[e & 3]);  // 0 * -inf adds nothing
+    for (int e = 0; e < E; e += 2) {  // two chains of pairs
+      float2 d = add2(make_float2(v[e], v[e + 1]), shift);
+      const float2 x2 = mul2(d, base2);
+      const float2 a = make_float2(exp2_approx(x2.x), exp2_approx(x2.y));
+      d = make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f));  // 0 * -inf adds nothing
+      const int c = (e >> 1) & 1;
+      sx[c] = add2(sx[c], a);
+      wx[c] = fma2(a, d, wx[c]);
     }
-    s = (sx[0] + sx[1]) + (sx[2] + sx[3]);
-    w = (wx[0] + wx[1]) + (wx[2] + wx[3]);
+    s = (sx[0].x + sx[0].y) + (sx[1].x + sx[1].y);
+    w = (wx[0].x + wx[0].y) + (wx[1].x + wx[1].y);
     if (!p.top) continue;
     if (c == 0) {
       choose(c0);
@@ -361,41 +361,57 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
     next = 2 * (c + 1);
   }
   lp_join(sh, m, s, w);
-  if (p.slices == 1) {
-    lp_finish<T>(p, sh, row, m, s, w);
-    return;
-  }
-  const int64_t at = (int64_t)row * p.slices + slice;
-  if (tid == 0) reinterpret_cast<float4*>(p.stats)[at] = make_float4(m, s, w, 0.f);
-  if (tid < p.top) p.lists[at * p.top + tid] = sh.list[tid];
-}
-
-// A row's slices joined (at most kLpThreads of them), their lists' keys spread over the threads.
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logprobs_join_kernel(const __grid_constant__ LogprobsParams p) {
-  pdl_trigger();
-  pdl_wait();
-  __shared__ LpShared sh;
-  const int row = blockIdx.x, tid = threadIdx.x;
-  float m = -INFINITY, s = 0.f, w = 0.f;
-  if (tid < p.slices) {  // at most kLpThreads slices
-    const float4 st = reinterpret_cast<const float4*>(p.stats)[(int64_t)row * p.slices + tid];
-    m = st.x;
-    s = st.y;
-    w = st.z;
-  }
-  lp_join(sh, m, s, w);
-  if (p.top) {
-    const unsigned long long* lists = p.lists + (int64_t)row * p.slices * p.top;
-    const int n = p.slices * p.top;
-    float best = -INFINITY;
-    for (int i = tid; i < n; i += kLpThreads) {
-      const unsigned long long k = __ldg(lists + i);
-      if (k) best = fmaxf(best, lp_value(k));
+  if (p.slices > 1) {
+    if (tid == 0) sh.stats = make_float4(m, s, w, 0.f);
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (slice == 0) {
+      auto remote = [&](const void* at, int q) {
+        uint32_t a;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(at)), "r"(q));
+        return a;
+      };
+      auto key_of = [&](int q, int i) {
+        unsigned long long k;
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(remote(&sh.list[i], q)) : "memory");
+        return k;
+      };
+      m = -INFINITY;
+      s = w = 0.f;
+      if (tid < p.slices) {
+        float unused;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(m), "=f"(s), "=f"(w), "=f"(unused)
+                     : "r"(remote(&sh.stats, tid))
+                     : "memory");
+      }
+      // a slice's list alone has `top` keys that reach its last: whatever is below the
+      // largest of the lasts is out, and little more than `top` keys are left to rank
+      unsigned long long key[kLpMaxSlices * kLogprobsMaxTop / kLpThreads], least = 0;
+      const int n = p.slices * p.top;
+#pragma unroll
+      for (int c = 0; c < kLpMaxSlices * kLogprobsMaxTop / kLpThreads; ++c) {
+        const int i = c * kLpThreads + tid;
+        key[c] = i < n ? key_of(i / p.top, i % p.top) : 0;
+        if (i < n && i % p.top == p.top - 1) least = max(least, key[c]);
+      }
+      for (int o = 16; o; o >>= 1) least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
+      if ((tid & 31) == 0) sh.best[tid >> 5] = least;
+      if (tid == 0) sh.count = 0;
+      lp_join(sh, m, s, w);  // and a barrier for the lines above
+#pragma unroll
+      for (int i = 0; i < 8; ++i) least = max(least, sh.best[i]);
+      least = max(least, 1ull);
+      __syncthreads();
+      if (tid < kLogprobsMaxTop) sh.list[tid] = 0;  // the keys of this CTA's own list are in registers
+#pragma unroll
+      for (int c = 0; c < kLpMaxSlices * kLogprobsMaxTop / kLpThreads; ++c)
+        if (key[c] >= least) sh.cand[atomicAdd(&sh.count, 1)] = key[c];
+      __syncthreads();
+      lp_rank(sh, p.top, sh.count);
     }
-    lp_select(sh, p.top, best, [&](float, auto f) {
-      for (int i = tid; i < n; i += kLpThreads) f(__ldg(lists + i));
-    });
+    // nobody leaves while its list may still be read
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (slice) return;
   }
   lp_finish<T>(p, sh, row, m, s, w);
 }

@@ -151,45 +151,71 @@ cudaError_t launch_tree(const mk::TreeTmaParams& tp, int few, dim3 grid, cudaStr
   return launch_ranges(mk::tree_attn_kernel<kFp8>, tp, grid, mk::kTreeThreads, smem, st);
 }
 
-// How a row is cut. Chunks of 16 logits a thread, or of one vector where the rows
-// have too few of those to give every SM work. A slice costs its chunks and about
-// kLpFixedChunks more (the choice of alternatives, the join); an SM's share is that
-// times the slices that fall to it, and the cut with the least is taken.
-constexpr int kLpMaxVocab = mk::kLpThreads * mk::kLpThreads * 8;  // the join takes a slice per thread
-constexpr int kLpFixedChunks = 2;
+// How a row is cut: chunks of 16 logits a thread or of one vector, and slices of
+// whole chunks. In quarters of a 16-logit chunk's time, a slice costs what it reads,
+// about kLpFixed for the first choice of alternatives and the join, and kLpRank for
+// each later ranking (after 2, 4, 8 ... chunks); an SM's share is that times the slices
+// that fall to it, and the cut with the least is taken. The slices of a row are a
+// cluster; more than the portable eight only for a few rows, which cannot fill the
+// GPU otherwise.
+constexpr int kLpMaxVocab = 1 << 30;
+constexpr int kLpFixed = 8, kLpRank = 2;
 struct LpCut {
   int per, slices, len;
 };
 LpCut lp_cut(int rows, int vocab, int vector) {
-  const int sms = device_sms();
-  auto chunks = [&](int per) { return (vocab + mk::kLpThreads * per - 1) / (mk::kLpThreads * per); };
-  int per = 16;
-  if ((long long)rows * chunks(per) < 2LL * sms && chunks(vector) <= mk::kLpThreads) per = vector;
-  const int n = chunks(per);
-  int each = n, slices = 1;
+  const int sms = device_sms(), most = rows <= 8 ? mk::kLpMaxSlices : 8;
+  LpCut best{};
   long long least = -1;
-  for (int want = 1; want <= std::min(n, mk::kLpThreads); ++want) {
-    const int e = (n + want - 1) / want, k = (n + e - 1) / e;
-    const long long cost = (((long long)rows * k + sms - 1) / sms) * (e + kLpFixedChunks);
-    if (k <= mk::kLpThreads && (least < 0 || cost < least)) {
-      least = cost;
-      each = e;
-      slices = k;
+  for (int per : {16, vector}) {
+    const int n = (int)(((long long)vocab + mk::kLpThreads * per - 1) / (mk::kLpThreads * per));
+    for (int want = 1; want <= std::min(n, most); ++want) {
+      const int e = (n + want - 1) / want, k = (n + e - 1) / e;
+      int ranks = 0;
+      while ((1 << ranks) < e) ++ranks;
+      const long long cost = (((long long)rows * k + sms - 1) / sms) * ((long long)e * per / 4 + kLpFixed + kLpRank * ranks);
+      if (least < 0 || cost < least) {
+        least = cost;
+        best = {per, k, e * mk::kLpThreads * per};
+      }
     }
   }
-  return {per, slices, each * mk::kLpThreads * per};
+  return best;
 }
 
-template <typename T, int E>
-cudaError_t launch_logprobs_e(const mk::LogprobsParams& p, bool vec, cudaStream_t st) {
-  return launch_pdl(vec ? mk::logprobs_kernel<T, E, true> : mk::logprobs_kernel<T, E, false>, dim3(p.slices, p.rows),
-                    dim3(mk::kLpThreads), 0, st, p);
+template <typename T, int E, bool kVec>
+cudaError_t launch_logprobs_k(const mk::LogprobsParams& p, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.slices, p.rows);
+  cfg.blockDim = dim3(mk::kLpThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.slices;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.slices > 1 ? 2 : 1;
+  if (p.slices > 8) {
+    static bool done[64];
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    if (dev >= 64 || !done[dev]) {
+      cudaError_t e = cudaFuncSetAttribute(mk::logprobs_kernel<T, E, kVec>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+      if (dev < 64) done[dev] = true;
+    }
+  }
+  return cudaLaunchKernelEx(&cfg, mk::logprobs_kernel<T, E, kVec>, p);
 }
 
 template <typename T>
 cudaError_t launch_logprobs(const mk::LogprobsParams& p, int per, bool vec, cudaStream_t st) {
   constexpr int N = 16 / (int)sizeof(T);
-  return per == N ? launch_logprobs_e<T, N>(p, vec, st) : launch_logprobs_e<T, 16>(p, vec, st);
+  if (per == N) return vec ? launch_logprobs_k<T, N, true>(p, st) : launch_logprobs_k<T, N, false>(p, st);
+  return vec ? launch_logprobs_k<T, 16, true>(p, st) : launch_logprobs_k<T, 16, false>(p, st);
 }
 
 }  // namespace
@@ -317,10 +343,10 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
 }
 
 int64_t mk_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top) {
-  if (rows < 1 || vocab < 1 || vocab > kLpMaxVocab || top < 0 || top > mk::kLogprobsMaxTop) return 0;
-  // either type's slices
-  const int64_t slices = std::max(lp_cut(rows, vocab, 4).slices, lp_cut(rows, vocab, 8).slices);
-  return slices == 1 ? 0 : (int64_t)rows * slices * (16 + 8 * top);
+  (void)rows;
+  (void)vocab;
+  (void)top;
+  return 0;  // a row's slices meet in distributed shared memory
 }
 
 int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t ld,
@@ -336,10 +362,8 @@ int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t v
     return fail(MK_EINVAL, "top %d must be in [0, min(%d, vocab)] and needs top_ids and top_logprobs", top,
                 mk::kLogprobsMaxTop);
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == MK_F32 ? 4 : 2)) return fail(MK_EINVAL, "logits are not aligned to their type");
-  const int64_t need = mk_token_logprobs_workspace(rows, vocab, top);
-  if (need > 0 && !aligned16(workspace)) return fail(MK_EINVAL, "the workspace must be 16-byte aligned");
-  if (need > 0 && (!workspace || workspace_bytes < need))
-    return fail(MK_EINVAL, "workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
+  (void)workspace;
+  (void)workspace_bytes;
   if (rows == 0) return MK_OK;
   mk::LogprobsParams p{};
   p.logits = logits;
@@ -359,8 +383,6 @@ int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t v
   const LpCut cut = lp_cut(rows, vocab, 16 / size);
   p.slices = cut.slices;
   p.slice_len = cut.len;
-  p.stats = static_cast<float*>(workspace);
-  p.lists = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(workspace) + (int64_t)rows * p.slices * 16);
   const bool vec = aligned16(logits) && (rows == 1 || (ld * size) % 16 == 0);
   // rows go in launches of at most 65,535 (the grid's second dimension)
   for (int r0 = 0; r0 < rows; r0 += 65535) {
@@ -374,9 +396,6 @@ int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t v
     q.top_ids += (int64_t)r0 * top;
     q.top_logprobs += (int64_t)r0 * top;
     MK_CUDA(dtype == MK_F32 ? launch_logprobs<float>(q, cut.per, vec, st) : launch_logprobs<__nv_bfloat16>(q, cut.per, vec, st));
-    if (p.slices > 1)
-      MK_CUDA(launch_pdl(dtype == MK_F32 ? mk::logprobs_join_kernel<float> : mk::logprobs_join_kernel<__nv_bfloat16>,
-                         dim3((unsigned)n), dim3(mk::kLpThreads), 0, st, q));
   }
   return MK_OK;
 }

@@ -318,29 +318,6 @@ __device__ __forceinline__ void tree_st16(uint32_t taddr, const uint32_t (&v)[16
       : "memory");
 }
 
-__device__ __forceinline__ float tree_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ float2 tree_fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(*reinterpret_cast<unsigned long long*>(&d))
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
-        "l"(*reinterpret_cast<unsigned long long*>(&c)));
-  return d;
-}
-__device__ __forceinline__ float2 tree_add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(*reinterpret_cast<unsigned long long*>(&d))
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
-  return d;
-}
-
 // Four e4m3 codes as bf16: {d0, d2} and {d1, d3}. A code s eeee mmm moved into
 // bf16's place for (exponent, mantissa) is its value times 2^(7 - 127), its
 // subnormals becoming bf16's, so one exact multiplication by 2^120 and the row's
@@ -424,7 +401,7 @@ __device__ __forceinline__ void tree_join(const TreeParams& p, uint32_t part, in
     for (int q = 0; q < ranges; ++q) {
       const uint32_t a = remote(q);
       const float2 ml = load(a), v = load(a + 8 + 8 * lane);
-      const float f = tree_exp2(ml.x - mu);
+      const float f = exp2_approx(ml.x - mu);
       sum = fmaf(ml.y, f, sum);
       o0 = fmaf(v.x, f, o0);
       o1 = fmaf(v.y, f, o1);
@@ -752,7 +729,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       mx *= c2;
       const bool grow = mx > m + 8.f;
       if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
-        const float alpha = grow ? tree_exp2(m - mx) : 1.f;  // 0 for the first maximum
+        const float alpha = grow ? exp2_approx(m - mx) : 1.f;  // 0 for the first maximum
         if (grow) m = mx;
         l *= alpha;
         if (j > 0) {
@@ -776,12 +753,12 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float2 x = make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
-          x = tree_fma2(x, scale2, shift2);
-          x = make_float2(tree_exp2(x.x), tree_exp2(x.y));
+          x = fma2(x, scale2, shift2);
+          x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
           if (i & 1) {
-            s1 = tree_add2(s1, x);
+            s1 = add2(s1, x);
           } else {
-            s0 = tree_add2(s0, x);
+            s0 = add2(s0, x);
           }
           __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
           w[i] = *reinterpret_cast<uint32_t*>(&h);
@@ -805,7 +782,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       const bool two = halves > 1;
       const float m1 = two ? other.x : -INFINITY;
       const float top = fmaxf(m, m1), mu = top == -INFINITY ? 0.f : top;
-      const float a = tree_exp2(m - mu), a1 = tree_exp2(m1 - mu);
+      const float a = exp2_approx(m - mu), a1 = exp2_approx(m1 - mu);
       const float sum = two ? l * a + other.y * a1 : l * a;
       const bool whole = p.splits == 1, any = sum != 0.f;  // NaN counts as something
       const float f = !whole ? a : any ? a / sum : 0.f, f1 = !whole ? a1 : any ? a1 / sum : 0.f;
@@ -876,7 +853,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     const float* q = src + s * stride;
-    const float a = tree_exp2(q[0] - mu);
+    const float a = exp2_approx(q[0] - mu);
     const float2 v = *reinterpret_cast<const float2*>(q + 2 + 2 * lane);
     l = fmaf(q[1], a, l);
     o0 = fmaf(v.x, a, o0);

@@ -407,7 +407,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
             if (t > m[mt][x] + 8.f) {
-              const float alpha = tree_exp2(m[mt][x] - t);  // 0 for the first maximum
+              const float alpha = exp2_approx(m[mt][x] - t);  // 0 for the first maximum
               m[mt][x] = t;
               l[mt][x] *= alpha;
 #pragma unroll
@@ -427,8 +427,8 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
           const float mu = m[mt][x] == -INFINITY ? 0.f : m[mt][x];
 #pragma unroll
           for (int nb = 0; nb < 4; ++nb) {
-            float e0 = tree_exp2(fmaf(s[mt][nb][2 * x], fac[mt][x], -mu));
-            float e1 = tree_exp2(fmaf(s[mt][nb][2 * x + 1], fac[mt][x], -mu));
+            float e0 = exp2_approx(fmaf(s[mt][nb][2 * x], fac[mt][x], -mu));
+            float e1 = exp2_approx(fmaf(s[mt][nb][2 * x + 1], fac[mt][x], -mu));
             l[mt][x] += e0 + e1;
             uint32_t& a = pa[mt][nb >> 1][(nb & 1) * 2 + x];
             if (kFp8) {
@@ -557,7 +557,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
 #pragma unroll
     for (int w = 0; w < kFewWarps; ++w) {
       const float* d = state + (w * R + r) * kTreePartial;
-      const float a = tree_exp2(d[0] - mu);
+      const float a = exp2_approx(d[0] - mu);
       const float2 v = *reinterpret_cast<const float2*>(d + 2 + 2 * lane);
       sum = fmaf(d[1], a, sum);
       o0 = fmaf(v.x, a, o0);

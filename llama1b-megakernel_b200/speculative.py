@@ -188,7 +188,7 @@ def tree_attention(q, layer: KVLayer, cu_nodes, mask, prefix_lens, max_nodes: in
 
 
 def token_logprobs(logits, targets=None, top: int = 0, logprobs=None, entropy=None, top_ids=None,
-                   top_logprobs=None, workspace=None, error=None):
+                   top_logprobs=None, error=None):
     """From ``logits`` [rows, vocab] (fp32 or bf16; rows may be strided): the log
     probabilities of ``targets`` [rows, n] (int32, negative: no token, 0), the
     entropy of every row in nats, and the ``top`` (<= 32) most likely ids with
@@ -221,17 +221,8 @@ def token_logprobs(logits, targets=None, top: int = 0, logprobs=None, entropy=No
     if top_logprobs is None:
         top_logprobs = logits.new_empty((rows, top), dtype=_F32)
     error = _error_word(error, logits.device)
-    lib = _lib.load()
-    if workspace is None:
-        nbytes = lib.mk_token_logprobs_workspace(rows, vocab, top)
-        wp = 0
-        if nbytes:
-            workspace = logits.new_empty(nbytes, dtype=_U8)
-            wp = workspace.data_ptr()
-    else:
-        wp, nbytes = _check(workspace, _U8, "workspace", index), workspace.numel()
-    _call(lib.mk_token_logprobs, index, logits.data_ptr(), dtype, rows, vocab, ld,
-          _check(targets, _I32, "targets", index, (rows, n)) if n else None, n, top, wp, nbytes,
+    _call(_lib.load().mk_token_logprobs, index, logits.data_ptr(), dtype, rows, vocab, ld,
+          _check(targets, _I32, "targets", index, (rows, n)) if n else None, n, top, None, 0,
           _check(logprobs, _F32, "logprobs", index, (rows, n)) if n else None,
           _check(entropy, _F32, "entropy", index, (rows,)),
           _check(top_ids, _I32, "top_ids", index, (rows, top)) if top else None,
