@@ -44,6 +44,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "mk_device.cuh"
 #include "mk_kv8.cuh"
 
@@ -454,6 +456,9 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int nblocks = (p1 - p0 + kTreeBlock - 1) / kTreeBlock;
   const int halves = (p1 - p0 + kTreeHalf - 1) / kTreeHalf;
   const int active = (trows + 31) >> 5;  // softmax warps with a row
+  // blocks from here on reach past the committed positions; before it a bf16 block
+  // goes from memory to the tensor cores untouched
+  const int tails = kFp8 ? 0 : min(nblocks, max(prefix - p0, 0) / kTreeBlock);
 
   if (threadIdx.x == 0) {
     auto init = [](uint32_t bar, uint32_t n) {
@@ -549,8 +554,11 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     constexpr uint32_t id_s = tree_idesc(kTreeHalf, false), id_o = tree_idesc(64, true);
     const uint64_t dq = tree_desc(base + L::kQ);
     int slot = 0, next = 0, next_phase = 0;  // the block's slot; the next one's, and its phase
+    int ahead = 0;                           // the next one's number
     auto scores = [&](int half) {
-      if (!half && !wait_all(ready(next), next_phase)) return false;
+      if (!half && !(ahead < tails ? wait_all(full(next), next_phase)
+                                   : wait_all(ready(next), kFp8 ? next_phase : ((ahead - tails) / L::kReady) & 1)))
+        return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       tree_mma_scores(t_s(half), dq, tree_desc(slot_at(next) + half * (kTreeHalf * 128)), id_s);
       tree_commit(b_s(half));
@@ -558,6 +566,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     };
     bool ok = wait_all(b_q, 0) && scores(0) && (halves < 2 || scores(1));
     for (int j = 0; j < nblocks && ok; ++j) {
+      ++ahead;
       if (++next == L::kReady) {
         next = 0;
         next_phase ^= 1;
@@ -584,8 +593,8 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     // ---- block warps, one thread per position
     const int r = threadIdx.x - 256;
     static_assert(L::kStages == L::kReady, "one slot counter for both rings");
-    int rd = 0, phase = 0;
-    for (int j = 0; j < nblocks; ++j) {
+    int rd = tails % L::kReady, phase = (tails / L::kReady) & 1;
+    for (int j = tails; j < nblocks; ++j) {
       const int st = rd, c0 = p0 + j * kTreeBlock, pos = c0 + r;
       const bool tail = c0 + kTreeBlock > prefix;
       const bool drafted = pos >= prefix && pos < end;
@@ -684,93 +693,90 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     const uint32_t s_at = t_s(half) + tl, o_at = t_o(half) + tl;
     const float c2 = p.scale * 1.4426950408889634f;  // scores in powers of two
     float m = -INFINITY, l = 0.f;  // m: the reference maximum, in powers of two
-    int rd = 0, rd_phase = 0;      // the block's ready slot
     const int mine = (halves + 1 - half) >> 1;
     bool ok = true;
-    for (int j = 0; j < mine; ++j) {
-      const int c0 = p0 + j * kTreeBlock + half * kTreeHalf;
-      const bool tail = c0 + kTreeHalf > prefix;
+    // one half block; kTail: it reaches past the committed positions
+    auto step = [&](auto kind, const int j) {
+      constexpr bool kTail = decltype(kind)::value;
       unsigned long long vis = ~0ull;
-      if (__builtin_expect(tail, 0)) {
-        vis = tree_bits(p.mask + (size_t)row * p.words, p.words, nodes, c0 - prefix);
-        ok = wait_all(ready(rd), rd_phase);
-        if (!ok) break;
+      if constexpr (kTail) {
+        const int rd = j % L::kReady;
+        vis = tree_bits(p.mask + (size_t)row * p.words, p.words, nodes, p0 + j * kTreeBlock + half * kTreeHalf - prefix);
+        if (!wait_all(ready(rd), ((j - tails) / L::kReady) & 1)) return false;
         // a row that sees a V that is not finite has no finite result
         if (vis & (bad[rd * 4 + 2 * half] | (unsigned long long)bad[rd * 4 + 2 * half + 1] << 32))
           l = __uint_as_float(0x7FFFFFFFu);
       }
-      if (++rd == L::kReady) {
-        rd = 0;
-        rd_phase ^= 1;
-      }
-      ok = wait_all(b_s(half), j & 1);
-      if (!ok) break;
+      if (!wait_all(b_s(half), j & 1)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      auto load = [&](int c, uint32_t (&raw)[32]) {
-        tree_ld32(s_at + 32 * c, raw);
-        if (__builtin_expect(tail, 0)) {
-          const uint32_t v = (uint32_t)(vis >> (32 * c));
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(v & (1u << i))) raw[i] = 0xFF800000u;  // -inf
-        }
-      };
-      float mx = -INFINITY;
+      // the probabilities under the maximum so far; where a row's has grown by more
+      // than 8 powers of two (or is the first), once more under the new one
+      uint32_t w[2][16];
+      float2 s0, s1;
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t raw[32];
-        load(c, raw);
-        float x[4] = {mx, __uint_as_float(raw[0]), __uint_as_float(raw[1]), -INFINITY};
+      for (int attempt = 0;; ++attempt) {
+        const float mu = m == -INFINITY ? 0.f : m;
+        const float2 scale2 = make_float2(c2, c2), shift2 = make_float2(-mu, -mu);
+        float top[2] = {-INFINITY, -INFINITY};
+        s0 = s1 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 2; i < 32; i += 2)
-          x[(i >> 1) & 3] = tree_max3(x[(i >> 1) & 3], __uint_as_float(raw[i]), __uint_as_float(raw[i + 1]));
-        mx = tree_max3(tree_max3(x[0], x[1], x[2]), x[3], -INFINITY);
-      }
-      mx *= c2;
-      const bool grow = mx > m + 8.f;
-      if (__builtin_expect(__any_sync(0xffffffffu, grow), 0)) {
-        const float alpha = grow ? exp2_approx(m - mx) : 1.f;  // 0 for the first maximum
-        if (grow) m = mx;
-        l *= alpha;
+        for (int c = 0; c < 2; ++c) {
+          uint32_t raw[32];
+          tree_ld32(s_at + 32 * c, raw);
+          if constexpr (kTail) {
+            const uint32_t v = (uint32_t)(vis >> (32 * c));
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(v & (1u << i))) raw[i] = 0xFF800000u;  // -inf
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 x = make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
+            x = fma2(x, scale2, shift2);
+            top[i & 1] = tree_max3(top[i & 1], x.x, x.y);
+            x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+            if (i & 1) {
+              s1 = add2(s1, x);
+            } else {
+              s0 = add2(s0, x);
+            }
+            __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+            w[c][i] = *reinterpret_cast<uint32_t*>(&h);
+          }
+        }
+        const float mx = fmaxf(top[0], top[1]);
+        const bool grow = mx > 8.f || m == -INFINITY;
+        if (attempt || __builtin_expect(!__any_sync(0xffffffffu, grow), 1)) break;
+        const float to = grow ? mx + mu : m;
+        const float alpha = grow ? exp2_approx(m - to) : 1.f;  // 0 for the first maximum
+        if (to != -INFINITY) l *= alpha;
+        m = to;
         if (j > 0) {
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t w[16];
-            tree_ld16(o_at + 16 * c, w);
+            uint32_t o[16];
+            tree_ld16(o_at + 16 * c, o);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
-            tree_st16(o_at + 16 * c, w);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * (m == -INFINITY ? 1.f : alpha));
+            tree_st16(o_at + 16 * c, o);
           }
         }
-      }
-      const float mu = m == -INFINITY ? 0.f : m;
-      const float2 scale2 = make_float2(c2, c2), shift2 = make_float2(-mu, -mu);
-      float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {  // P of the first 32 scores goes over scores already used, and so on
-        uint32_t raw[32], w[16];
-        load(c, raw);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float2 x = make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
-          x = fma2(x, scale2, shift2);
-          x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-          if (i & 1) {
-            s1 = add2(s1, x);
-          } else {
-            s0 = add2(s0, x);
-          }
-          __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
-          w[i] = *reinterpret_cast<uint32_t*>(&h);
-        }
-        tree_st16(s_at + 16 * c, w);
       }
       l += (s0.x + s0.y) + (s1.x + s1.y);
+      tree_st16(s_at, w[0]);  // P over S
+      tree_st16(s_at + 16, w[1]);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) tree_arrive(b_p(half));
-    }
+      return true;
+    };
+    const int plain = min(mine, max(prefix - p0 - half * kTreeHalf + kTreeHalf, 0) / kTreeBlock);
+    int j = 0;
+#pragma unroll 1
+    for (; j < plain && ok; ++j) ok = step(std::false_type{}, j);
+#pragma unroll 1
+    for (; j < mine && ok; ++j) ok = step(std::true_type{}, j);
     // ---- the two softmaxes joined: the second's (m, l) by way of shared memory
     if (ok) ok = wait_all(b_o, 0);  // no MMA reads Q any more
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
