@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     if (ok) {
       const uint2* c = reinterpret_cast<const uint2*>(p.cos_t + (size_t)pos * 64) + l;
       const uint2* s = reinterpret_cast<const uint2*>(p.sin_t + (size_t)pos * 64) + l;
-      const uint2 c0 = __ldg(c), c1 = __ldg(c + 8), s0 = __ldg(s), s1 = __ldg(s + 8);
+      const uint2 c0 = c[0], c1 = c[8], s0 = s[0], s1 = s[8];
       const float cl[4] = {bf_lo(c0.x), bf_hi(c0.x), bf_lo(c0.y), bf_hi(c0.y)};
       const float ch[4] = {bf_lo(c1.x), bf_hi(c1.x), bf_lo(c1.y), bf_hi(c1.y)};
       const float sl[4] = {bf_lo(s0.x), bf_hi(s0.x), bf_lo(s0.y), bf_hi(s0.y)};

@@ -56,7 +56,7 @@ struct LogprobsParams {
   int* error;
 };
 
-__device__ __forceinline__ float lp_load(const float* x, int64_t i) { return __ldg(x + i); }
+__device__ __forceinline__ float lp_load(const float* x, int64_t i) { return x[i]; }
 __device__ __forceinline__ float lp_load(const __nv_bfloat16* x, int64_t i) { return __bfloat162float(x[i]); }
 
 // (logit, id) as one integer that orders as the alternatives do; -0 counts as 0.
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kLpThreads, sizeof(T) * E >= 64 || (!kVec && E
     if (kVec && c0 + C <= i1) {
 #pragma unroll
       for (int c = 0; c < E / N; ++c) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + c0) + c * kLpThreads + tid);
+        const uint4 u = (reinterpret_cast<const uint4*>(x + c0))[c * kLpThreads + tid];
         raw[4 * c] = u.x;
         raw[4 * c + 1] = u.y;
         raw[4 * c + 2] = u.z;

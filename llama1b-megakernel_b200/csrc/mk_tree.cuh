@@ -122,12 +122,13 @@ __device__ __forceinline__ uint32_t tree_try(uint32_t bar, uint32_t parity) {
   return ok;
 }
 
-// Wait with a limit of 2 s. A wait that runs out reports error 2 and raises the
+// Wait with a limit: 2 s and a thousand looks, so that neither a pause of the whole
+// GPU nor a timer that steps back is taken for a wait that ran out. One that did reports error 2 and raises the
 // CTA's abort word, on which every other wait of the CTA gives up. The waiting is
 // kept out of the roles' loops, which have to stay in the instruction cache.
 __device__ __noinline__ bool tree_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_word, int* error) {
   uint64_t t0 = 0;
-  for (;;) {
+  for (uint32_t looks = 0;; ++looks) {
     // asleep until the phase ends, 1 ms at most: warps that poll take issue slots from the softmax
     uint32_t ok;
     asm volatile(
@@ -142,7 +143,7 @@ __device__ __noinline__ bool tree_wait_slow(uint32_t bar, uint32_t parity, volat
     const uint64_t now = global_ns();
     if (!t0) {
       t0 = now;
-    } else if (now - t0 > 2000000000ull) {
+    } else if (looks >= 1000 && (int64_t)(now - t0) > 2000000000ll) {
       *abort_word = 1;
       atomicCAS(error, 0, 2);
       return false;
@@ -162,11 +163,11 @@ struct TreePages {
   const int* table;
   int count, ps, num_pages, base, cur, nxt, lane;
   int* error;
-  __device__ __forceinline__ int window(int w) const { return w + lane < count ? __ldg(table + w + lane) : 0; }
-  // positions [p0, p1) of the sequence behind `table_`
-  __device__ __forceinline__ TreePages(const KVLayer& kv, const int* table_, int p0, int p1, int lane_, int* error_)
-      : table(table_), count((p1 + kv.ps - 1) / kv.ps), ps(kv.ps), num_pages(kv.num_pages), base(p0 / kv.ps), lane(lane_),
-        error(error_) {
+  __device__ __forceinline__ int window(int w) const { return lane < count - w ? table[w + lane] : 0; }
+  // sequence b from position p0 on; its length need not be known yet
+  __device__ __forceinline__ TreePages(const KVLayer& kv, int b, int p0, int lane_, int* error_)
+      : table(kv.block_tables + (size_t)b * kv.max_blocks), count(kv.max_blocks), ps(kv.ps), num_pages(kv.num_pages),
+        base(p0 / kv.ps), lane(lane_), error(error_) {
     cur = window(base);
     nxt = window(base + 32);
   }
@@ -441,7 +442,25 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   volatile uint32_t* abort_word = words;      // words[1]: TMEM base
   volatile uint32_t* bad = words + 4;         // [kReady][4] drafted positions whose V is not finite
 
+  auto init = [](uint32_t bar, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+  };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 3; ++i) {
+      init(full(i), kFp8 ? 33 : 1);   // the expected bytes; each producer lane's scale bytes
+      init(empty(i), kFp8 ? 4 : 1);   // the block warps have read the codes; P V has read the rows
+      init(ready(i), 4);
+      init(free_(i), 1);
+    }
+    init(b_s(0), 1);
+    init(b_s(1), 1);
+    init(b_o, 1);
+    *abort_word = 0;
+  }
+  const int p0 = split * p.split_len;
   pdl_wait();
+  // the producer's first page ids and the sequence's lengths are on their way together
+  TreePages pages(kv, b, p0, warp == 12 ? lane : 1 << 30, p.error);
   int row0, nodes, prefix;
   if (!tree_sequence(p, b, row0, nodes, prefix)) return;
   if (base & 1023) {  // the swizzled layouts count on it
@@ -451,39 +470,25 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int trow0 = tile * kTreeRows;  // first row (node * group + head) of the tile
   const int trows = min(kTreeRows, nodes * p.group - trow0);
   const int end = prefix + nodes;
-  const int p0 = split * p.split_len, p1 = min(end, p0 + p.split_len);
+  const int p1 = min(end, p0 + p.split_len);
   if (trows <= 0 || p0 >= p1) return;
+  if (warp == 13) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 148),
+                 "r"(kTreeTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   const int nblocks = (p1 - p0 + kTreeBlock - 1) / kTreeBlock;
   const int halves = (p1 - p0 + kTreeHalf - 1) / kTreeHalf;
   const int active = (trows + 31) >> 5;  // softmax warps with a row
   // blocks from here on reach past the committed positions; before it a bf16 block
   // goes from memory to the tensor cores untouched
   const int tails = kFp8 ? 0 : min(nblocks, max(prefix - p0, 0) / kTreeBlock);
-
   if (threadIdx.x == 0) {
-    auto init = [](uint32_t bar, uint32_t n) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n) : "memory");
-    };
-    for (int i = 0; i < 3; ++i) {
-      init(full(i), kFp8 ? 33 : 1);   // the expected bytes; each producer lane's scale bytes
-      init(empty(i), kFp8 ? 4 : 1);   // the block warps have read the codes; P V has read the rows
-      init(ready(i), 4);
-      init(free_(i), 1);
-    }
     init(b_q, active);
-    for (int i = 0; i < 2; ++i) {
-      init(b_s(i), 1);
-      init(b_p(i), active);
-    }
-    init(b_o, 1);
-    *abort_word = 0;
+    init(b_p(0), active);
+    init(b_p(1), active);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 13) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 148),
-                 "r"(kTreeTmem)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -501,7 +506,6 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   if (warp == 12) {
     // ---- producer
     const int ps = kv.ps, nbox = kTreeBlock / p.box, blks = kTreeBlock / ps, offs = kTreeBlock % ps;
-    TreePages pages(kv, kv.block_tables + (size_t)b * kv.max_blocks, p0, p1, lane, p.error);
     TreePlace first(p0, ps), box(p0 + lane * p.box, ps), four(p0 + 4 * lane, ps);  // the block's, this lane's box's, its four scales'
     const uint32_t box_bytes = p.box * (kFp8 ? 64 : 128);
     int issued = 0, st = 0, phase = 1;
@@ -679,7 +683,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       uint8_t* dst = smem + L::kQ + r * 128;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        uint4 u = real ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        uint4 u = real ? src[c] : make_uint4(0, 0, 0, 0);
         if (kFp8)  // the order of dims that tree_decode leaves: 0, 2, 1, 3
           u = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632),
                          __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
@@ -709,8 +713,26 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       }
       if (!wait_all(b_s(half), j & 1)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (j == 0) {  // the first maximum
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t raw[32];
+          tree_ld32(s_at + 32 * c, raw);
+          const uint32_t v = (uint32_t)(vis >> (32 * c));
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            if (kTail) {
+              if (!(v & (1u << i))) raw[i] = 0xFF800000u;  // -inf
+              if (!(v & (2u << i))) raw[i + 1] = 0xFF800000u;
+            }
+            top[(i >> 1) & 1] = tree_max3(top[(i >> 1) & 1], __uint_as_float(raw[i]), __uint_as_float(raw[i + 1]));
+          }
+        }
+        m = fmaxf(top[0], top[1]) * c2;
+      }
       // the probabilities under the maximum so far; where a row's has grown by more
-      // than 8 powers of two (or is the first), once more under the new one
+      // than 8 powers of two (or only now has one), once more under the new one
       uint32_t w[2][16];
       float2 s0, s1;
 #pragma unroll 1

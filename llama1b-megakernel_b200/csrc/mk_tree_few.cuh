@@ -107,19 +107,6 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
   auto empty = [&](int i) { return base + L::kBars + 64 + 8 * i; };
   volatile uint32_t* abort_word = reinterpret_cast<volatile uint32_t*>(smem + L::kBars + 128);
 
-  pdl_wait();
-  int row0, nodes, prefix;
-  if (!tree_sequence(p, b, row0, nodes, prefix)) return;
-  if (base & 1023) {
-    atomicCAS(p.error, 0, 2);
-    return;
-  }
-  const int trow0 = tile * R;
-  const int trows = min(R, nodes * p.group - trow0);
-  const int end = prefix + nodes;
-  const int p0 = split * p.split_len, p1 = min(end, p0 + p.split_len);
-  if (trows <= 0 || p0 >= p1) return;
-  const int nchunks = (p1 - p0 + C - 1) / C;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kFewStages; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(i)), "r"(kFp8 ? 33 : 1) : "memory");
@@ -129,6 +116,22 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
+  const int p0 = split * p.split_len;
+  pdl_wait();
+  // the producer's first page ids and the sequence's lengths are on their way together
+  TreePages pages(kv, b, p0, warp == kFewWarps ? lane : 1 << 30, p.error);
+  int row0, nodes, prefix;
+  if (!tree_sequence(p, b, row0, nodes, prefix)) return;
+  if (base & 1023) {
+    atomicCAS(p.error, 0, 2);
+    return;
+  }
+  const int trow0 = tile * R;
+  const int trows = min(R, nodes * p.group - trow0);
+  const int end = prefix + nodes;
+  const int p1 = min(end, p0 + p.split_len);
+  if (trows <= 0 || p0 >= p1) return;
+  const int nchunks = (p1 - p0 + C - 1) / C;
   auto wait_all = [&](uint32_t bar, uint32_t parity) {
     return (bool)__all_sync(0xffffffffu, tree_wait(bar, parity, abort_word, p.error));
   };
@@ -136,7 +139,6 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
   if (warp == kFewWarps) {
     // ---- producer
     const int ps = kv.ps, nbox = C / p.box, blks = C / ps, offs = C % ps;
-    TreePages pages(kv, kv.block_tables + (size_t)b * kv.max_blocks, p0, p1, lane, p.error);
     // the chunk's place, this lane's box's, and its four scales': lanes 0-15 K's, 16-31 V's
     TreePlace first(p0, ps), box(p0 + lane * p.box, ps), four(p0 + 4 * (lane & 15), ps);
     const uint32_t box_bytes = p.box * (kFp8 ? 64 : 128);
@@ -203,8 +205,8 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
       if (!kFp8) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {  // dims 16 kk + 2 t4 (+ 1), and 8 more
-          qa[mt][kk][x] = real ? __ldg(q + 8 * kk + t4) : 0u;
-          qa[mt][kk][2 + x] = real ? __ldg(q + 8 * kk + 4 + t4) : 0u;
+          qa[mt][kk][x] = real ? q[8 * kk + t4] : 0u;
+          qa[mt][kk][2 + x] = real ? q[8 * kk + 4 + t4] : 0u;
         }
         fac[mt][x] = c2;
       } else {
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          w[i] = real ? __ldg(q + 8 * t4 + i) : 0u;
+          w[i] = real ? q[8 * t4 + i] : 0u;
           top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
