@@ -377,16 +377,19 @@ __device__ __forceinline__ void tree_write(const TreeParams& p, int row, int hea
     p.lse[(size_t)row * p.NQ + head] = any ? (m == -INFINITY ? 0.f : m) * 0.6931471805599453f + logf(sum) : -INFINITY;
 }
 
-// Join the ranges of a cluster: every CTA with a range has its partials
-// [rows][kTreePartial] at shared address `part` (the same in each) and comes here with
-// all its threads; warp `warp` of `warps` takes rows of its own. A CTA without a
-// range, or a warp that has nothing to do, may have left: the barrier only counts
-// threads that have not.
-__device__ __forceinline__ void tree_join(const TreeParams& p, uint32_t part, int ranges, int split, int warp, int warps,
-                                          int lane, int row0, int trow0, int trows, int g) {
+__device__ __forceinline__ void tree_cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  for (int r = split * warps + warp; r < trows; r += ranges * warps) {
+}
+
+// Join the ranges of a cluster: every CTA with a range has its partials
+// [rows][kTreePartial] at shared address `part` (the same in each); the first `warps`
+// warps take rows of their own. All threads of all CTAs of the cluster pass its two
+// barriers, those without a range in tree_leave.
+__device__ __forceinline__ void tree_join(const TreeParams& p, uint32_t part, int ranges, int split, int warp, int warps,
+                                          int lane, int row0, int trow0, int trows, int g) {
+  tree_cluster_sync();
+  for (int r = warp < warps ? split * warps + warp : trows; r < trows; r += ranges * warps) {
     auto remote = [&](int q) {
       uint32_t a;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(part + r * kTreePartial * 4), "r"(q));
@@ -412,8 +415,15 @@ __device__ __forceinline__ void tree_join(const TreeParams& p, uint32_t part, in
     const int pr = trow0 + r;
     tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, m, sum, o0, o1);
   }
-  __syncwarp();  // nobody leaves while another may still read its partials
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  tree_cluster_sync();  // nobody leaves while another may still read its partials
+}
+
+// A CTA whose sequence ends before its range.
+__device__ __forceinline__ void tree_leave(const TreeParams& p) {
+  if (p.cluster) {
+    tree_cluster_sync();
+    tree_cluster_sync();
+  }
 }
 
 template <bool kFp8>
@@ -471,7 +481,8 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int trows = min(kTreeRows, nodes * p.group - trow0);
   const int end = prefix + nodes;
   const int p1 = min(end, p0 + p.split_len);
-  if (trows <= 0 || p0 >= p1) return;
+  if (trows <= 0) return;
+  if (p0 >= p1) return tree_leave(p);
   if (warp == 13) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kBars + 148),
                  "r"(kTreeTmem)

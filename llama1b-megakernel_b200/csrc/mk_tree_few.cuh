@@ -7,7 +7,7 @@
 // mma.sync.m16n8k16, whose B operand comes straight from registers:
 //  * four consumer warps take turns at the chunks of the range (32 positions of
 //    bf16, 64 of 8-bit codes: 8 KB either way), each with its own maximum, sum and O,
-//    joined in shared memory at the end; a producer warp keeps six chunks in
+//    joined in shared memory at the end; a producer warp keeps eight chunks in
 //    flight by TMA;
 //  * bf16: fragments by ldmatrix from the 128-byte-swizzled rows, P bf16;
 //  * 8-bit: all products in f16, where every code is exact and one conversion makes
@@ -33,7 +33,11 @@
 namespace mk {
 
 constexpr int kFewWarps = 4;
-constexpr int kFewStages = 6;
+constexpr int kFewStages = 8;
+// A stage is always the same warp's, who has then waited for each of its phases. With
+// another number a warp may come to a stage that others filled and drained since it
+// last looked; a parity then does not tell the phase it waits for from the one before it.
+static_assert(kFewStages % kFewWarps == 0, "a stage belongs to one warp");
 constexpr int kFewStageBytes = 8192;  // K rows, then V rows
 
 template <bool kFp8>
@@ -130,7 +134,8 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
   const int trows = min(R, nodes * p.group - trow0);
   const int end = prefix + nodes;
   const int p1 = min(end, p0 + p.split_len);
-  if (trows <= 0 || p0 >= p1) return;
+  if (trows <= 0) return;
+  if (p0 >= p1) return tree_leave(p);
   const int nchunks = (p1 - p0 + C - 1) / C;
   auto wait_all = [&](uint32_t bar, uint32_t parity) {
     return (bool)__all_sync(0xffffffffu, tree_wait(bar, parity, abort_word, p.error));
@@ -185,394 +190,392 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
              global_ns() - t0 < 4000000000ull) {
       }
     }
-    return;
-  }
-
-  // ---- consumers. Fragment rows of thread (g8, t4): g8 and g8 + 8 of each 16.
-  const int g8 = lane >> 2, t4 = lane & 3;
-  const uint32_t pick0 = 0x0444u | (uint32_t)few_place(2 * t4 & 3) << 12, pick1 = 0x0444u | (uint32_t)(few_place((2 * t4 & 3) + 1) & 3) << 12;
-  uint32_t qa[MT][4][4] = {};
-  float fac[MT][2];  // scores in powers of two: times this (and, 8-bit, the K scale)
-  const float c2 = p.scale * 1.4426950408889634f;
+  } else {
+    // ---- consumers. Fragment rows of thread (g8, t4): g8 and g8 + 8 of each 16.
+    const int g8 = lane >> 2, t4 = lane & 3;
+    const uint32_t pick0 = 0x0444u | (uint32_t)few_place(2 * t4 & 3) << 12, pick1 = 0x0444u | (uint32_t)(few_place((2 * t4 & 3) + 1) & 3) << 12;
+    uint32_t qa[MT][4][4] = {};
+    float fac[MT][2];  // scores in powers of two: times this (and, 8-bit, the K scale)
+    const float c2 = p.scale * 1.4426950408889634f;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+    for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-    for (int x = 0; x < X; ++x) {
-      const int r = mt * 16 + x * 8 + g8, pr = trow0 + r;
-      const bool real = r < trows;
-      const uint32_t* q = reinterpret_cast<const uint32_t*>(
-          p.q + ((size_t)(row0 + (real ? pr / p.group : 0)) * p.NQ + g * p.group + (real ? pr % p.group : 0)) * 64);
-      if (!kFp8) {
+      for (int x = 0; x < X; ++x) {
+        const int r = mt * 16 + x * 8 + g8, pr = trow0 + r;
+        const bool real = r < trows;
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(
+            p.q + ((size_t)(row0 + (real ? pr / p.group : 0)) * p.NQ + g * p.group + (real ? pr % p.group : 0)) * 64);
+        if (!kFp8) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {  // dims 16 kk + 2 t4 (+ 1), and 8 more
-          qa[mt][kk][x] = real ? q[8 * kk + t4] : 0u;
-          qa[mt][kk][2 + x] = real ? q[8 * kk + 4 + t4] : 0u;
-        }
-        fac[mt][x] = c2;
-      } else {
-        // dims 16 t4 + 4 kk (+ 1), and 2 more
-        uint32_t w[8];
-        uint32_t top = 0;
+          for (int kk = 0; kk < 4; ++kk) {  // dims 16 kk + 2 t4 (+ 1), and 8 more
+            qa[mt][kk][x] = real ? q[8 * kk + t4] : 0u;
+            qa[mt][kk][2 + x] = real ? q[8 * kk + 4 + t4] : 0u;
+          }
+          fac[mt][x] = c2;
+        } else {
+          // dims 16 t4 + 4 kk (+ 1), and 2 more
+          uint32_t w[8];
+          uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          w[i] = real ? q[8 * t4 + i] : 0u;
-          top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the largest exponent becomes 14 (an infinity or NaN stays one; a row of zeros may take any factor)
-        const int e = min(max((int)(top >> 7), 30), 254);  // biased
-        const float f = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
-        fac[mt][x] = fmaxf(c2 / f, 1.2e-38f);  // never 0: it meets masked scores of -inf
+          for (int i = 0; i < 8; ++i) {
+            w[i] = real ? q[8 * t4 + i] : 0u;
+            top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+          }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // the largest exponent becomes 14 (an infinity or NaN stays one; a row of zeros may take any factor)
+          const int e = min(max((int)(top >> 7), 30), 254);  // biased
+          const float f = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
+          fac[mt][x] = fmaxf(c2 / f, 1.2e-38f);  // never 0: it meets masked scores of -inf
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
+          for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const uint32_t u = w[2 * kk + y];
-            __half2 h = __floats2half2_rn(bf_lo(u) * f, bf_hi(u) * f);
-            qa[mt][kk][2 * y + x] = *reinterpret_cast<uint32_t*>(&h);
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t u = w[2 * kk + y];
+              __half2 h = __floats2half2_rn(bf_lo(u) * f, bf_hi(u) * f);
+              qa[mt][kk][2 * y + x] = *reinterpret_cast<uint32_t*>(&h);
+            }
           }
         }
       }
     }
-  }
-  float m[MT][2], l[MT][2], o[MT][8][4];
+    float m[MT][2], l[MT][2], o[MT][8][4];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m[mt][0] = m[mt][1] = -INFINITY;
-    l[mt][0] = l[mt][1] = 0.f;
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
-  }
-  int top_v = 0;  // 8-bit: O's unit is 2^(top_v - 127)
-  bool ok = true;
-  // this thread's places in 32 rows of a chunk
-  const uint32_t k_at = kFp8 ? few_place(g8) * 64 + ((t4 ^ ((few_place(g8) >> 1) & 3)) << 4) : (lane & 7) * 128;
-  const uint32_t v_at[2] = {few_v_at(2 * t4, g8), few_v_at(2 * t4 + 1, g8)};
-  const int scale_at = (t4 >> 1) * 4;
-  int st = warp, phase = 0;
-  static_assert(kFewWarps <= kFewStages, "a warp's first chunk is in the ring's first round");
-  for (int j = warp; j < nchunks; j += kFewWarps) {
-    ok = wait_all(full(st), phase);
-    if (!ok) break;
-    bool odd = false, wide = false;  // 8-bit: the chunk has a NaN scale; V's scales span more than f16 holds
-    if (kFp8) {
-      // the scales of positions 2 lane and 2 lane + 1; those behind the end, and NaN, do not count
-      const uint8_t* sc = smem + L::kScales + st * 2 * C;
-      const uint32_t k2 = reinterpret_cast<const uint16_t*>(sc)[lane], v2 = reinterpret_cast<const uint16_t*>(sc + C)[lane];
-      const int v0 = v2 & 255, v1 = v2 >> 8, pos = p0 + j * C + 2 * lane;
-      odd = __any_sync(0xffffffffu, (k2 & 255) == kScaleNaN || (k2 >> 8) == kScaleNaN || v0 == kScaleNaN || v1 == kScaleNaN);
-      const bool in0 = pos < end && v0 != kScaleNaN, in1 = pos + 1 < end && v1 != kScaleNaN;
-      const int most = __reduce_max_sync(0xffffffffu, max(in0 ? v0 : 0, in1 ? v1 : 0));
-      if (most > top_v) {
-        const float f = top_v ? e8m0_value(max(127 + top_v - most, 1)) : 1.f;
+      for (int i = 0; i < 8; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
+    }
+    int top_v = 0;  // 8-bit: O's unit is 2^(top_v - 127)
+    bool ok = true;
+    // this thread's places in 32 rows of a chunk
+    const uint32_t k_at = kFp8 ? few_place(g8) * 64 + ((t4 ^ ((few_place(g8) >> 1) & 3)) << 4) : (lane & 7) * 128;
+    const uint32_t v_at[2] = {few_v_at(2 * t4, g8), few_v_at(2 * t4 + 1, g8)};
+    const int scale_at = (t4 >> 1) * 4;
+    int st = warp, phase = 0;
+    for (int j = warp; j < nchunks; j += kFewWarps) {
+      ok = wait_all(full(st), phase);
+      if (!ok) break;
+      bool odd = false, wide = false;  // 8-bit: the chunk has a NaN scale; V's scales span more than f16 holds
+      if (kFp8) {
+        // the scales of positions 2 lane and 2 lane + 1; those behind the end, and NaN, do not count
+        const uint8_t* sc = smem + L::kScales + st * 2 * C;
+        const uint32_t k2 = reinterpret_cast<const uint16_t*>(sc)[lane], v2 = reinterpret_cast<const uint16_t*>(sc + C)[lane];
+        const int v0 = v2 & 255, v1 = v2 >> 8, pos = p0 + j * C + 2 * lane;
+        odd = __any_sync(0xffffffffu, (k2 & 255) == kScaleNaN || (k2 >> 8) == kScaleNaN || v0 == kScaleNaN || v1 == kScaleNaN);
+        const bool in0 = pos < end && v0 != kScaleNaN, in1 = pos + 1 < end && v1 != kScaleNaN;
+        const int most = __reduce_max_sync(0xffffffffu, max(in0 ? v0 : 0, in1 ? v1 : 0));
+        if (most > top_v) {
+          const float f = top_v ? e8m0_value(max(127 + top_v - most, 1)) : 1.f;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 2 * X; ++e) o[mt][i][e] *= f;
+          top_v = most;
+        }
+        wide = __reduce_min_sync(0xffffffffu, min(in0 ? v0 : 255, in1 ? v1 : 255)) < top_v - 10;
+      }
+      const float v_unit = kFp8 ? e8m0_value(max(254 - top_v, 1)) : 1.f;  // 2^(127 - top_v)
+      // 32 positions; kPlain: all committed, every scale a number and V's within f16's reach
+      auto step = [&](auto plain, const int sub) {
+        constexpr bool kPlain = decltype(plain)::value;
+        const int c0 = p0 + j * C + sub * 32;
+        const bool tail = !kPlain && c0 + 32 > prefix;
+        const uint32_t kb = base + st * kFewStageBytes + sub * 32 * (kFp8 ? 64 : 128), vb = kb + kFewStageBytes / 2;
+        const uint8_t* krow = smem + (kb - base);
+        const uint8_t* sc = smem + L::kScales + st * 2 * C + sub * 32;  // K scales; V's are C further
+        uint32_t vis[MT][2], dead = 0;  // seen positions; positions without a finite V
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) vis[mt][0] = vis[mt][1] = 0xffffffffu;
+        if (tail) {
+          const int pos = c0 + lane;
+          bool bad = false;
+          if (kFp8) {
+            bad = sc[C + lane] == kScaleNaN;
+          } else if (pos >= prefix && pos < end) {
+            const uint4* v = reinterpret_cast<const uint4*>(smem + (vb - base) + lane * 128);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint4 u = v[c];
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                bad |= (w[e] & 0x7F800000u) == 0x7F800000u || (w[e] & 0x7F80u) == 0x7F80u;
+            }
+          }
+          if (pos >= end || bad) {  // V becomes 0: a masked P of 0 must not meet a NaN
+            uint4* v = reinterpret_cast<uint4*>(smem + (vb - base) + lane * (kFp8 ? 64 : 128));
+#pragma unroll
+            for (int c = 0; c < (kFp8 ? 4 : 8); ++c) v[c] = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          bad = bad && pos >= prefix && pos < end;
+          const uint32_t poison = __ballot_sync(0xffffffffu, bad);
+          dead = poison | __ballot_sync(0xffffffffu, pos >= end);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int x = 0; x < X; ++x) {
+              const int r = mt * 16 + x * 8 + g8;
+              vis[mt][x] = 0;
+              if (r < trows)
+                vis[mt][x] = (uint32_t)tree_bits(p.mask + (size_t)(row0 + (trow0 + r) / p.group) * p.words, p.words,
+                                                 nodes, c0 - prefix);
+              // a row that sees a V that is not finite has no finite result
+              if (vis[mt][x] & poison) l[mt][x] = __uint_as_float(0x7FFFFFFFu);
+            }
+          }
+          __syncwarp();
+        }
+        // ---- scores: four blocks of 8 positions
+        float s[MT][4][4];
+        float sv[4][2];  // 8-bit: V's scales of this thread's columns
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb) {
+          if (!kFp8) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              uint32_t kf[4];
+              few_ldmatrix(kf, kb + k_at + nb * 1024 + (((hf * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) few_mma<false>(s[mt][nb], qa[mt][hf * 2 + u], kf[2 * u], kf[2 * u + 1], hf == 0 && u == 0);
+            }
+          } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(krow + k_at + nb * 512);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint32_t b0 = few_half2(w[kk], false), b1 = few_half2(w[kk], true);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) few_mma<true>(s[mt][nb], qa[mt][kk], b0, b1, kk == 0);
+            }
+            // the scales of this thread's two columns, out of four neighbouring bytes
+            const uint32_t ks = *reinterpret_cast<const uint32_t*>(sc + scale_at + nb * 8);
+            const uint32_t vs = *reinterpret_cast<const uint32_t*>(sc + scale_at + C + nb * 8);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // the byte on top, then down by one: a float's exponent
+              const uint32_t kx = __byte_perm(ks, 0, e ? pick1 : pick0) >> 1, vx = __byte_perm(vs, 0, e ? pick1 : pick0) >> 1;
+              float kf = __uint_as_float(kx), vf = __uint_as_float(vx) * v_unit;
+              if (!kPlain && (tail || odd)) {
+                if (kx == 0x7F800000u) kf = __uint_as_float(0x7FFFFFFFu);
+                if (vx == 0x7F800000u) vf = __uint_as_float(0x7FFFFFFFu);
+                if ((dead >> (nb * 8 + few_place(2 * t4 + e))) & 1) vf = 0.f;
+              }
+              sv[nb][e] = vf;
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int x = 0; x < X; ++x) s[mt][nb][2 * x + e] *= kf;
+            }
+          }
+        }
+        if (tail) {
+#pragma unroll
+          for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int at = nb * 8 + (kFp8 ? few_place(2 * t4 + e) : 2 * t4 + e);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int x = 0; x < X; ++x)
+                  if (!((vis[mt][x] >> at) & 1)) s[mt][nb][2 * x + e] = -INFINITY;
+              }
+            }
+        }
+        // ---- maxima
+        float mx[MT][2];
+        bool grow = false;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int x = 0; x < X; ++x) {
+            float t = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 2 * X; ++e) o[mt][i][e] *= f;
-        top_v = most;
-      }
-      wide = __reduce_min_sync(0xffffffffu, min(in0 ? v0 : 255, in1 ? v1 : 255)) < top_v - 10;
-    }
-    const float v_unit = kFp8 ? e8m0_value(max(254 - top_v, 1)) : 1.f;  // 2^(127 - top_v)
-    // 32 positions; kPlain: all committed, every scale a number and V's within f16's reach
-    auto step = [&](auto plain, const int sub) {
-      constexpr bool kPlain = decltype(plain)::value;
-      const int c0 = p0 + j * C + sub * 32;
-      const bool tail = !kPlain && c0 + 32 > prefix;
-      const uint32_t kb = base + st * kFewStageBytes + sub * 32 * (kFp8 ? 64 : 128), vb = kb + kFewStageBytes / 2;
-      const uint8_t* krow = smem + (kb - base);
-      const uint8_t* sc = smem + L::kScales + st * 2 * C + sub * 32;  // K scales; V's are C further
-      uint32_t vis[MT][2], dead = 0;  // seen positions; positions without a finite V
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) vis[mt][0] = vis[mt][1] = 0xffffffffu;
-      if (tail) {
-        const int pos = c0 + lane;
-        bool bad = false;
-        if (kFp8) {
-          bad = sc[C + lane] == kScaleNaN;
-        } else if (pos >= prefix && pos < end) {
-          const uint4* v = reinterpret_cast<const uint4*>(smem + (vb - base) + lane * 128);
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const uint4 u = v[c];
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              bad |= (w[e] & 0x7F800000u) == 0x7F800000u || (w[e] & 0x7F80u) == 0x7F80u;
+            for (int nb = 0; nb < 4; ++nb) t = tree_max3(t, s[mt][nb][2 * x], s[mt][nb][2 * x + 1]);
+            mx[mt][x] = t * fac[mt][x];
+            grow |= mx[mt][x] > m[mt][x] + 8.f;
           }
-        }
-        if (pos >= end || bad) {  // V becomes 0: a masked P of 0 must not meet a NaN
-          uint4* v = reinterpret_cast<uint4*>(smem + (vb - base) + lane * (kFp8 ? 64 : 128));
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int c = 0; c < (kFp8 ? 4 : 8); ++c) v[c] = make_uint4(0, 0, 0, 0);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < X; ++x) {
+              float t = mx[mt][x];  // the row's four lanes agree
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+              if (t > m[mt][x] + 8.f) {
+                const float alpha = exp2_approx(m[mt][x] - t);  // 0 for the first maximum
+                m[mt][x] = t;
+                l[mt][x] *= alpha;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  o[mt][i][2 * x] *= alpha;
+                  o[mt][i][2 * x + 1] *= alpha;
+                }
+              }
+            }
         }
-        bad = bad && pos >= prefix && pos < end;
-        const uint32_t poison = __ballot_sync(0xffffffffu, bad);
-        dead = poison | __ballot_sync(0xffffffffu, pos >= end);
+        // ---- probabilities, as the A fragments of P V
+        uint32_t pa[MT][2][4] = {};
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int x = 0; x < X; ++x) {
-            const int r = mt * 16 + x * 8 + g8;
-            vis[mt][x] = 0;
-            if (r < trows)
-              vis[mt][x] = (uint32_t)tree_bits(p.mask + (size_t)(row0 + (trow0 + r) / p.group) * p.words, p.words,
-                                               nodes, c0 - prefix);
-            // a row that sees a V that is not finite has no finite result
-            if (vis[mt][x] & poison) l[mt][x] = __uint_as_float(0x7FFFFFFFu);
-          }
-        }
-        __syncwarp();
-      }
-      // ---- scores: four blocks of 8 positions
-      float s[MT][4][4];
-      float sv[4][2];  // 8-bit: V's scales of this thread's columns
+            const float mu = m[mt][x] == -INFINITY ? 0.f : m[mt][x];
 #pragma unroll
-      for (int nb = 0; nb < 4; ++nb) {
-        if (!kFp8) {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t kf[4];
-            few_ldmatrix(kf, kb + k_at + nb * 1024 + (((hf * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) few_mma<false>(s[mt][nb], qa[mt][hf * 2 + u], kf[2 * u], kf[2 * u + 1], hf == 0 && u == 0);
-          }
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4*>(krow + k_at + nb * 512);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint32_t b0 = few_half2(w[kk], false), b1 = few_half2(w[kk], true);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) few_mma<true>(s[mt][nb], qa[mt][kk], b0, b1, kk == 0);
-          }
-          // the scales of this thread's two columns, out of four neighbouring bytes
-          const uint32_t ks = *reinterpret_cast<const uint32_t*>(sc + scale_at + nb * 8);
-          const uint32_t vs = *reinterpret_cast<const uint32_t*>(sc + scale_at + C + nb * 8);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            // the byte on top, then down by one: a float's exponent
-            const uint32_t kx = __byte_perm(ks, 0, e ? pick1 : pick0) >> 1, vx = __byte_perm(vs, 0, e ? pick1 : pick0) >> 1;
-            float kf = __uint_as_float(kx), vf = __uint_as_float(vx) * v_unit;
-            if (!kPlain && (tail || odd)) {
-              if (kx == 0x7F800000u) kf = __uint_as_float(0x7FFFFFFFu);
-              if (vx == 0x7F800000u) vf = __uint_as_float(0x7FFFFFFFu);
-              if ((dead >> (nb * 8 + few_place(2 * t4 + e))) & 1) vf = 0.f;
-            }
-            sv[nb][e] = vf;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int x = 0; x < X; ++x) s[mt][nb][2 * x + e] *= kf;
-          }
-        }
-      }
-      if (tail) {
-#pragma unroll
-        for (int nb = 0; nb < 4; ++nb)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int at = nb * 8 + (kFp8 ? few_place(2 * t4 + e) : 2 * t4 + e);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-              for (int x = 0; x < X; ++x)
-                if (!((vis[mt][x] >> at) & 1)) s[mt][nb][2 * x + e] = -INFINITY;
-            }
-          }
-      }
-      // ---- maxima
-      float mx[MT][2];
-      bool grow = false;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int x = 0; x < X; ++x) {
-          float t = -INFINITY;
-#pragma unroll
-          for (int nb = 0; nb < 4; ++nb) t = tree_max3(t, s[mt][nb][2 * x], s[mt][nb][2 * x + 1]);
-          mx[mt][x] = t * fac[mt][x];
-          grow |= mx[mt][x] > m[mt][x] + 8.f;
-        }
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int x = 0; x < X; ++x) {
-            float t = mx[mt][x];  // the row's four lanes agree
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            if (t > m[mt][x] + 8.f) {
-              const float alpha = exp2_approx(m[mt][x] - t);  // 0 for the first maximum
-              m[mt][x] = t;
-              l[mt][x] *= alpha;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                o[mt][i][2 * x] *= alpha;
-                o[mt][i][2 * x + 1] *= alpha;
+            for (int nb = 0; nb < 4; ++nb) {
+              float e0 = exp2_approx(fmaf(s[mt][nb][2 * x], fac[mt][x], -mu));
+              float e1 = exp2_approx(fmaf(s[mt][nb][2 * x + 1], fac[mt][x], -mu));
+              l[mt][x] += e0 + e1;
+              uint32_t& a = pa[mt][nb >> 1][(nb & 1) * 2 + x];
+              if (kFp8) {
+                e0 *= sv[nb][0];
+                e1 *= sv[nb][1];
+              }
+              if (!kFp8 || (!kPlain && wide)) {
+                __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
+                a = *reinterpret_cast<uint32_t*>(&h);
+              } else {
+                __half2 h = __floats2half2_rn(e0, e1);
+                a = *reinterpret_cast<uint32_t*>(&h);
               }
             }
           }
-      }
-      // ---- probabilities, as the A fragments of P V
-      uint32_t pa[MT][2][4] = {};
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int x = 0; x < X; ++x) {
-          const float mu = m[mt][x] == -INFINITY ? 0.f : m[mt][x];
-#pragma unroll
-          for (int nb = 0; nb < 4; ++nb) {
-            float e0 = exp2_approx(fmaf(s[mt][nb][2 * x], fac[mt][x], -mu));
-            float e1 = exp2_approx(fmaf(s[mt][nb][2 * x + 1], fac[mt][x], -mu));
-            l[mt][x] += e0 + e1;
-            uint32_t& a = pa[mt][nb >> 1][(nb & 1) * 2 + x];
-            if (kFp8) {
-              e0 *= sv[nb][0];
-              e1 *= sv[nb][1];
-            }
-            if (!kFp8 || (!kPlain && wide)) {
-              __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-              a = *reinterpret_cast<uint32_t*>(&h);
-            } else {
-              __half2 h = __floats2half2_rn(e0, e1);
-              a = *reinterpret_cast<uint32_t*>(&h);
-            }
-          }
         }
-      }
-      // ---- P . V: two steps of 16 positions, eight blocks of 8 dims
+        // ---- P . V: two steps of 16 positions, eight blocks of 8 dims
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        if (!kFp8) {
+        for (int ks = 0; ks < 2; ++ks) {
+          if (!kFp8) {
 #pragma unroll
-          for (int dp = 0; dp < 4; ++dp) {
-            uint32_t vf[4];
-            const int r = ks * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), c = dp * 2 + (lane >> 4);
-            few_ldmatrix_t(vf, vb + r * 128 + ((c ^ (r & 7)) << 4));
+            for (int dp = 0; dp < 4; ++dp) {
+              uint32_t vf[4];
+              const int r = ks * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), c = dp * 2 + (lane >> 4);
+              few_ldmatrix_t(vf, vb + r * 128 + ((c ^ (r & 7)) << 4));
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+              for (int u = 0; u < 2; ++u)
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][dp * 2 + u], pa[mt][ks], vf[2 * u], vf[2 * u + 1]);
-          }
-        } else {
-          uint2 v[2][2];  // [8 positions][column e]: dims 8 g8 .. 8 g8 + 7 of a position
-#pragma unroll
-          for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              v[q][e] = *reinterpret_cast<const uint2*>(krow + kFewStageBytes / 2 + v_at[e] + (ks * 16 + q * 8) * 64);
-            }
-          if (kPlain || !wide) {
-#pragma unroll
-            for (int d = 0; d < 8; d += 2) {
-              uint32_t bf[2][2];  // [dim][8 positions]
-#pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const uint32_t lo = d < 4 ? v[q][0].x : v[q][0].y, hi = d < 4 ? v[q][1].x : v[q][1].y;
-                const uint32_t w = __byte_perm(lo, hi, (d & 2) ? 0x7362 : 0x5140);
-                bf[0][q] = few_half2(w, false);
-                bf[1][q] = few_half2(w, true);
-              }
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                few_mma<true>(o[mt][d], pa[mt][ks], bf[0][0], bf[0][1]);
-                few_mma<true>(o[mt][d + 1], pa[mt][ks], bf[1][0], bf[1][1]);
-              }
+                for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][dp * 2 + u], pa[mt][ks], vf[2 * u], vf[2 * u + 1]);
             }
           } else {
-            const __nv_bfloat162 f = tree_pow2(247);  // 2^120
+            uint2 v[2][2];  // [8 positions][column e]: dims 8 g8 .. 8 g8 + 7 of a position
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-              uint32_t bf[2];
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const uint32_t lo = d < 4 ? v[q][0].x : v[q][0].y, hi = d < 4 ? v[q][1].x : v[q][1].y;
-                const uint32_t w = __byte_perm(lo, hi, (d & 3) << 4 | (4 + (d & 3)) << 12);
-                const uint32_t z = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);
-                const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&z), f);
-                bf[q] = *reinterpret_cast<const uint32_t*>(&y);
+              for (int e = 0; e < 2; ++e) {
+                v[q][e] = *reinterpret_cast<const uint2*>(krow + kFewStageBytes / 2 + v_at[e] + (ks * 16 + q * 8) * 64);
               }
+            if (kPlain || !wide) {
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][d], pa[mt][ks], bf[0], bf[1]);
+              for (int d = 0; d < 8; d += 2) {
+                uint32_t bf[2][2];  // [dim][8 positions]
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const uint32_t lo = d < 4 ? v[q][0].x : v[q][0].y, hi = d < 4 ? v[q][1].x : v[q][1].y;
+                  const uint32_t w = __byte_perm(lo, hi, (d & 2) ? 0x7362 : 0x5140);
+                  bf[0][q] = few_half2(w, false);
+                  bf[1][q] = few_half2(w, true);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  few_mma<true>(o[mt][d], pa[mt][ks], bf[0][0], bf[0][1]);
+                  few_mma<true>(o[mt][d + 1], pa[mt][ks], bf[1][0], bf[1][1]);
+                }
+              }
+            } else {
+              const __nv_bfloat162 f = tree_pow2(247);  // 2^120
+#pragma unroll
+              for (int d = 0; d < 8; ++d) {
+                uint32_t bf[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const uint32_t lo = d < 4 ? v[q][0].x : v[q][0].y, hi = d < 4 ? v[q][1].x : v[q][1].y;
+                  const uint32_t w = __byte_perm(lo, hi, (d & 3) << 4 | (4 + (d & 3)) << 12);
+                  const uint32_t z = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);
+                  const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&z), f);
+                  bf[q] = *reinterpret_cast<const uint32_t*>(&y);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][d], pa[mt][ks], bf[0], bf[1]);
+              }
             }
           }
         }
-      }
-    };
+      };
 #pragma unroll 1
-    for (int sub = 0; sub < C / 32; ++sub) {
-      const int c0 = p0 + j * C + sub * 32;
-      if (c0 >= p1) break;
-      if (c0 + 32 > prefix || odd || wide)
-        step(std::false_type{}, sub);
-      else
-        step(std::true_type{}, sub);
+      for (int sub = 0; sub < C / 32; ++sub) {
+        const int c0 = p0 + j * C + sub * 32;
+        if (c0 >= p1) break;
+        if (c0 + 32 > prefix || odd || wide)
+          step(std::false_type{}, sub);
+        else
+          step(std::true_type{}, sub);
+      }
+      __syncwarp();
+      if (lane == 0) tree_arrive(empty(st));
+      st += kFewWarps;
+      if (st >= kFewStages) {
+        st -= kFewStages;
+        phase ^= 1;
+      }
     }
-    __syncwarp();
-    if (lane == 0) tree_arrive(empty(st));
-    st += kFewWarps;
-    if (st >= kFewStages) {
-      st -= kFewStages;
-      phase ^= 1;
-    }
-  }
 
-  // ---- the four warps joined; their states lie over the ring, which nobody reads any more
-  float* state = reinterpret_cast<float*>(smem);  // [warp][R][66]
-  const float unit = kFp8 && top_v ? e8m0_value(top_v) : 1.f;
-  asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
+    // ---- the four warps joined; their states lie over the ring, which nobody reads any more
+    float* state = reinterpret_cast<float*>(smem);  // [warp][R][66]
+    const float unit = kFp8 && top_v ? e8m0_value(top_v) : 1.f;
+    asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int x = 0; x < X; ++x) {
-      float t = l[mt][x];
-      t += __shfl_xor_sync(0xffffffffu, t, 1);
-      t += __shfl_xor_sync(0xffffffffu, t, 2);
-      float* d = state + (warp * R + mt * 16 + x * 8 + g8) * kTreePartial;
-      if (t4 == 0) *reinterpret_cast<float2*>(d) = make_float2(m[mt][x], t);
+      for (int x = 0; x < X; ++x) {
+        float t = l[mt][x];
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        float* d = state + (warp * R + mt * 16 + x * 8 + g8) * kTreePartial;
+        if (t4 == 0) *reinterpret_cast<float2*>(d) = make_float2(m[mt][x], t);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (!kFp8) {  // dims 8 i + 2 t4 (+ 1)
-          *reinterpret_cast<float2*>(d + 2 + 8 * i + 2 * t4) = make_float2(o[mt][i][2 * x], o[mt][i][2 * x + 1]);
-        } else {  // in units of V's largest scale; dims 16 t4 + i and 8 more
-          d[2 + 16 * t4 + i] = o[mt][i][2 * x] * unit;
-          d[2 + 16 * t4 + 8 + i] = o[mt][i][2 * x + 1] * unit;
+        for (int i = 0; i < 8; ++i) {
+          if (!kFp8) {  // dims 8 i + 2 t4 (+ 1)
+            *reinterpret_cast<float2*>(d + 2 + 8 * i + 2 * t4) = make_float2(o[mt][i][2 * x], o[mt][i][2 * x + 1]);
+          } else {  // in units of V's largest scale; dims 16 t4 + i and 8 more
+            d[2 + 16 * t4 + i] = o[mt][i][2 * x] * unit;
+            d[2 + 16 * t4 + 8 + i] = o[mt][i][2 * x + 1] * unit;
+          }
         }
       }
-    }
-  asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
-  float* joined = state + kFewWarps * R * kTreePartial;  // in a cluster: [R][66], for its other CTAs
-  static_assert((kFewWarps + 1) * R * kTreePartial * 4 <= kFewStages * kFewStageBytes, "the states fit over the ring");
-  for (int r = warp; ok && r < trows; r += kFewWarps) {  // a lane has two dims
-    float top = -INFINITY;
+    asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
+    float* joined = state + kFewWarps * R * kTreePartial;  // in a cluster: [R][66], for its other CTAs
+    static_assert((kFewWarps + 1) * R * kTreePartial * 4 <= kFewStages * kFewStageBytes, "the states fit over the ring");
+    for (int r = warp; ok && r < trows; r += kFewWarps) {  // a lane has two dims
+      float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, state[(w * R + r) * kTreePartial]);
-    const float mu = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+      for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, state[(w * R + r) * kTreePartial]);
+      const float mu = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) {
-      const float* d = state + (w * R + r) * kTreePartial;
-      const float a = exp2_approx(d[0] - mu);
-      const float2 v = *reinterpret_cast<const float2*>(d + 2 + 2 * lane);
-      sum = fmaf(d[1], a, sum);
-      o0 = fmaf(v.x, a, o0);
-      o1 = fmaf(v.y, a, o1);
-    }
-    const int pr = trow0 + r;
-    if (p.splits > 1) {
-      float* dst = p.cluster ? joined + r * kTreePartial
-                             : p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
-      if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(top, sum);
-      *reinterpret_cast<float2*>(dst + 2 + 2 * lane) = make_float2(o0, o1);
-    } else {
-      tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, top, sum, o0, o1);
+      for (int w = 0; w < kFewWarps; ++w) {
+        const float* d = state + (w * R + r) * kTreePartial;
+        const float a = exp2_approx(d[0] - mu);
+        const float2 v = *reinterpret_cast<const float2*>(d + 2 + 2 * lane);
+        sum = fmaf(d[1], a, sum);
+        o0 = fmaf(v.x, a, o0);
+        o1 = fmaf(v.y, a, o1);
+      }
+      const int pr = trow0 + r;
+      if (p.splits > 1) {
+        float* dst = p.cluster ? joined + r * kTreePartial
+                               : p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
+        if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(top, sum);
+        *reinterpret_cast<float2*>(dst + 2 + 2 * lane) = make_float2(o0, o1);
+      } else {
+        tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, top, sum, o0, o1);
+      }
     }
   }
   if (p.cluster)

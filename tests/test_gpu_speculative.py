@@ -287,6 +287,24 @@ def test_tree_attention(fmt, i):
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("nodes", [1, 4, 8])
+def test_full_gpu_of_long_sequences(fmt, nodes):
+    """Every ring goes round many times while copies finish in any order: each call gives
+    the same bits, the right ones."""
+    s = _setup([4096 - 61 * i for i in range(32)], [nodes] * 32, 32, 8, 64, fmt, "tree", seed=nodes)
+    out, lse, err = _attend(s)
+    for _ in range(30):
+        again, lse2, _ = _attend(s, err=err)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+    assert int(err) == 0
+    for b in range(0, 32, 5):  # the comparison in 64 bits, of some
+        rows = slice(b * nodes, (b + 1) * nodes)
+        one = dict(s, prefixes=s["prefixes"][b:b + 1], nodes=[nodes], masks=s["masks"][b:b + 1], q=s["q"][rows],
+                   right_tables=s["right_tables"][b:b + 1])
+        _check(one, out[rows], lse[rows])
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 @pytest.mark.parametrize("nodes", [1, 7, 40])
 def test_large_scores(fmt, nodes):
     """Scores of hundreds: the running maximum has to carry the sums."""
