@@ -492,9 +492,6 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int nblocks = (p1 - p0 + kTreeBlock - 1) / kTreeBlock;
   const int halves = (p1 - p0 + kTreeHalf - 1) / kTreeHalf;
   const int active = (trows + 31) >> 5;  // softmax warps with a row
-  // blocks from here on reach past the committed positions; before it a bf16 block
-  // goes from memory to the tensor cores untouched
-  const int tails = kFp8 ? 0 : min(nblocks, max(prefix - p0, 0) / kTreeBlock);
   if (threadIdx.x == 0) {
     init(b_q, active);
     init(b_p(0), active);
@@ -569,11 +566,8 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     constexpr uint32_t id_s = tree_idesc(kTreeHalf, false), id_o = tree_idesc(64, true);
     const uint64_t dq = tree_desc(base + L::kQ);
     int slot = 0, next = 0, next_phase = 0;  // the block's slot; the next one's, and its phase
-    int ahead = 0;                           // the next one's number
     auto scores = [&](int half) {
-      if (!half && !(ahead < tails ? wait_all(full(next), next_phase)
-                                   : wait_all(ready(next), kFp8 ? next_phase : ((ahead - tails) / L::kReady) & 1)))
-        return false;
+      if (!half && !wait_all(ready(next), next_phase)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       tree_mma_scores(t_s(half), dq, tree_desc(slot_at(next) + half * (kTreeHalf * 128)), id_s);
       tree_commit(b_s(half));
@@ -581,7 +575,6 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     };
     bool ok = wait_all(b_q, 0) && scores(0) && (halves < 2 || scores(1));
     for (int j = 0; j < nblocks && ok; ++j) {
-      ++ahead;
       if (++next == L::kReady) {
         next = 0;
         next_phase ^= 1;
@@ -605,11 +598,12 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     tree_commit(b_o);
     wait_all(b_o, 0);
   } else if (warp >= 8) {
-    // ---- block warps, one thread per position
+    // ---- block warps, one thread per position. They pass every block, also those that
+    // need nothing: a wait for a phase means something only to who has waited for the last
     const int r = threadIdx.x - 256;
     static_assert(L::kStages == L::kReady, "one slot counter for both rings");
-    int rd = tails % L::kReady, phase = (tails / L::kReady) & 1;
-    for (int j = tails; j < nblocks; ++j) {
+    int rd = 0, phase = 0;
+    for (int j = 0; j < nblocks; ++j) {
       const int st = rd, c0 = p0 + j * kTreeBlock, pos = c0 + r;
       const bool tail = c0 + kTreeBlock > prefix;
       const bool drafted = pos >= prefix && pos < end;
@@ -717,7 +711,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       if constexpr (kTail) {
         const int rd = j % L::kReady;
         vis = tree_bits(p.mask + (size_t)row * p.words, p.words, nodes, p0 + j * kTreeBlock + half * kTreeHalf - prefix);
-        if (!wait_all(ready(rd), ((j - tails) / L::kReady) & 1)) return false;
+        if (!wait_all(ready(rd), (j / L::kReady) & 1)) return false;
         // a row that sees a V that is not finite has no finite result
         if (vis & (bad[rd * 4 + 2 * half] | (unsigned long long)bad[rd * 4 + 2 * half + 1] << 32))
           l = __uint_as_float(0x7FFFFFFFu);

@@ -346,6 +346,38 @@ def test_masked_places_have_no_effect(fmt, nodes):
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("prefix", [300, 640, 1500, 2047])
+def test_masked_places_behind_long_prefixes(fmt, prefix):
+    """The blocks with drafted nodes come after many without: what lies behind the last
+    node, and in a node that only itself sees, still has no effect, on a busy GPU."""
+    batch, nodes = 24, 20
+    s = _setup([prefix - i for i in range(batch)], [nodes] * batch, 32, 8, 64, fmt, "tree", seed=prefix)
+    where = torch.zeros(s["k"].shape[:3], dtype=torch.bool, device=DEV)
+    for b, p in enumerate(s["prefixes"]):
+        at = torch.arange(p + nodes - 1, s["tables"].shape[1] * 64, device=DEV)  # a leaf, and all behind it
+        where[s["tables"][b].long()[at // 64], :, at % 64] = True
+    if fmt == "bf16":
+        s["v"][where] = math.nan
+    else:
+        s["v"].view(torch.uint8)[where] = 0xFF
+        s["vs"][where] = NAN_BYTE
+    err = _err()
+    out, lse, _ = _attend(s, err=err)
+    for _ in range(20):
+        again, lse2, _ = _attend(s, err=err)
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+        assert torch.equal(lse.view(torch.int32), lse2.view(torch.int32))
+    assert int(err) == 0
+    leaves = torch.arange(nodes - 1, batch * nodes, nodes, device=DEV)
+    assert out[leaves].isnan().all() and lse[leaves].isnan().all()
+    for b in range(0, batch, 7):
+        rows = slice(b * nodes, (b + 1) * nodes)
+        one = dict(s, prefixes=s["prefixes"][b:b + 1], nodes=[nodes], masks=s["masks"][b:b + 1], q=s["q"][rows],
+                   right_tables=s["right_tables"][b:b + 1])
+        _check(one, out[rows], lse[rows], skip={(0, nodes - 1)})
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 def test_value_of_a_seen_node_is_not_finite(fmt):
     """Only V holds the NaN: rows that see the node are not finite, the others are untouched."""
     s = _setup([70], [30], 8, 2, 16, fmt, "chain", seed=3)
