@@ -45,7 +45,7 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 
 // Which kernel a call takes and how the positions of a sequence are split over its
 // CTAs. Up to kTreeFewRows rows (nodes x query heads of a K/V head) go to the
-// mma.sync kernel, in one tile of 8, 16 or 32; more to the tcgen05 kernel in tiles of
+// mma.sync kernel, in one tile of 8 or 16; more to the tcgen05 kernel in tiles of
 // 128. A launch of n CTAs, c to an SM, takes about ceil(n / (c SMs)) waves of one
 // range each; a range costs its length and a fixed part (launch, first bytes, the
 // store). Joining ranges costs a little in a cluster (up to eight ranges) and a
@@ -54,22 +54,22 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 // CTAs of a cluster wait for one another's slots, and the row tiles that share
 // positions drift apart. 4 sequences of 256 nodes at 16,000: 211 us whole, 247 in
 // four.)
-constexpr int kTreeFewRows = 32;
+constexpr int kTreeFewRows = 16;
 constexpr int kTreeCluster = 8;  // the portable size
 struct TreePlan {
-  int few;  // eights of rows in a tile of the mma.sync kernel (1, 2, 4), 0: tcgen05
+  int few;  // eights of rows in a tile of the mma.sync kernel (1, 2), 0: tcgen05
   int tiles, splits, len;
   bool cluster() const { return splits > 1 && splits <= kTreeCluster; }
 };
 TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
   TreePlan t{};
-  t.few = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= kTreeFewRows ? 4 : 0;
+  t.few = rows <= 8 ? 1 : rows <= kTreeFewRows ? 2 : 0;
   const int tile_rows = t.few ? 8 * t.few : mk::kTreeRows;
   t.tiles = (rows + tile_rows - 1) / tile_rows;
   const int unit = mk::kTreeBlock, units = (max_len + unit - 1) / unit;
   const int fixed = t.few ? 2 : 3;  // in units, like the costs of a join: 1 and 3
   const long long ctas = (long long)batch * num_kv_heads * t.tiles;
-  const long long slots = (t.few == 1 ? 4LL : t.few == 2 ? 3LL : 2LL) * device_sms();
+  const long long slots = (t.few ? (long long)mk::kFewCtas : 2LL) * device_sms();
   long long best = -1;
   int last = 0;
   for (int want = 1; want <= units; ++want) {
@@ -148,7 +148,6 @@ template <bool kFp8>
 cudaError_t launch_tree(const mk::TreeTmaParams& tp, int few, dim3 grid, cudaStream_t st) {
   if (few == 1) return launch_few<kFp8, 1>(tp, grid, st);
   if (few == 2) return launch_few<kFp8, 2>(tp, grid, st);
-  if (few == 4) return launch_few<kFp8, 4>(tp, grid, st);
   static bool done[64];
   constexpr int smem = mk::TreeSmem<kFp8>::kBytes;
   if (cudaError_t e = allow_smem(mk::tree_attn_kernel<kFp8>, smem, done)) return e;

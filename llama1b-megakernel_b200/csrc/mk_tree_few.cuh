@@ -32,12 +32,13 @@
 
 namespace mk {
 
-constexpr int kFewWarps = 4;
-constexpr int kFewStages = 8;
+constexpr int kFewWarps = 3;
+constexpr int kFewStages = 6;
 // A stage is always the same warp's, who has then waited for each of its phases. With
 // another number a warp may come to a stage that others filled and drained since it
 // last looked; a parity then does not tell the phase it waits for from the one before it.
 static_assert(kFewStages % kFewWarps == 0, "a stage belongs to one warp");
+constexpr int kFewCtas = 4;           // of an SM: 16 warps of 128 registers, 12 of them consumers
 constexpr int kFewStageBytes = 8192;  // K rows, then V rows
 
 template <bool kFp8>
@@ -91,13 +92,13 @@ __device__ __forceinline__ uint32_t few_half2(uint32_t w, bool high) {
   return h;
 }
 
+// RT: eights of rows, 1 or 2
 template <bool kFp8, int RT>
-__global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 3 : 2)
+__global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
     tree_few_kernel(const __grid_constant__ TreeTmaParams tp) {
   using L = FewShape<kFp8>;
   constexpr int C = L::kChunk, R = 8 * RT;
-  constexpr int MT = RT == 4 ? 2 : 1;  // tiles of 16
-  constexpr int X = RT == 1 ? 1 : 2;   // their upper and lower eight rows
+  constexpr int X = RT;  // the tile's upper and lower eight rows, of 16
   const TreeParams& p = tp.p;
   const KVLayer& kv = p.kv;
   pdl_trigger();
@@ -194,59 +195,53 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
     // ---- consumers. Fragment rows of thread (g8, t4): g8 and g8 + 8 of each 16.
     const int g8 = lane >> 2, t4 = lane & 3;
     const uint32_t pick0 = 0x0444u | (uint32_t)few_place(2 * t4 & 3) << 12, pick1 = 0x0444u | (uint32_t)(few_place((2 * t4 & 3) + 1) & 3) << 12;
-    uint32_t qa[MT][4][4] = {};
-    float fac[MT][2];  // scores in powers of two: times this (and, 8-bit, the K scale)
+    uint32_t qa[4][4] = {};
+    float fac[2];  // scores in powers of two: times this (and, 8-bit, the K scale)
     const float c2 = p.scale * 1.4426950408889634f;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int x = 0; x < X; ++x) {
+      const int r = x * 8 + g8, pr = trow0 + r;
+      const bool real = r < trows;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(
+          p.q + ((size_t)(row0 + (real ? pr / p.group : 0)) * p.NQ + g * p.group + (real ? pr % p.group : 0)) * 64);
+      if (!kFp8) {
 #pragma unroll
-      for (int x = 0; x < X; ++x) {
-        const int r = mt * 16 + x * 8 + g8, pr = trow0 + r;
-        const bool real = r < trows;
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(
-            p.q + ((size_t)(row0 + (real ? pr / p.group : 0)) * p.NQ + g * p.group + (real ? pr % p.group : 0)) * 64);
-        if (!kFp8) {
+        for (int kk = 0; kk < 4; ++kk) {  // dims 16 kk + 2 t4 (+ 1), and 8 more
+          qa[kk][x] = real ? q[8 * kk + t4] : 0u;
+          qa[kk][2 + x] = real ? q[8 * kk + 4 + t4] : 0u;
+        }
+        fac[x] = c2;
+      } else {
+        // dims 16 t4 + 4 kk (+ 1), and 2 more
+        uint32_t w[8];
+        uint32_t top = 0;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {  // dims 16 kk + 2 t4 (+ 1), and 8 more
-            qa[mt][kk][x] = real ? q[8 * kk + t4] : 0u;
-            qa[mt][kk][2 + x] = real ? q[8 * kk + 4 + t4] : 0u;
-          }
-          fac[mt][x] = c2;
-        } else {
-          // dims 16 t4 + 4 kk (+ 1), and 2 more
-          uint32_t w[8];
-          uint32_t top = 0;
+        for (int i = 0; i < 8; ++i) {
+          w[i] = real ? q[8 * t4 + i] : 0u;
+          top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the largest exponent becomes 14 (an infinity or NaN stays one; a row of zeros may take any factor)
+        const int e = min(max((int)(top >> 7), 30), 254);  // biased
+        const float f = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
+        fac[x] = fmaxf(c2 / f, 1.2e-38f);  // never 0: it meets masked scores of -inf
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            w[i] = real ? q[8 * t4 + i] : 0u;
-            top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
-          }
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          // the largest exponent becomes 14 (an infinity or NaN stays one; a row of zeros may take any factor)
-          const int e = min(max((int)(top >> 7), 30), 254);  // biased
-          const float f = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
-          fac[mt][x] = fmaxf(c2 / f, 1.2e-38f);  // never 0: it meets masked scores of -inf
+        for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const uint32_t u = w[2 * kk + y];
-              __half2 h = __floats2half2_rn(bf_lo(u) * f, bf_hi(u) * f);
-              qa[mt][kk][2 * y + x] = *reinterpret_cast<uint32_t*>(&h);
-            }
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t u = w[2 * kk + y];
+            __half2 h = __floats2half2_rn(bf_lo(u) * f, bf_hi(u) * f);
+            qa[kk][2 * y + x] = *reinterpret_cast<uint32_t*>(&h);
           }
         }
       }
     }
-    float m[MT][2], l[MT][2], o[MT][8][4];
+    float m[2], l[2], o[8][4];
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      m[mt][0] = m[mt][1] = -INFINITY;
-      l[mt][0] = l[mt][1] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
-    }
+    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     int top_v = 0;  // 8-bit: O's unit is 2^(top_v - 127)
     bool ok = true;
     // this thread's places in 32 rows of a chunk
@@ -269,11 +264,9 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
         if (most > top_v) {
           const float f = top_v ? e8m0_value(max(127 + top_v - most, 1)) : 1.f;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-              for (int e = 0; e < 2 * X; ++e) o[mt][i][e] *= f;
+            for (int e = 0; e < 2 * X; ++e) o[i][e] *= f;
           top_v = most;
         }
         wide = __reduce_min_sync(0xffffffffu, min(in0 ? v0 : 255, in1 ? v1 : 255)) < top_v - 10;
@@ -287,9 +280,8 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
         const uint32_t kb = base + st * kFewStageBytes + sub * 32 * (kFp8 ? 64 : 128), vb = kb + kFewStageBytes / 2;
         const uint8_t* krow = smem + (kb - base);
         const uint8_t* sc = smem + L::kScales + st * 2 * C + sub * 32;  // K scales; V's are C further
-        uint32_t vis[MT][2], dead = 0;  // seen positions; positions without a finite V
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) vis[mt][0] = vis[mt][1] = 0xffffffffu;
+        uint32_t vis[2], dead = 0;  // seen positions; positions without a finite V
+        vis[0] = vis[1] = 0xffffffffu;
         if (tail) {
           const int pos = c0 + lane;
           bool bad = false;
@@ -316,22 +308,19 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
           const uint32_t poison = __ballot_sync(0xffffffffu, bad);
           dead = poison | __ballot_sync(0xffffffffu, pos >= end);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int x = 0; x < X; ++x) {
-              const int r = mt * 16 + x * 8 + g8;
-              vis[mt][x] = 0;
-              if (r < trows)
-                vis[mt][x] = (uint32_t)tree_bits(p.mask + (size_t)(row0 + (trow0 + r) / p.group) * p.words, p.words,
-                                                 nodes, c0 - prefix);
-              // a row that sees a V that is not finite has no finite result
-              if (vis[mt][x] & poison) l[mt][x] = __uint_as_float(0x7FFFFFFFu);
-            }
+          for (int x = 0; x < X; ++x) {
+            const int r = x * 8 + g8;
+            vis[x] = 0;
+            if (r < trows)
+              vis[x] = (uint32_t)tree_bits(p.mask + (size_t)(row0 + (trow0 + r) / p.group) * p.words, p.words,
+                                               nodes, c0 - prefix);
+            // a row that sees a V that is not finite has no finite result
+            if (vis[x] & poison) l[x] = __uint_as_float(0x7FFFFFFFu);
           }
           __syncwarp();
         }
         // ---- scores: four blocks of 8 positions
-        float s[MT][4][4];
+        float s[4][4];
         float sv[4][2];  // 8-bit: V's scales of this thread's columns
 #pragma unroll
         for (int nb = 0; nb < 4; ++nb) {
@@ -342,8 +331,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
               few_ldmatrix(kf, kb + k_at + nb * 1024 + (((hf * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
 #pragma unroll
               for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) few_mma<false>(s[mt][nb], qa[mt][hf * 2 + u], kf[2 * u], kf[2 * u + 1], hf == 0 && u == 0);
+                few_mma<false>(s[nb], qa[hf * 2 + u], kf[2 * u], kf[2 * u + 1], hf == 0 && u == 0);
             }
           } else {
             const uint4 u = *reinterpret_cast<const uint4*>(krow + k_at + nb * 512);
@@ -351,8 +339,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
               const uint32_t b0 = few_half2(w[kk], false), b1 = few_half2(w[kk], true);
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) few_mma<true>(s[mt][nb], qa[mt][kk], b0, b1, kk == 0);
+              few_mma<true>(s[nb], qa[kk], b0, b1, kk == 0);
             }
             // the scales of this thread's two columns, out of four neighbouring bytes
             const uint32_t ks = *reinterpret_cast<const uint32_t*>(sc + scale_at + nb * 8);
@@ -369,9 +356,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
               }
               sv[nb][e] = vf;
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int x = 0; x < X; ++x) s[mt][nb][2 * x + e] *= kf;
+              for (int x = 0; x < X; ++x) s[nb][2 * x + e] *= kf;
             }
           }
         }
@@ -382,70 +367,60 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
             for (int e = 0; e < 2; ++e) {
               const int at = nb * 8 + (kFp8 ? few_place(2 * t4 + e) : 2 * t4 + e);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                for (int x = 0; x < X; ++x)
-                  if (!((vis[mt][x] >> at) & 1)) s[mt][nb][2 * x + e] = -INFINITY;
-              }
+              for (int x = 0; x < X; ++x)
+                if (!((vis[x] >> at) & 1)) s[nb][2 * x + e] = -INFINITY;
             }
         }
         // ---- maxima
-        float mx[MT][2];
+        float mx[2];
         bool grow = false;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int x = 0; x < X; ++x) {
+          float t = -INFINITY;
 #pragma unroll
-          for (int x = 0; x < X; ++x) {
-            float t = -INFINITY;
-#pragma unroll
-            for (int nb = 0; nb < 4; ++nb) t = tree_max3(t, s[mt][nb][2 * x], s[mt][nb][2 * x + 1]);
-            mx[mt][x] = t * fac[mt][x];
-            grow |= mx[mt][x] > m[mt][x] + 8.f;
-          }
+          for (int nb = 0; nb < 4; ++nb) t = tree_max3(t, s[nb][2 * x], s[nb][2 * x + 1]);
+          mx[x] = t * fac[x];
+          grow |= mx[x] > m[x] + 8.f;
+        }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int x = 0; x < X; ++x) {
+            float t = mx[x];  // the row's four lanes agree
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            if (t > m[x] + 8.f) {
+              const float alpha = exp2_approx(m[x] - t);  // 0 for the first maximum
+              m[x] = t;
+              l[x] *= alpha;
 #pragma unroll
-            for (int x = 0; x < X; ++x) {
-              float t = mx[mt][x];  // the row's four lanes agree
-              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-              if (t > m[mt][x] + 8.f) {
-                const float alpha = exp2_approx(m[mt][x] - t);  // 0 for the first maximum
-                m[mt][x] = t;
-                l[mt][x] *= alpha;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  o[mt][i][2 * x] *= alpha;
-                  o[mt][i][2 * x + 1] *= alpha;
-                }
+              for (int i = 0; i < 8; ++i) {
+                o[i][2 * x] *= alpha;
+                o[i][2 * x + 1] *= alpha;
               }
             }
+          }
         }
         // ---- probabilities, as the A fragments of P V
-        uint32_t pa[MT][2][4] = {};
+        uint32_t pa[2][4] = {};
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int x = 0; x < X; ++x) {
+          const float mu = m[x] == -INFINITY ? 0.f : m[x];
 #pragma unroll
-          for (int x = 0; x < X; ++x) {
-            const float mu = m[mt][x] == -INFINITY ? 0.f : m[mt][x];
-#pragma unroll
-            for (int nb = 0; nb < 4; ++nb) {
-              float e0 = exp2_approx(fmaf(s[mt][nb][2 * x], fac[mt][x], -mu));
-              float e1 = exp2_approx(fmaf(s[mt][nb][2 * x + 1], fac[mt][x], -mu));
-              l[mt][x] += e0 + e1;
-              uint32_t& a = pa[mt][nb >> 1][(nb & 1) * 2 + x];
-              if (kFp8) {
-                e0 *= sv[nb][0];
-                e1 *= sv[nb][1];
-              }
-              if (!kFp8 || (!kPlain && wide)) {
-                __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-                a = *reinterpret_cast<uint32_t*>(&h);
-              } else {
-                __half2 h = __floats2half2_rn(e0, e1);
-                a = *reinterpret_cast<uint32_t*>(&h);
-              }
+          for (int nb = 0; nb < 4; ++nb) {
+            float e0 = exp2_approx(fmaf(s[nb][2 * x], fac[x], -mu));
+            float e1 = exp2_approx(fmaf(s[nb][2 * x + 1], fac[x], -mu));
+            l[x] += e0 + e1;
+            uint32_t& a = pa[nb >> 1][(nb & 1) * 2 + x];
+            if (kFp8) {
+              e0 *= sv[nb][0];
+              e1 *= sv[nb][1];
+            }
+            if (!kFp8 || (!kPlain && wide)) {
+              __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
+              a = *reinterpret_cast<uint32_t*>(&h);
+            } else {
+              __half2 h = __floats2half2_rn(e0, e1);
+              a = *reinterpret_cast<uint32_t*>(&h);
             }
           }
         }
@@ -460,8 +435,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
               few_ldmatrix_t(vf, vb + r * 128 + ((c ^ (r & 7)) << 4));
 #pragma unroll
               for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][dp * 2 + u], pa[mt][ks], vf[2 * u], vf[2 * u + 1]);
+                few_mma<false>(o[dp * 2 + u], pa[ks], vf[2 * u], vf[2 * u + 1]);
             }
           } else {
             uint2 v[2][2];  // [8 positions][column e]: dims 8 g8 .. 8 g8 + 7 of a position
@@ -482,11 +456,8 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
                   bf[0][q] = few_half2(w, false);
                   bf[1][q] = few_half2(w, true);
                 }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                  few_mma<true>(o[mt][d], pa[mt][ks], bf[0][0], bf[0][1]);
-                  few_mma<true>(o[mt][d + 1], pa[mt][ks], bf[1][0], bf[1][1]);
-                }
+                few_mma<true>(o[d], pa[ks], bf[0][0], bf[0][1]);
+                few_mma<true>(o[d + 1], pa[ks], bf[1][0], bf[1][1]);
               }
             } else {
               const __nv_bfloat162 f = tree_pow2(247);  // 2^120
@@ -501,8 +472,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
                   const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&z), f);
                   bf[q] = *reinterpret_cast<const uint32_t*>(&y);
                 }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) few_mma<false>(o[mt][d], pa[mt][ks], bf[0], bf[1]);
+                few_mma<false>(o[d], pa[ks], bf[0], bf[1]);
               }
             }
           }
@@ -531,24 +501,22 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, RT == 1 ? 4 : RT == 2 ? 
     const float unit = kFp8 && top_v ? e8m0_value(top_v) : 1.f;
     asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int x = 0; x < X; ++x) {
+      float t = l[x];
+      t += __shfl_xor_sync(0xffffffffu, t, 1);
+      t += __shfl_xor_sync(0xffffffffu, t, 2);
+      float* d = state + (warp * R + x * 8 + g8) * kTreePartial;
+      if (t4 == 0) *reinterpret_cast<float2*>(d) = make_float2(m[x], t);
 #pragma unroll
-      for (int x = 0; x < X; ++x) {
-        float t = l[mt][x];
-        t += __shfl_xor_sync(0xffffffffu, t, 1);
-        t += __shfl_xor_sync(0xffffffffu, t, 2);
-        float* d = state + (warp * R + mt * 16 + x * 8 + g8) * kTreePartial;
-        if (t4 == 0) *reinterpret_cast<float2*>(d) = make_float2(m[mt][x], t);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (!kFp8) {  // dims 8 i + 2 t4 (+ 1)
-            *reinterpret_cast<float2*>(d + 2 + 8 * i + 2 * t4) = make_float2(o[mt][i][2 * x], o[mt][i][2 * x + 1]);
-          } else {  // in units of V's largest scale; dims 16 t4 + i and 8 more
-            d[2 + 16 * t4 + i] = o[mt][i][2 * x] * unit;
-            d[2 + 16 * t4 + 8 + i] = o[mt][i][2 * x + 1] * unit;
-          }
+      for (int i = 0; i < 8; ++i) {
+        if (!kFp8) {  // dims 8 i + 2 t4 (+ 1)
+          *reinterpret_cast<float2*>(d + 2 + 8 * i + 2 * t4) = make_float2(o[i][2 * x], o[i][2 * x + 1]);
+        } else {  // in units of V's largest scale; dims 16 t4 + i and 8 more
+          d[2 + 16 * t4 + i] = o[i][2 * x] * unit;
+          d[2 + 16 * t4 + 8 + i] = o[i][2 * x + 1] * unit;
         }
       }
+    }
     asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
     float* joined = state + kFewWarps * R * kTreePartial;  // in a cluster: [R][66], for its other CTAs
     static_assert((kFewWarps + 1) * R * kTreePartial * 4 <= kFewStages * kFewStageBytes, "the states fit over the ring");
