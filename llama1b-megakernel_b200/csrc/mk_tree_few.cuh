@@ -135,8 +135,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
   const int trows = min(R, nodes * p.group - trow0);
   const int end = prefix + nodes;
   const int p1 = min(end, p0 + p.split_len);
-  if (trows <= 0) return;
-  if (p0 >= p1) return tree_leave(p);
+  if (trows <= 0 || p0 >= p1) return;
   const int nchunks = (p1 - p0 + C - 1) / C;
   auto wait_all = [&](uint32_t bar, uint32_t parity) {
     return (bool)__all_sync(0xffffffffu, tree_wait(bar, parity, abort_word, p.error));
