@@ -55,7 +55,7 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 // positions drift apart. 4 sequences of 256 nodes at 16,000: 211 us whole, 247 in
 // four.)
 constexpr int kTreeFewRows = 16;
-constexpr int kTreeCluster = 8;  // the portable size
+using mk::kTreeCluster;
 struct TreePlan {
   int few;  // eights of rows in a tile of the mma.sync kernel (1, 2), 0: tcgen05
   int tiles, splits, len;
@@ -311,6 +311,7 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   const int64_t need = mk_tree_attention_workspace(batch, num_q_heads, nkv, max_nodes, max_len);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(MK_EINVAL, "workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
+  if (need > 0 && !aligned16(workspace)) return fail(MK_EINVAL, "workspace must be 16-byte aligned");
   if (rows == 0) return MK_OK;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.cu_nodes = cu_nodes;
@@ -322,6 +323,7 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   p.max_len = max_len;
   p.NQ = num_q_heads;
   p.group = group;
+  p.group_log = group == 8 ? 3 : group >> 1;
   p.scale = scale;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
@@ -341,7 +343,7 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   const dim3 grid(p.tiles * p.splits, nkv, batch);
   MK_CUDA(fp8 ? launch_tree<true>(tp, plan.few, grid, st) : launch_tree<false>(tp, plan.few, grid, st));
   if (p.splits > 1 && !p.cluster)
-    MK_CUDA(launch_pdl(mk::tree_merge_kernel, dim3((max_nodes * group + 7) / 8, nkv, batch), dim3(256), 0, st, p));
+    MK_CUDA(launch_pdl(mk::tree_merge_kernel, dim3((max_nodes * group + 16 * mk::kMergeRows - 1) / (16 * mk::kMergeRows), nkv, batch), dim3(256), 0, st, p));
   return MK_OK;
 }
 

@@ -56,7 +56,8 @@ constexpr int kTreeRows = 128;     // rows of a tile (the MMA's M)
 constexpr int kTreeBlock = 128;    // positions of a block
 constexpr int kTreeHalf = 64;      // of a step of the softmax
 constexpr int kTreeThreads = 448;  // 2 x 4 softmax warps, 4 block warps, producer, issuer
-constexpr int kTreePartial = 66;   // m, l, o[64]
+constexpr int kTreePartial = 68;   // o[64], m, l, two to align
+constexpr int kTreeCluster = 8;    // ranges that may join in a cluster: the portable size
 constexpr uint32_t kTreeTmem = 256;  // columns: S (and P over it) 2 x 64, O 2 x 64
 constexpr uint32_t kTreeTileBytes = kTreeBlock * 128;  // a bf16 K or V block (and the Q tile)
 constexpr uint32_t kTreeRawBytes = kTreeBlock * 64;    // an 8-bit one
@@ -79,7 +80,8 @@ struct TreeParams {
   const int* cu_nodes;              // [batch + 1]
   const unsigned long long* mask;   // [rows][words]
   const int* prefix;                // [batch]
-  int rows, words, max_nodes, max_len, NQ, group;
+  int rows, words, max_nodes, max_len, NQ;
+  int group, group_log;             // query heads of a K/V head: 1, 2, 4 or 8
   int box;                          // rows of a TMA box
   int tiles, splits, split_len;     // split_len: a multiple of kTreeBlock
   int cluster;                      // the ranges of a tile are a cluster (else: partials in work)
@@ -368,14 +370,60 @@ __device__ __forceinline__ void tree_item(const TreeParams& p, int& tile, int& s
   }
 }
 
-// One row's result, two dims a lane: o not yet divided by the sum.
-__device__ __forceinline__ void tree_write(const TreeParams& p, int row, int head, int lane, float m, float sum, float o0, float o1) {
-  const bool any = sum != 0.f;  // NaN counts as something
-  reinterpret_cast<__nv_bfloat162*>(p.out + ((size_t)row * p.NQ + head) * 64)[lane] =
-      __floats2bfloat162_rn(any ? o0 / sum : 0.f, any ? o1 / sum : 0.f);
-  if (p.lse && lane == 0)
-    p.lse[(size_t)row * p.NQ + head] = any ? (m == -INFINITY ? 0.f : m) * 0.6931471805599453f + logf(sum) : -INFINITY;
+// lse of a row out of its maximum, in powers of two, and sum (not 0); lg2.approx is
+// within 2^-22 of 1 or of the logarithm.
+__device__ __forceinline__ float tree_lse(float m, float sum) {
+  float lg;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(sum));
+  return ((m == -INFINITY ? 0.f : m) + lg) * 0.6931471805599453f;
 }
+__device__ __forceinline__ float tree_inverse(float sum) {  // within an ulp
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(sum));
+  return y;
+}
+
+// A row's partials joined, four dims a lane (16 lanes a row), four partials at a time so
+// that all their loads are on their way before the first is used. (One lane group at a
+// time, in a loop of dependent loads, with divisions: 1,400 cycles a row and warp.)
+struct TreeRow {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  // load(q, ml, v): partial q's (m, l) and this lane's dims
+  template <typename Load>
+  __device__ __forceinline__ void add(int n, Load load) {
+    for (int q0 = 0; q0 < n; q0 += 4) {
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        ml[q] = make_float2(-INFINITY, 0.f);
+        v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (q0 + q < n) load(q0 + q, ml[q], v[q]);
+      }
+      const float top = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+      const float mu = top == -INFINITY ? 0.f : top, was = exp2_approx(m - mu);
+      m = top;
+      l *= was;
+      o = make_float4(o.x * was, o.y * was, o.z * was, o.w * was);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float f = exp2_approx(ml[q].x - mu);
+        l = fmaf(ml[q].y, f, l);
+        o = make_float4(fmaf(v[q].x, f, o.x), fmaf(v[q].y, f, o.y), fmaf(v[q].z, f, o.z), fmaf(v[q].w, f, o.w));
+      }
+    }
+  }
+  __device__ __forceinline__ void write(const TreeParams& p, int row, int head, int lane16) const {
+    const bool any = l != 0.f;  // NaN counts as something
+    const float f = any ? tree_inverse(l) : 0.f;
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(any ? o.x * f : 0.f, any ? o.y * f : 0.f),
+                           __floats2bfloat162_rn(any ? o.z * f : 0.f, any ? o.w * f : 0.f)};
+    *reinterpret_cast<uint2*>(p.out + ((size_t)row * p.NQ + head) * 64 + 4 * lane16) =
+        make_uint2(*reinterpret_cast<uint32_t*>(&h[0]), *reinterpret_cast<uint32_t*>(&h[1]));
+    if (p.lse && lane16 == 0) p.lse[(size_t)row * p.NQ + head] = any ? tree_lse(m, l) : -INFINITY;
+  }
+};
 
 __device__ __forceinline__ void tree_cluster_sync() {
   __syncwarp();
@@ -391,31 +439,19 @@ __device__ __forceinline__ void tree_cluster_sync() {
 __device__ __forceinline__ void tree_join(const TreeParams& p, uint32_t part, int ranges, int split, int warp, int warps,
                                           int lane, int row0, int trow0, int trows, int g) {
   tree_cluster_sync();
-  for (int r = warp < warps ? split * warps + warp : trows; r < trows; r += ranges * warps) {
-    auto remote = [&](int q) {
+  const int lane16 = lane & 15;
+  for (int r = warp < warps ? 2 * (split * warps + warp) + (lane >> 4) : trows; r < trows; r += 2 * ranges * warps) {
+    TreeRow t;
+    t.add(ranges, [&](int q, float2& ml, float4& v) {
       uint32_t a;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(part + r * kTreePartial * 4), "r"(q));
-      return a;
-    };
-    auto load = [](uint32_t a) {
-      float2 v;
-      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
-      return v;
-    };
-    float m = -INFINITY;
-    for (int q = 0; q < ranges; ++q) m = fmaxf(m, load(remote(q)).x);
-    const float mu = m == -INFINITY ? 0.f : m;
-    float sum = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int q = 0; q < ranges; ++q) {
-      const uint32_t a = remote(q);
-      const float2 ml = load(a), v = load(a + 8 + 8 * lane);
-      const float f = exp2_approx(ml.x - mu);
-      sum = fmaf(ml.y, f, sum);
-      o0 = fmaf(v.x, f, o0);
-      o1 = fmaf(v.y, f, o1);
-    }
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "r"(a + 256));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                   : "r"(a + 16 * lane16));
+    });
     const int pr = trow0 + r;
-    tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, m, sum, o0, o1);
+    t.write(p, row0 + (pr >> p.group_log), g * p.group + (pr & (p.group - 1)), lane16);
   }
   tree_cluster_sync();  // nobody leaves while another may still read its partials
 }
@@ -432,13 +468,13 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   tree_item(p, tile, split);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-  // barriers: full[3], empty[3], ready[3], free[3], q, s[2], p[2], o; then words
+  // barriers: full[3], empty[3], ready[3], free[3], -, s[2], p[2], o; then words
   const uint32_t bars = base + L::kBars;
   auto full = [&](int i) { return bars + 8 * i; };
   auto empty = [&](int i) { return bars + 24 + 8 * i; };
   auto ready = [&](int i) { return bars + 48 + 8 * i; };
   auto free_ = [&](int i) { return bars + 72 + 8 * i; };
-  const uint32_t b_q = bars + 96, b_o = bars + 136;            // Q is in place; all O are complete
+  const uint32_t b_o = bars + 136;                             // all O are complete
   // of the first and second halves of the blocks, a phase per block
   auto b_s = [&](int half) { return bars + 104 + 8 * half; };  // S is in TMEM (and O has the block before)
   auto b_p = [&](int half) { return bars + 120 + 8 * half; };  // P is in TMEM
@@ -460,7 +496,9 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     init(b_s(1), 1);
     init(b_o, 1);
     *abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncthreads();  // the producer and the block warps need no other
   const int p0 = split * p.split_len;
   pdl_wait();
   // the producer's first page ids and the sequence's lengths are on their way together
@@ -486,14 +524,32 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const int halves = (p1 - p0 + kTreeHalf - 1) / kTreeHalf;
   const int active = (trows + 31) >> 5;  // softmax warps with a row
   if (threadIdx.x == 0) {
-    init(b_q, active);
     init(b_p(0), active);
     init(b_p(1), active);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  // while the first copies are under way, thread r of the first softmax brings row r of Q in
+  const int pr = trow0 + (threadIdx.x & 127);  // a softmax thread's row
+  const bool real = warp < 8 && pr < nodes * p.group;
+  const int row = row0 + (real ? pr >> p.group_log : 0), head = g * p.group + (pr & (p.group - 1));
+  if (warp < active && warp < 4) {
+    const uint4* src = reinterpret_cast<const uint4*>(p.q + ((size_t)row * p.NQ + head) * 64);
+    uint8_t* dst = smem + L::kQ + threadIdx.x * 128;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      uint4 u = real ? src[c] : make_uint4(0, 0, 0, 0);
+      if (kFp8)  // the order of dims that tree_decode leaves: 0, 2, 1, 3
+        u = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632),
+                       __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
+      *reinterpret_cast<uint4*>(dst + ((c ^ (threadIdx.x & 7)) << 4)) = u;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp < 8 || warp == 13) {  // Q, TMEM and the barriers of P are there
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("bar.sync 2, 288;" ::: "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  }
   const uint32_t tmem = words[1];
   // of the first and second halves of the blocks
   auto t_s = [&](int half) { return tmem + 64 * half; };  // P lies over the first 32 columns of S
@@ -566,7 +622,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       tree_commit(b_s(half));
       return true;
     };
-    bool ok = wait_all(b_q, 0) && scores(0) && (halves < 2 || scores(1));
+    bool ok = scores(0) && (halves < 2 || scores(1));
     for (int j = 0; j < nblocks && ok; ++j) {
       if (++next == L::kReady) {
         next = 0;
@@ -672,25 +728,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     }
   } else if ((warp & 3) < active) {
     // ---- softmax, one thread per row; warps 0-3 the first halves, 4-7 the second
-    const int half = warp >> 2, r = threadIdx.x & 127, pr = trow0 + r;
-    const bool real = r < trows;
-    const int node = real ? pr / p.group : 0, head = g * p.group + (real ? pr % p.group : 0);
-    const int row = row0 + node;
-    if (half == 0) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + ((size_t)row * p.NQ + head) * 64);
-      uint8_t* dst = smem + L::kQ + r * 128;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint4 u = real ? src[c] : make_uint4(0, 0, 0, 0);
-        if (kFp8)  // the order of dims that tree_decode leaves: 0, 2, 1, 3
-          u = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632),
-                         __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
-        *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) = u;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) tree_arrive(b_q);
-    }
+    const int half = warp >> 2, r = threadIdx.x & 127;
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = t_s(half) + tl, o_at = t_o(half) + tl;
     const float c2 = p.scale * 1.4426950408889634f;  // scores in powers of two
@@ -797,37 +835,39 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     for (; j < plain && ok; ++j) ok = step(std::false_type{}, j);
 #pragma unroll 1
     for (; j < mine && ok; ++j) ok = step(std::true_type{}, j);
-    // ---- the two softmaxes joined: the second's (m, l) by way of shared memory
+    // ---- the two softmaxes joined, (m, l) by way of shared memory; each writes half the dims
     if (ok) ok = wait_all(b_o, 0);  // no MMA reads Q any more
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     float2* ml = reinterpret_cast<float2*>(smem + L::kQ);
-    if (half) ml[r] = make_float2(m, l);
+    ml[threadIdx.x] = make_float2(m, l);
     asm volatile("bar.sync 1, %0;" ::"r"(64 * active) : "memory");
-    if (ok && !half) {
-      const float2 other = ml[r];
+    if (ok) {
       const bool two = halves > 1;
-      const float m1 = two ? other.x : -INFINITY;
-      const float top = fmaxf(m, m1), mu = top == -INFINITY ? 0.f : top;
-      const float a = exp2_approx(m - mu), a1 = exp2_approx(m1 - mu);
-      const float sum = two ? l * a + other.y * a1 : l * a;
+      const float2 x0 = ml[r], x1 = two ? ml[128 + r] : make_float2(-INFINITY, 0.f);
+      const float top = fmaxf(x0.x, x1.x), mu = top == -INFINITY ? 0.f : top;
+      const float a0 = exp2_approx(x0.x - mu), a1 = exp2_approx(x1.x - mu);
+      const float sum = fmaf(x1.y, a1, x0.y * a0);
       const bool whole = p.splits == 1, any = sum != 0.f;  // NaN counts as something
-      const float f = !whole ? a : any ? a / sum : 0.f, f1 = !whole ? a1 : any ? a1 / sum : 0.f;
+      const float inv = !whole ? 1.f : any ? tree_inverse(sum) : 0.f, f0 = a0 * inv, f1 = a1 * inv;
       // in a cluster the partials lie over the blocks, which no copy and no MMA needs any more
       float* part = p.cluster ? reinterpret_cast<float*>(smem + L::kTiles) + r * kTreePartial
                               : p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
-      if (real && !whole) *reinterpret_cast<float2*>(part) = make_float2(top, sum);
-      if (real && whole && p.lse)
-        p.lse[(size_t)row * p.NQ + head] = any ? mu * 0.6931471805599453f + logf(sum) : -INFINITY;
+      if (real && !half) {
+        if (!whole)
+          *reinterpret_cast<float2*>(part + 64) = make_float2(top, sum);
+        else if (p.lse)
+          p.lse[(size_t)row * p.NQ + head] = any ? tree_lse(mu, sum) : -INFINITY;
+      }
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 2 * half; c < 2 * half + 2; ++c) {
         uint32_t w[16], w1[16];
         float o[16];
         __syncwarp();
-        tree_ld16(o_at + 16 * c, w);
+        tree_ld16(t_o(0) + tl + 16 * c, w);
         if (two) tree_ld16(t_o(1) + tl + 16 * c, w1);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float x = __uint_as_float(w[i]) * f;
+          const float x = __uint_as_float(w[i]) * f0;
           o[kFp8 && (i & 3) % 3 ? (i ^ 3) : i] = two ? fmaf(__uint_as_float(w1[i]), f1, x) : x;
         }
         if (real && whole) {
@@ -837,14 +877,15 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
             uint32_t v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              __nv_bfloat162 h = __floats2bfloat162_rn(any ? o[8 * q + 2 * e] : 0.f, any ? o[8 * q + 2 * e + 1] : 0.f);
-              v[e] = *reinterpret_cast<uint32_t*>(&h);
+              __nv_bfloat162 h = __floats2bfloat162_rn(o[8 * q + 2 * e], o[8 * q + 2 * e + 1]);
+              v[e] = any ? *reinterpret_cast<uint32_t*>(&h) : 0u;
             }
             dst[q] = make_uint4(v[0], v[1], v[2], v[3]);
           }
         } else if (real) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) reinterpret_cast<float2*>(part + 2 + 16 * c)[i] = make_float2(o[2 * i], o[2 * i + 1]);
+          for (int i = 0; i < 4; ++i)
+            reinterpret_cast<float4*>(part + 16 * c)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
     }
@@ -860,32 +901,29 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
               trows, g);
 }
 
-// One warp per (node, query head): the splits' partials joined, in split order.
+// The splits' partials joined, in split order: a warp takes kMergeRows pairs of rows
+// (node, query head).
+constexpr int kMergeRows = 2;
 __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeParams p) {
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, g = blockIdx.y, b = blockIdx.z;
-  const int pr = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane16 = threadIdx.x & 15, g = blockIdx.y, b = blockIdx.z;
   int row0, nodes, prefix;
-  if (!tree_sequence(p, b, row0, nodes, prefix) || pr >= nodes * p.group) return;
+  if (!tree_sequence(p, b, row0, nodes, prefix)) return;
   const int splits = (prefix + nodes + p.split_len - 1) / p.split_len;
   const size_t stride = (size_t)p.max_nodes * p.group * kTreePartial;
-  const float* src = p.work + ((size_t)b * p.kv.NKV + g) * p.splits * stride + (size_t)pr * kTreePartial;
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, src[s * stride]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float* q = src + s * stride;
-    const float a = exp2_approx(q[0] - mu);
-    const float2 v = *reinterpret_cast<const float2*>(q + 2 + 2 * lane);
-    l = fmaf(q[1], a, l);
-    o0 = fmaf(v.x, a, o0);
-    o1 = fmaf(v.y, a, o1);
+  const float* work = p.work + ((size_t)b * p.kv.NKV + g) * p.splits * stride;
+  for (int i = 0; i < kMergeRows; ++i) {
+    const int pr = (blockIdx.x * kMergeRows + i) * 16 + (threadIdx.x >> 4);
+    if (pr >= nodes * p.group) return;
+    TreeRow t;
+    t.add(splits, [&](int q, float2& ml, float4& v) {
+      const float* src = work + q * stride + (size_t)pr * kTreePartial;
+      ml = *reinterpret_cast<const float2*>(src + 64);
+      v = *reinterpret_cast<const float4*>(src + 4 * lane16);
+    });
+    t.write(p, row0 + (pr >> p.group_log), g * p.group + (pr & (p.group - 1)), lane16);
   }
-  tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, m, l, o0, o1);
 }
 
 }  // namespace mk

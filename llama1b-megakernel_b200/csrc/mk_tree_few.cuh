@@ -202,7 +202,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
       const int r = x * 8 + g8, pr = trow0 + r;
       const bool real = r < trows;
       const uint32_t* q = reinterpret_cast<const uint32_t*>(
-          p.q + ((size_t)(row0 + (real ? pr / p.group : 0)) * p.NQ + g * p.group + (real ? pr % p.group : 0)) * 64);
+          p.q + ((size_t)(row0 + (real ? pr >> p.group_log : 0)) * p.NQ + g * p.group + (pr & (p.group - 1))) * 64);
       if (!kFp8) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {  // dims 16 kk + 2 t4 (+ 1), and 8 more
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
             const int r = x * 8 + g8;
             vis[x] = 0;
             if (r < trows)
-              vis[x] = (uint32_t)tree_bits(p.mask + (size_t)(row0 + (trow0 + r) / p.group) * p.words, p.words,
+              vis[x] = (uint32_t)tree_bits(p.mask + (size_t)(row0 + ((trow0 + r) >> p.group_log)) * p.words, p.words,
                                                nodes, c0 - prefix);
             // a row that sees a V that is not finite has no finite result
             if (vis[x] & poison) l[x] = __uint_as_float(0x7FFFFFFFu);
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
     }
 
     // ---- the four warps joined; their states lie over the ring, which nobody reads any more
-    float* state = reinterpret_cast<float*>(smem);  // [warp][R][66]
+    float* state = reinterpret_cast<float*>(smem);  // [warp][R][kTreePartial]
     const float unit = kFp8 && top_v ? e8m0_value(top_v) : 1.f;
     asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
 #pragma unroll
@@ -505,48 +505,41 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
       t += __shfl_xor_sync(0xffffffffu, t, 1);
       t += __shfl_xor_sync(0xffffffffu, t, 2);
       float* d = state + (warp * R + x * 8 + g8) * kTreePartial;
-      if (t4 == 0) *reinterpret_cast<float2*>(d) = make_float2(m[x], t);
+      if (t4 == 0) *reinterpret_cast<float2*>(d + 64) = make_float2(m[x], t);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (!kFp8) {  // dims 8 i + 2 t4 (+ 1)
-          *reinterpret_cast<float2*>(d + 2 + 8 * i + 2 * t4) = make_float2(o[i][2 * x], o[i][2 * x + 1]);
+          *reinterpret_cast<float2*>(d + 8 * i + 2 * t4) = make_float2(o[i][2 * x], o[i][2 * x + 1]);
         } else {  // in units of V's largest scale; dims 16 t4 + i and 8 more
-          d[2 + 16 * t4 + i] = o[i][2 * x] * unit;
-          d[2 + 16 * t4 + 8 + i] = o[i][2 * x + 1] * unit;
+          d[16 * t4 + i] = o[i][2 * x] * unit;
+          d[16 * t4 + 8 + i] = o[i][2 * x + 1] * unit;
         }
       }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
-    float* joined = state + kFewWarps * R * kTreePartial;  // in a cluster: [R][66], for its other CTAs
+    float* joined = state + kFewWarps * R * kTreePartial;  // in a cluster: [R], for its other CTAs
     static_assert((kFewWarps + 1) * R * kTreePartial * 4 <= kFewStages * kFewStageBytes, "the states fit over the ring");
-    for (int r = warp; ok && r < trows; r += kFewWarps) {  // a lane has two dims
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, state[(w * R + r) * kTreePartial]);
-      const float mu = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) {
+    const int lane16 = lane & 15;
+    for (int r = 2 * warp + (lane >> 4); ok && r < trows; r += 2 * kFewWarps) {
+      TreeRow t;
+      t.add(kFewWarps, [&](int w, float2& ml, float4& v) {
         const float* d = state + (w * R + r) * kTreePartial;
-        const float a = exp2_approx(d[0] - mu);
-        const float2 v = *reinterpret_cast<const float2*>(d + 2 + 2 * lane);
-        sum = fmaf(d[1], a, sum);
-        o0 = fmaf(v.x, a, o0);
-        o1 = fmaf(v.y, a, o1);
-      }
+        ml = *reinterpret_cast<const float2*>(d + 64);
+        v = *reinterpret_cast<const float4*>(d + 4 * lane16);
+      });
       const int pr = trow0 + r;
       if (p.splits > 1) {
         float* dst = p.cluster ? joined + r * kTreePartial
                                : p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
-        if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(top, sum);
-        *reinterpret_cast<float2*>(dst + 2 + 2 * lane) = make_float2(o0, o1);
+        if (lane16 == 0) *reinterpret_cast<float2*>(dst + 64) = make_float2(t.m, t.l);
+        *reinterpret_cast<float4*>(dst + 4 * lane16) = t.o;
       } else {
-        tree_write(p, row0 + pr / p.group, g * p.group + pr % p.group, lane, top, sum, o0, o1);
+        t.write(p, row0 + (pr >> p.group_log), g * p.group + (pr & (p.group - 1)), lane16);
       }
     }
   }
   if (p.cluster)
-    tree_join(p, base + kFewWarps * R * kTreePartial * 4, (end + p.split_len - 1) / p.split_len, split, warp, kFewWarps, lane,
+    tree_join(p, base + kFewWarps * R * kTreePartial * 4, (end + p.split_len - 1) / p.split_len, split, warp, kFewWarps + 1, lane,
               row0, trow0, trows, g);
 }
 
