@@ -430,15 +430,14 @@ __device__ __forceinline__ void tree_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Join the ranges of a cluster: every CTA with a range has its partials
-// [rows][kTreePartial] at shared address `part` (the same in each); the first `warps`
-// warps take rows of their own. All threads of these CTAs pass the two barriers; a CTA
-// without a range has left, as they wait for threads that have not exited only (kept to
-// the end, such CTAs took the slots of others: 17.4 us for 8 sequences of 25 nodes
-// behind 0 to 1,111 positions, 15.5 so).
+// Join the ranges of a cluster, after tree_cluster_sync: every CTA with a range has its
+// partials [rows][kTreePartial] at shared address `part` (the same in each) and writes a
+// share of the rows, its first `warps` warps two at a time. All threads of these CTAs
+// pass the barriers; a CTA without a range has left, as they wait for threads that have
+// not exited only (kept to the end, such CTAs took the slots of others: 17.4 us for 8
+// sequences of 25 nodes behind 0 to 1,111 positions, 15.5 so).
 __device__ __forceinline__ void tree_join(const TreeParams& p, uint32_t part, int ranges, int split, int warp, int warps,
                                           int lane, int row0, int trow0, int trows, int g) {
-  tree_cluster_sync();
   const int lane16 = lane & 15;
   for (int r = warp < warps ? 2 * (split * warps + warp) + (lane >> 4) : trows; r < trows; r += 2 * ranges * warps) {
     TreeRow t;
@@ -528,20 +527,25 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     init(b_p(1), active);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // while the first copies are under way, thread r of the first softmax brings row r of Q in
-  const int pr = trow0 + (threadIdx.x & 127);  // a softmax thread's row
-  const bool real = warp < 8 && pr < nodes * p.group;
-  const int row = row0 + (real ? pr >> p.group_log : 0), head = g * p.group + (pr & (p.group - 1));
-  if (warp < active && warp < 4) {
-    const uint4* src = reinterpret_cast<const uint4*>(p.q + ((size_t)row * p.NQ + head) * 64);
-    uint8_t* dst = smem + L::kQ + threadIdx.x * 128;
+  // while the first copies are under way, the softmax warps bring Q in, 16 rows each
+  // and eight lanes a row (a row a lane is 32 cache lines a load: 1,000 cycles more)
+  if (warp < 8) {
+    uint4 u[4];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      uint4 u = real ? src[c] : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) {
+      const int at = trow0 + warp * 16 + i * 4 + (lane >> 3);
+      u[i] = make_uint4(0, 0, 0, 0);
+      if (at < trow0 + trows)
+        u[i] = reinterpret_cast<const uint4*>(
+            p.q + ((size_t)(row0 + (at >> p.group_log)) * p.NQ + g * p.group + (at & (p.group - 1))) * 64)[lane & 7];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = warp * 16 + i * 4 + (lane >> 3);
       if (kFp8)  // the order of dims that tree_decode leaves: 0, 2, 1, 3
-        u = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632),
-                       __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
-      *reinterpret_cast<uint4*>(dst + ((c ^ (threadIdx.x & 7)) << 4)) = u;
+        u[i] = make_uint4(__byte_perm(u[i].x, u[i].y, 0x5410), __byte_perm(u[i].x, u[i].y, 0x7632),
+                          __byte_perm(u[i].z, u[i].w, 0x5410), __byte_perm(u[i].z, u[i].w, 0x7632));
+      *reinterpret_cast<uint4*>(smem + L::kQ + at * 128 + (((lane & 7) ^ (at & 7)) << 4)) = u[i];
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -729,6 +733,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   } else if ((warp & 3) < active) {
     // ---- softmax, one thread per row; warps 0-3 the first halves, 4-7 the second
     const int half = warp >> 2, r = threadIdx.x & 127;
+    const int row = row0 + (r < trows ? (trow0 + r) >> p.group_log : 0);
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = t_s(half) + tl, o_at = t_o(half) + tl;
     const float c2 = p.scale * 1.4426950408889634f;  // scores in powers of two
@@ -849,20 +854,20 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       const float sum = fmaf(x1.y, a1, x0.y * a0);
       const bool whole = p.splits == 1, any = sum != 0.f;  // NaN counts as something
       const float inv = !whole ? 1.f : any ? tree_inverse(sum) : 0.f, f0 = a0 * inv, f1 = a1 * inv;
-      // in a cluster the partials lie over the blocks, which no copy and no MMA needs any more
-      float* part = p.cluster ? reinterpret_cast<float*>(smem + L::kTiles) + r * kTreePartial
-                              : p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + pr) * kTreePartial;
-      if (real && !half) {
+      // the row's result or partial goes over the blocks, which no copy and no MMA needs any
+      // more, and leaves from there with neighbouring lanes on neighbouring addresses
+      uint8_t* tiles = smem + L::kTiles;
+      float* part = reinterpret_cast<float*>(tiles) + r * kTreePartial;
+      if (!half) {
         if (!whole)
           *reinterpret_cast<float2*>(part + 64) = make_float2(top, sum);
-        else if (p.lse)
-          p.lse[(size_t)row * p.NQ + head] = any ? tree_lse(mu, sum) : -INFINITY;
+        else if (p.lse && r < trows)
+          p.lse[(size_t)row * p.NQ + g * p.group + ((trow0 + r) & (p.group - 1))] = any ? tree_lse(mu, sum) : -INFINITY;
       }
 #pragma unroll 1
       for (int c = 2 * half; c < 2 * half + 2; ++c) {
         uint32_t w[16], w1[16];
         float o[16];
-        __syncwarp();
         tree_ld16(t_o(0) + tl + 16 * c, w);
         if (two) tree_ld16(t_o(1) + tl + 16 * c, w1);
 #pragma unroll
@@ -870,8 +875,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
           const float x = __uint_as_float(w[i]) * f0;
           o[kFp8 && (i & 3) % 3 ? (i ^ 3) : i] = two ? fmaf(__uint_as_float(w1[i]), f1, x) : x;
         }
-        if (real && whole) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)row * p.NQ + head) * 64 + 16 * c);
+        if (whole) {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             uint32_t v[4];
@@ -880,9 +884,9 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
               __nv_bfloat162 h = __floats2bfloat162_rn(o[8 * q + 2 * e], o[8 * q + 2 * e + 1]);
               v[e] = any ? *reinterpret_cast<uint32_t*>(&h) : 0u;
             }
-            dst[q] = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(tiles + r * 128 + (((2 * c + q) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
           }
-        } else if (real) {
+        } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             reinterpret_cast<float4*>(part + 16 * c)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -891,14 +895,30 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  if (p.cluster)
+    tree_cluster_sync();
+  else
+    __syncthreads();
   if (warp == 13) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTreeTmem) : "memory");
   }
-  if (p.cluster)
+  if (p.cluster) {
     tree_join(p, base + L::kTiles, (end + p.split_len - 1) / p.split_len, split, warp, kTreeThreads / 32, lane, row0, trow0,
               trows, g);
+  } else if (p.splits > 1) {
+    float4* dst = reinterpret_cast<float4*>(
+        p.work + ((((size_t)b * kv.NKV + g) * p.splits + split) * p.max_nodes * p.group + trow0) * kTreePartial);
+    for (int i = threadIdx.x; i < trows * (kTreePartial / 4); i += kTreeThreads)
+      dst[i] = reinterpret_cast<const float4*>(smem + L::kTiles)[i];
+  } else {
+    for (int i = threadIdx.x; i < trows * 8; i += kTreeThreads) {
+      const int r = i >> 3, pr = trow0 + r;
+      reinterpret_cast<uint4*>(p.out + ((size_t)(row0 + (pr >> p.group_log)) * p.NQ + g * p.group + (pr & (p.group - 1))) *
+                                           64)[i & 7] =
+          *reinterpret_cast<const uint4*>(smem + L::kTiles + r * 128 + (((i & 7) ^ (r & 7)) << 4));
+    }
+  }
 }
 
 // The splits' partials joined, in split order: a warp takes kMergeRows pairs of rows

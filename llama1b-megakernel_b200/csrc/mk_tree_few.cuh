@@ -538,9 +538,11 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
       }
     }
   }
-  if (p.cluster)
+  if (p.cluster) {
+    tree_cluster_sync();
     tree_join(p, base + kFewWarps * R * kTreePartial * 4, (end + p.split_len - 1) / p.split_len, split, warp, kFewWarps + 1, lane,
               row0, trow0, trows, g);
+  }
 }
 
 }  // namespace mk
