@@ -45,15 +45,22 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 
 // Which kernel a call takes and how the positions of a sequence are split over its
 // CTAs. Up to kTreeFewRows rows (nodes x query heads of a K/V head) go to the
-// mma.sync kernel, in one tile of 8 or 16; more to the tcgen05 kernel in tiles of
-// 128. A launch of n CTAs, c to an SM, takes about ceil(n / (c SMs)) waves of one
-// range each; a range costs its length and a fixed part (launch, first bytes, the
-// store). Joining ranges costs a little in a cluster (up to eight ranges) and a
-// launch and a trip through the workspace otherwise. The cheapest cut is taken.
-// (Splitting a launch that fills the GPU once, to even out the SMs, does not pay: the
-// CTAs of a cluster wait for one another's slots, and the row tiles that share
-// positions drift apart. 4 sequences of 256 nodes at 16,000: 211 us whole, 247 in
-// four.)
+// mma.sync kernel, in one tile of 8 or 16; more to the tcgen05 kernel in tiles of 128.
+// (16 rows at 32 x 4096: 44.8 us against 45.0 of bf16, 39 against 56 of 8-bit rows; 20
+// rows need two of the small tiles: 64 against 45, 57 against 56.)
+//
+// The cut with the least estimated time is taken, in tenths of a microsecond, fitted to
+// launches of 1 to 50 sequences: a CTA costs a fixed part (first bytes, the store) and
+// its share of 128 positions, more when the SM has another one; the launch costs as many
+// waves of that as it fills; ranges that join cost a little in a cluster (up to eight
+// ranges) and a launch and a trip through the workspace otherwise. 10 sequences of 25
+// nodes behind 2,000 to 4,000 positions: 38 us whole, 34 in two, 27 in three, 29 in four.
+//
+// No cut is finer than it takes to fill the slots once. What the estimate promises
+// beyond that, ragged lengths eat, as the hardware hands out whole CTAs more evenly than
+// the waves here (20 such sequences: 41 us whole, 39 in two, 45 in three), and row tiles
+// that share positions drift apart (4 sequences of 256 nodes at 16,000: 198 us whole, 216
+// in two).
 constexpr int kTreeFewRows = 16;
 using mk::kTreeCluster;
 struct TreePlan {
@@ -67,18 +74,21 @@ TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
   const int tile_rows = t.few ? 8 * t.few : mk::kTreeRows;
   t.tiles = (rows + tile_rows - 1) / tile_rows;
   const int unit = mk::kTreeBlock, units = (max_len + unit - 1) / unit;
-  const int fixed = t.few ? 2 : 3;  // in units, like the costs of a join: 1 and 3
-  const long long ctas = (long long)batch * num_kv_heads * t.tiles;
-  const long long slots = (t.few ? (long long)mk::kFewCtas : 2LL) * device_sms();
+  const long long ctas = (long long)batch * num_kv_heads * t.tiles, sms = device_sms();
+  const long long slots = (t.few ? mk::kFewCtas : 2) * sms;
   long long best = -1;
   int last = 0;
   for (int want = 1; want <= units; ++want) {
     const int per = (units + want - 1) / want, splits = (units + per - 1) / per;
     if (splits == last) continue;
+    if (ctas * last >= slots) break;
     last = splits;
-    const long long waves = (ctas * splits + slots - 1) / slots;
-    if (best >= 0 && waves > 1 && splits > 4 * kTreeCluster) break;  // finer cuts only add waves
-    const long long cost = waves * (per + fixed) + (splits == 1 ? 0 : splits <= kTreeCluster ? 1 : 3);
+    const long long n = ctas * splits;
+    auto wave = [&](long long k) -> long long {
+      return k == 0 ? 0 : t.few ? 26 + 15 * per : k <= sms ? 51 + 11 * per : 65 + 18 * per;
+    };
+    const int join = splits == 1 ? 0 : splits <= kTreeCluster ? (t.few ? 9 : 16) : (t.few ? 25 : 50) + 2 * splits;
+    const long long cost = n / slots * wave(slots) + wave(n % slots) + join;
     if (best < 0 || cost < best) {
       best = cost;
       t.splits = splits;
