@@ -93,12 +93,13 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
   pdl_trigger();
   pdl_wait();
   const KVLayer& kv = p.kv;
-  const int nh = p.NQ + 2 * kv.NKV;
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;
+  const uint32_t nh = p.NQ + 2 * kv.NKV;
+  // 32 bits: 2^32 of these would be 550 GB of qkv (a 64-bit division is a third of the kernel)
+  const uint32_t unit = blockIdx.x * 32u + (threadIdx.x >> 3);
   const int l = threadIdx.x & 7;
-  const bool live = unit < (int64_t)p.rows * nh;  // whole groups of eight lanes
-  const int row = live ? (int)(unit / nh) : 0, hd = live ? (int)(unit % nh) : 0;
-  const uint4 u = live ? reinterpret_cast<const uint4*>(p.qkv)[unit * 8 + l] : make_uint4(0, 0, 0, 0);
+  const int row = unit / nh, hd = unit - row * nh;
+  const bool live = row < p.rows;  // whole groups of eight lanes
+  const uint4 u = live ? reinterpret_cast<const uint4*>(p.qkv)[(size_t)unit * 8 + l] : make_uint4(0, 0, 0, 0);
   float lo[4] = {bf_lo(u.x), bf_lo(u.y), bf_lo(u.z), bf_lo(u.w)};
   float hi[4] = {bf_hi(u.x), bf_hi(u.y), bf_hi(u.z), bf_hi(u.w)};
   bool ok = live;
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
   const int seq = p.seqs[row];
   const bool is_k = hd < p.NQ + kv.NKV;
   const int g = hd - p.NQ - (is_k ? 0 : kv.NKV);
-  const int blk = slot / kv.ps;
+  const int blk = slot / kv.ps, off = slot - blk * kv.ps;
   int page = -1;
   if (slot >= 0 && blk < kv.max_blocks && seq >= 0 && seq < kv.batch)
     page = kv.block_tables[(size_t)seq * kv.max_blocks + blk];
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     atomicExch(p.error, 1);
     return;
   }
-  const size_t r = ((size_t)page * kv.NKV + g) * kv.ps + slot % kv.ps;
+  const size_t r = ((size_t)page * kv.NKV + g) * kv.ps + off;
   uint8_t* pool = is_k ? kv.k : kv.v;
   if (!kFp8) {
     uint2* dst = reinterpret_cast<uint2*>(pool + r * 128) + l;
