@@ -100,11 +100,18 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
   const int row = unit / nh, hd = unit - row * nh;
   const bool live = row < p.rows;  // whole groups of eight lanes
   const uint4 u = live ? reinterpret_cast<const uint4*>(p.qkv)[(size_t)unit * 8 + l] : make_uint4(0, 0, 0, 0);
+  // all that does not wait for another load, then the page, under way with the rotation's tables
+  const bool stored = live && hd >= p.NQ;
+  const int pos = live && hd < p.NQ + kv.NKV ? p.positions[row] : 0;
+  const int slot = stored ? p.slots[row] : -1, seq = stored ? p.seqs[row] : 0;
+  const int blk = slot / kv.ps, off = slot - blk * kv.ps;
+  int page = -1;
+  if (slot >= 0 && blk < kv.max_blocks && seq >= 0 && seq < kv.batch)
+    page = kv.block_tables[(size_t)seq * kv.max_blocks + blk];
   float lo[4] = {bf_lo(u.x), bf_lo(u.y), bf_lo(u.z), bf_lo(u.w)};
   float hi[4] = {bf_hi(u.x), bf_hi(u.y), bf_hi(u.z), bf_hi(u.w)};
   bool ok = live;
   if (live && hd < p.NQ + kv.NKV) {
-    const int pos = p.positions[row];
     ok = pos >= 0 && pos < p.rope_len;
     if (ok) {
       const uint2* c = reinterpret_cast<const uint2*>(p.cos_t + (size_t)pos * 64) + l;
@@ -143,15 +150,9 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     q[8] = pack(hi);
     return;
   }
-  const int slot = p.slots[row];
   if (slot == -1) return;
-  const int seq = p.seqs[row];
   const bool is_k = hd < p.NQ + kv.NKV;
   const int g = hd - p.NQ - (is_k ? 0 : kv.NKV);
-  const int blk = slot / kv.ps, off = slot - blk * kv.ps;
-  int page = -1;
-  if (slot >= 0 && blk < kv.max_blocks && seq >= 0 && seq < kv.batch)
-    page = kv.block_tables[(size_t)seq * kv.max_blocks + blk];
   if (page < 0 || page >= kv.num_pages) {
     atomicExch(p.error, 1);
     return;

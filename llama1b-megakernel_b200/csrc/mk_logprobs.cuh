@@ -22,9 +22,15 @@
 // `top` more come, and the warps run free of each other. (Ranked rarely, nearly
 // every warp went through the collection in every chunk: 28 instructions issued a
 // logit, 8 of them for the sums.) Chunks with more than kLpCandidates beyond the
-// threshold (rising or equal logits) are read again and chosen from one by one. A
-// second kernel joins a row's slices with the same selection over
-// their lists.
+// threshold (rising or equal logits) are read again and chosen from one by one. The
+// slices of a row are a cluster; its first CTA joins them, ranking out of their lists
+// what reaches the largest of the lists' last keys.
+//
+// Many fp32 rows are bound by memory: 2,047 of 128,256 in 185 us, 5.7 TB/s. Of bf16, with
+// half the bytes for as many exponentials and comparisons, by instruction latency: 200
+// rows with five alternatives in 27.4 us (1.9 TB/s, 15 instructions a logit, issued in 49%
+// of the cycles, three CTAs on an SM), 20.0 without alternatives. One row is latency:
+// 9.9 us with twenty.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -165,14 +165,15 @@ cudaError_t launch_tree(const mk::TreeTmaParams& tp, int few, dim3 grid, cudaStr
 }
 
 // How a row is cut: chunks of 16 logits a thread or of one vector, and slices of
-// whole chunks. In quarters of a 16-logit chunk's time, a slice costs what it reads,
-// about kLpFixed for the first choice of alternatives and the join, and kLpRank for
-// each later ranking (after 2, 4, 8 ... chunks); an SM's share is that times the slices
-// that fall to it, and the cut with the least is taken. The slices of a row are a
-// cluster; more than the portable eight only for a few rows, which cannot fill the
-// GPU otherwise.
+// whole chunks. A CTA beside k - 1 others on its SM (four fit) takes about, in
+// hundredths of a microsecond, 300 + 200 k, 60 for each ranking after the first (they
+// come after 2, 4, 8 ... chunks), and 55 + 10 k a chunk of 16 (a smaller one costs more
+// than its share): latency more than work, so a second CTA costs little. The cut with the
+// least is taken. 128,256 bf16 logits, five alternatives: one row 10 us in 16 slices, 27
+// whole; 148 rows 21 in two, 28 whole; 200 rows 27 in two, 33 whole, 34 in three; 700
+// rows 62 whole, 67 in two. The slices of a row are a cluster; more than the portable
+// eight only for a few rows, which cannot fill the GPU otherwise.
 constexpr int kLpMaxVocab = 1 << 30;
-constexpr int kLpFixed = 8, kLpRank = 2;
 struct LpCut {
   int per, slices, len;
 };
@@ -186,7 +187,12 @@ LpCut lp_cut(int rows, int vocab, int vector) {
       const int e = (n + want - 1) / want, k = (n + e - 1) / e;
       int ranks = 0;
       while ((1 << ranks) < e) ++ranks;
-      const long long cost = (((long long)rows * k + sms - 1) / sms) * ((long long)e * per / 4 + kLpFixed + kLpRank * ranks);
+      auto wave = [&](long long on) -> long long {
+        return on == 0 ? 0 : 300 + 200 * on + 60 * ranks + e * (per == 16 ? 16 : per + 2) * (55 + 10 * on) / 16;
+      };
+      // clusters do not fill the last slots (148 rows in four: 28 us, in two 21)
+      const long long ctas = (long long)rows * k, on = (ctas + (k > 1 ? ctas / 32 : 0) + sms - 1) / sms;
+      const long long cost = on / 4 * wave(4) + wave(on % 4);
       if (least < 0 || cost < least) {
         least = cost;
         best = {per, k, e * mk::kLpThreads * per};
