@@ -77,12 +77,10 @@ TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
   const long long ctas = (long long)batch * num_kv_heads * t.tiles, sms = device_sms();
   const long long slots = (t.few ? mk::kFewCtas : 2) * sms;
   long long best = -1;
-  int last = 0;
-  for (int want = 1; want <= units; ++want) {
+  for (int want = 1, last = 0; want <= units && ctas * last < slots;) {
     const int per = (units + want - 1) / want, splits = (units + per - 1) / per;
-    if (splits == last) continue;
-    if (ctas * last >= slots) break;
     last = splits;
+    want = per > 1 ? (units + per - 2) / (per - 1) : units + 1;  // the next that shortens the ranges
     const long long n = ctas * splits;
     auto wave = [&](long long k) -> long long {
       return k == 0 ? 0 : t.few ? 26 + 15 * per : k <= sms ? 51 + 11 * per : 65 + 18 * per;
@@ -96,6 +94,11 @@ TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
     }
   }
   return t;
+}
+
+int64_t tree_workspace(const TreePlan& t, int batch, int num_kv_heads, int rows) {
+  if (t.splits == 1 || t.cluster()) return 0;
+  return (int64_t)batch * num_kv_heads * t.splits * rows * mk::kTreePartial * 4;
 }
 
 // A page pool as rows of 64 values, boxes of `box` whole rows: bf16 rows with the
@@ -297,9 +300,7 @@ int64_t mk_tree_attention_workspace(int32_t batch, int32_t num_q_heads, int32_t 
                                     int32_t max_nodes, int32_t max_len) {
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_nodes < 1 || max_len < 1) return 0;
   const int group = num_q_heads / num_kv_heads;
-  const TreePlan sp = tree_plan(batch, num_kv_heads, max_nodes * group, max_len);
-  if (sp.splits == 1 || sp.cluster()) return 0;
-  return (int64_t)batch * num_kv_heads * sp.splits * max_nodes * group * mk::kTreePartial * 4;
+  return tree_workspace(tree_plan(batch, num_kv_heads, max_nodes * group, max_len), batch, num_kv_heads, max_nodes * group);
 }
 
 int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_nodes,
@@ -324,7 +325,8 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   if (!aligned16(q) || !aligned16(out)) return fail(MK_EINVAL, "q and out must be 16-byte aligned");
   const long long pool_rows = (long long)kv->num_pages * nkv * kv->page_size;
   if (pool_rows > 0x7fffffffLL) return fail(MK_EINVAL, "KV pool of %lld rows", pool_rows);
-  const int64_t need = mk_tree_attention_workspace(batch, num_q_heads, nkv, max_nodes, max_len);
+  const TreePlan plan = tree_plan(batch, nkv, max_nodes * group, max_len);
+  const int64_t need = tree_workspace(plan, batch, nkv, max_nodes * group);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(MK_EINVAL, "workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   if (need > 0 && !aligned16(workspace)) return fail(MK_EINVAL, "workspace must be 16-byte aligned");
@@ -344,7 +346,6 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   p.error = error;
-  const TreePlan plan = tree_plan(batch, nkv, max_nodes * group, max_len);
   p.tiles = plan.tiles;
   p.splits = plan.splits;
   p.split_len = plan.len;
