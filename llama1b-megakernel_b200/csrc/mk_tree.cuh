@@ -28,7 +28,8 @@
 //    second, each with its own S, maximum, sum and O, which are joined at the end: a
 //    row's thread spends as long on waits, loads and bookkeeping as on its 64
 //    exponentials, so four warps (two CTAs) on each scheduler keep the special
-//    function unit busy where two did not (235 us to X for the chunk case). A thread
+//    function unit busy where two did not (4 sequences of 256 nodes at 16,000: 235 us
+//    with one softmax warpgroup, 211 with two). A thread
 //    has a row (TMEM lane): the 64 scores, the exponentials, P as bf16 pairs over S.
 //    O is only rescaled when a row's maximum has grown by more than 8 powers of two
 //    since it was last set: until then p is at most 256, which costs bf16 and fp32
@@ -302,6 +303,27 @@ __device__ __forceinline__ float tree_max3(float a, float b, float c) {  // NaN 
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+// 2^x of two numbers on the FMA pipe, for some of a row's: the special function unit
+// (16 exponentials a cycle) is what bounds the softmax of bf16 rows. x = n + f, |f| <= 1/2, and a polynomial for 2^f (least largest relative error, fitted by
+// reweighted least squares: 2^-22.1 in fp32, as good as ex2.approx); n goes into the
+// exponent by a multiplication, which keeps a NaN. Below 2^-126 the result is 2^-126, so
+// it is not for masked scores. 4 sequences of 256 nodes at 16,000: none 199 us, 2 of 16
+// 184, 3 of 16 181, 4 of 16 183, 5 of 16 195; with 8-bit rows, whose conversion takes the issue slots,
+// 32 x 64 nodes: none 223 us, 2 of 16 235.
+__device__ __forceinline__ float2 tree_exp2(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  auto both = [](float c) { return make_float2(c, c); };
+  const float2 t = add2(x, both(12583039.f));  // 1.5 * 2^23 + 127: n, biased, in the low bits
+  const float2 f = fma2(add2(t, both(-12583039.f)), both(-1.f), x);
+  float2 q = fma2(f, both(0.0013276466634124517f), both(0.009675540961325169f));
+  q = fma2(q, f, both(0.05550713464617729f));
+  q = fma2(q, f, both(0.24022120237350464f));
+  q = fma2(q, f, both(0.6931469440460205f));
+  q = fma2(q, f, both(1.0000001192092896f));
+  return mul2(q, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 
 __device__ __forceinline__ void tree_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -742,7 +764,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     bool ok = true;
     // one half block; kTail: it reaches past the committed positions
     auto step = [&](auto kind, const int j) {
-      constexpr bool kTail = decltype(kind)::value;
+      constexpr bool kTail = decltype(kind)::value, kPoly = !kFp8 && !kTail;
       unsigned long long vis = ~0ull;
       if constexpr (kTail) {
         const int rd = j % L::kReady;
@@ -797,7 +819,10 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
             float2 x = make_float2(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
             x = fma2(x, scale2, shift2);
             top[i & 1] = tree_max3(top[i & 1], x.x, x.y);
-            x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+            if (kPoly && i % 5 == 3)
+              x = tree_exp2(x);
+            else
+              x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
             if (i & 1) {
               s1 = add2(s1, x);
             } else {

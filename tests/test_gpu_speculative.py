@@ -393,6 +393,28 @@ def test_value_of_a_seen_node_is_not_finite(fmt):
     assert not out[20:, :, 5].isfinite().any()
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("nodes", [1, 4, 20])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_committed_row_is_not_finite(fmt, nodes, which):
+    """A NaN row at any place of a block of committed positions makes its K/V head's
+    results NaN, and no others."""
+    batch, nq, nkv = 64, 8, 2
+    s = _setup([300] * batch, [nodes] * batch, nq, nkv, 16, fmt, "chain", seed=nodes)
+    b = torch.arange(batch, device=DEV)
+    page, off = s["tables"][b, (64 + b) // 16].long(), (64 + b) % 16  # position 64 + b of sequence b
+    if fmt == "bf16":
+        s[which][page, 0, off] = math.nan
+    else:
+        s[which + "s"][page, 0, off] = NAN_BYTE
+    out, lse, err = _attend(s)
+    assert int(err) == 0
+    assert out[:, :nq // nkv].isnan().all() and out[:, nq // nkv:].isfinite().all()
+    assert lse[:, nq // nkv:].isfinite().all()
+    if which == "k":
+        assert lse[:, :nq // nkv].isnan().all()
+
+
 def test_strided_sequences_of_a_larger_table_and_other_stream():
     """Fewer sequences than the table has rows, on a stream of its own."""
     s = _setup([90, 33, 200], [6, 2, 11], 8, 2, 16, "e4m3", "tree", seed=8)
