@@ -1,14 +1,14 @@
 // Attention of few drafted rows per K/V head (mk_tree.cuh has the definition, the
 // parameters and the join of split ranges): decode steps and small trees.
 //
-// With at most 32 rows (nodes x query heads of a K/V head) a 128-row tensor tile
+// With at most 16 rows (nodes x query heads of a K/V head) a 128-row tensor tile
 // would be mostly empty and its softmax would run on a quarter of the SM, while the
-// work is to stream K and V once. So a tile is 8, 16 or 32 rows (RT eights) on
+// work is to stream K and V once. So a tile is 8 or 16 rows (RT eights) on
 // mma.sync.m16n8k16, whose B operand comes straight from registers:
-//  * four consumer warps take turns at the chunks of the range (32 positions of
+//  * three consumer warps take turns at the chunks of the range (32 positions of
 //    bf16, 64 of 8-bit codes: 8 KB either way), each with its own maximum, sum and O,
-//    joined in shared memory at the end; a producer warp keeps eight chunks in
-//    flight by TMA;
+//    joined in shared memory at the end; a producer warp keeps six chunks in
+//    flight by TMA, two for each consumer;
 //  * bf16: fragments by ldmatrix from the 128-byte-swizzled rows, P bf16;
 //  * 8-bit: all products in f16, where every code is exact and one conversion makes
 //    two of them. A thread's K fragment is 16 consecutive codes of a position (one
@@ -24,6 +24,13 @@
 //    in memory (few_place) so that both loads are free of bank conflicts under the
 //    64-byte swizzle.
 // O is rescaled when a maximum grew by more than 8 powers of two, as in mk_tree.cuh.
+//
+// What bounds it: memory, where sequences fill the GPU (36 of 1,000 to 2,000 positions in
+// 8 bits: 18 us; 64 of 2,600 to 4,100: 55 us, 4.1 TB/s, as their 512 CTAs end one by one),
+// and the latency of a CTA's few chunks where they do not (one of 1,025 bf16: 6.0 us).
+// The split of an SM was measured (consumers x stages x CTAs; 64 of 2,600 to 4,100 in 8
+// bits, and 32 of 2,700 to 4,100 in bf16 with 16 rows): 3 x 6 x 4 55 and 45 us, 4 x 8 x 3 80
+// and 50, 4 x 4 x 4 (32 of 8-bit: 35 against 34) and 45; with 5 or 6 CTAs registers spill.
 #pragma once
 
 #include <type_traits>
