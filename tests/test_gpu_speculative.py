@@ -20,6 +20,7 @@ import math
 import pytest
 import torch
 
+from llama1b_megakernel_b200 import _lib
 from llama1b_megakernel_b200 import speculative as sp
 
 pytestmark = pytest.mark.gpu
@@ -413,6 +414,23 @@ def test_committed_row_is_not_finite(fmt, nodes, which):
     assert lse[:, nq // nkv:].isfinite().all()
     if which == "k":
         assert lse[:, :nq // nkv].isnan().all()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("nodes", [1, 20])
+def test_more_ranges_than_a_cluster(fmt, nodes):
+    """Few long sequences are split further than a cluster joins: partials in the workspace."""
+    s = _setup([17000, 40, 9000], [nodes] * 3, 4, 1, 64, fmt, "tree", seed=nodes)
+    nbytes = _lib.load().mk_tree_attention_workspace(3, 4, 1, nodes, s["max_len"])
+    assert nbytes > 0
+    ws = torch.empty(nbytes + 8, dtype=torch.uint8, device=DEV)
+    out, lse, err = _attend(s, workspace=ws[:nbytes])
+    assert int(err) == 0
+    _check(s, out, lse)
+    with pytest.raises(_lib.MkError, match="16-byte"):
+        _attend(s, workspace=ws[8:])
+    with pytest.raises(_lib.MkError, match="workspace"):
+        _attend(s, workspace=ws[:nbytes - 16])
 
 
 def test_strided_sequences_of_a_larger_table_and_other_stream():
