@@ -56,16 +56,25 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 // ranges) and a launch and a trip through the workspace otherwise. 10 sequences of 25
 // nodes behind 2,000 to 4,000 positions: 38 us whole, 34 in two, 27 in three, 29 in four.
 //
+// Where an SM gets a second CTA (of few rows: where not all fit at once) the longer
+// sequences go first, so that short ones share SMs and fill the last wave: 28 sequences of
+// 25 nodes behind 2,000 to 4,000 positions 50 us as they come, 40 so; 12 of 64 nodes behind
+// 4,000 to 8,000 83 and 61; 32 of 64 over 5,200 to 8,200 8-bit positions 223 and 205. It
+// costs a CTA half a microsecond, more with many sequences, which even out by themselves
+// (200 of 25 nodes: 80 and 88): up to kTreeSort sequences.
+//
 // No cut is finer than it takes to fill the slots once. What the estimate promises
 // beyond that, ragged lengths eat, as the hardware hands out whole CTAs more evenly than
 // the waves here (20 such sequences: 41 us whole, 39 in two, 45 in three), and row tiles
 // that share positions drift apart (4 sequences of 256 nodes at 16,000: 198 us whole, 216
 // in two).
 constexpr int kTreeFewRows = 16;
+constexpr int kTreeSort = 128;
 using mk::kTreeCluster;
 struct TreePlan {
   int few;  // eights of rows in a tile of the mma.sync kernel (1, 2), 0: tcgen05
   int tiles, splits, len;
+  bool sorted;  // the longer sequences first
   bool cluster() const { return splits > 1 && splits <= kTreeCluster; }
 };
 TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
@@ -91,6 +100,7 @@ TreePlan tree_plan(int batch, int num_kv_heads, int rows, int max_len) {
       best = cost;
       t.splits = splits;
       t.len = per * unit;
+      t.sorted = batch > 1 && batch <= kTreeSort && n > (t.few ? slots : sms);
     }
   }
   return t;
@@ -350,6 +360,8 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   p.splits = plan.splits;
   p.split_len = plan.len;
   p.cluster = plan.cluster();
+  if (plan.sorted)
+    for (p.sorted = 1; max_len >> (p.sorted - 1) > 31;) ++p.sorted;
   p.work = static_cast<float*>(workspace);
   const bool fp8 = kv->format == MK_KV_E4M3;
   p.box = !plan.few ? mk::kTreeBlock : fp8 ? mk::FewShape<true>::kChunk : mk::FewShape<false>::kChunk;

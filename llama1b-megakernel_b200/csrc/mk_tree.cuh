@@ -93,6 +93,7 @@ struct TreeParams {
   int box;                          // rows of a TMA box
   int tiles, splits, split_len;     // split_len: a multiple of kTreeBlock
   int cluster;                      // the ranges of a tile are a cluster (else: partials in work)
+  int sorted;                       // long sequences first (tree_turn): 1 + log2 of a bucket's positions; 0: as they come
   float scale;
   float* work;                      // [batch][NKV][splits][max_nodes * group][kTreePartial]
   __nv_bfloat16* out;               // [rows][NQ][64]
@@ -399,6 +400,45 @@ __device__ __forceinline__ void tree_item(const TreeParams& p, int& tile, int& s
   }
 }
 
+// The CTA's sequence: as they come, or the longer ones first, by buckets of their
+// committed positions (at most 32 buckets; within one as they come). Every warp finds out
+// by itself: lane k counts bucket 31 - k, a scan gives the bucket of this CTA's turn, and
+// the turn within it is a set bit of the ballots.
+__device__ __forceinline__ int tree_turn(const TreeParams& p) {
+  const int turn = blockIdx.z;
+  if (!p.sorted) return turn;
+  const int lane = threadIdx.x & 31, batch = p.kv.batch;
+  // the place of sequence b's bucket in the order, 32 for none
+  auto bucket = [&](int b) { return b < batch ? 31 - min(max(p.prefix[b], 0) >> (p.sorted - 1), 31) : 32; };
+  int count = 0;
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    const int k = bucket(b0 + lane);
+    uint32_t same = __ballot_sync(0xffffffffu, k < 32);  // the lanes whose k is this lane's number
+#pragma unroll
+    for (int bit = 0; bit < 5; ++bit) {
+      const uint32_t set = __ballot_sync(0xffffffffu, (k >> bit) & 1);
+      same &= (lane >> bit) & 1 ? set : ~set;
+    }
+    count += __popc(same);
+  }
+  int upto = count;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += x;
+  }
+  const int mine = __ffs(__ballot_sync(0xffffffffu, upto > turn)) - 1;
+  int left = turn - __shfl_sync(0xffffffffu, upto - count, mine);
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    const bool in = bucket(b0 + lane) == mine;
+    const uint32_t there = __ballot_sync(0xffffffffu, in);
+    const uint32_t hit = __ballot_sync(0xffffffffu, in && __popc(there & ((1u << lane) - 1)) == left);
+    if (hit) return b0 + __ffs(hit) - 1;
+    left -= __popc(there);
+  }
+  return 0;  // not reached: the buckets hold `batch` sequences
+}
+
 // lse of a row out of its maximum, in powers of two, and sum (not 0); lg2.approx is
 // within 2^-22 of 1 or of the logarithm.
 __device__ __forceinline__ float tree_lse(float m, float sum) {
@@ -491,7 +531,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   const KVLayer& kv = p.kv;
   pdl_trigger();
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int g = blockIdx.y, b = blockIdx.z;
+  const int g = blockIdx.y;
   int tile, split;
   tree_item(p, tile, split);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -529,6 +569,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
   __syncthreads();  // the producer and the block warps need no other
   const int p0 = split * p.split_len;
   pdl_wait();
+  const int b = tree_turn(p);
   // the producer's first page ids and the sequence's lengths are on their way together
   TreePages pages(kv, b, p0, warp == 12 ? lane : 1 << 30, p.error);
   int row0, nodes, prefix;

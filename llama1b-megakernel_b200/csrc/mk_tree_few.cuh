@@ -110,7 +110,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
   const KVLayer& kv = p.kv;
   pdl_trigger();
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int g = blockIdx.y, b = blockIdx.z;
+  const int g = blockIdx.y;
   int tile, split;
   tree_item(p, tile, split);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
   __syncthreads();
   const int p0 = split * p.split_len;
   pdl_wait();
+  const int b = tree_turn(p);
   // the producer's first page ids and the sequence's lengths are on their way together
   TreePages pages(kv, b, p0, warp == kFewWarps ? lane : 1 << 30, p.error);
   int row0, nodes, prefix;
