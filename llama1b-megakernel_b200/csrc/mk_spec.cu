@@ -47,7 +47,7 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 // CTAs. Up to kTreeFewRows rows (nodes x query heads of a K/V head) go to the
 // mma.sync kernel, in one tile of 8 or 16; more to the tcgen05 kernel in tiles of 128.
 // (16 rows at 32 x 4096: 44.8 us against 45.0 of bf16, 39 against 56 of 8-bit rows; 20
-// rows need two of the small tiles: 64 against 45, 57 against 56.)
+// to 32 rows in a small tile of 32: 64 to 66 against 45, 57 to 59 against 56.)
 //
 // The cut with the least estimated time is taken, in tenths of a microsecond, fitted to
 // launches of 1 to 50 sequences: a CTA costs a fixed part (first bytes, the store) and
@@ -65,8 +65,8 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 //
 // No cut is finer than it takes to fill the slots once. What the estimate promises
 // beyond that, ragged lengths eat, as the hardware hands out whole CTAs more evenly than
-// the waves here (20 such sequences: 41 us whole, 39 in two, 45 in three), and row tiles
-// that share positions drift apart (4 sequences of 256 nodes at 16,000: 198 us whole, 216
+// the waves here (20 such sequences: 40 us whole, 36 in two, 45 in three), and row tiles
+// that share positions drift apart (4 sequences of 256 nodes at 16,000: 182 us whole, 205
 // in two).
 constexpr int kTreeFewRows = 16;
 constexpr int kTreeSort = 128;
