@@ -28,8 +28,7 @@
 //
 // Many fp32 rows are bound by memory: 2,047 of 128,256 in 185 us, 5.7 TB/s. Of bf16, with
 // half the bytes for as many exponentials and comparisons, by instruction latency: 200
-// rows with five alternatives in 27.4 us (1.9 TB/s, 15 instructions a logit, issued in 49%
-// of the cycles, three CTAs on an SM), 20.0 without alternatives. One row is latency:
+// rows with five alternatives in 25.3 us (2.0 TB/s, 15 instructions a logit), 17.4 without. One row is latency:
 // 9.9 us with twenty.
 #pragma once
 
@@ -219,7 +218,7 @@ __device__ __forceinline__ void lp_finish(const LogprobsParams& p, const LpShare
 // One slice of a row. Thread t holds E logits of a chunk, in vectors of 16 bytes
 // that neighbouring threads read side by side (kVec: every row starts on 16 bytes).
 template <typename T, int E, bool kVec>
-__global__ void __launch_bounds__(kLpThreads, sizeof(T) * E >= 64 || (!kVec && E == 16) ? 3 : 4) logprobs_kernel(const __grid_constant__ LogprobsParams p) {
+__global__ void __launch_bounds__(kLpThreads, E == 16 ? 3 : 4) logprobs_kernel(const __grid_constant__ LogprobsParams p) {
   pdl_trigger();
   pdl_wait();
   __shared__ LpShared sh;
@@ -232,8 +231,12 @@ __global__ void __launch_bounds__(kLpThreads, sizeof(T) * E >= 64 || (!kVec && E
   auto index = [&](int c0, int e) {
     return kVec ? c0 + ((e / N) * kLpThreads + tid) * N + e % N : c0 + e * kLpThreads + tid;
   };
-  uint32_t raw[E * sizeof(T) / 4];  // the chunk on its way
-  auto fetch = [&](int c0) {
+  // the chunk on its way, and of bf16, whose chunks have half the bytes, the one after it
+  // (three CTAs with two in flight: 25.3 us for 200 rows; four with one: 27.5)
+  constexpr int W = E * sizeof(T) / 4;
+  constexpr bool kTwo = sizeof(T) == 2;
+  uint32_t raw[W], after[kTwo ? W : 1];
+  auto fetch = [&](auto& raw, int c0) {
     if (kVec && c0 + C <= i1) {
 #pragma unroll
       for (int c = 0; c < E / N; ++c) {
@@ -304,11 +307,18 @@ __global__ void __launch_bounds__(kLpThreads, sizeof(T) * E >= 64 || (!kVec && E
   };
   const int chunks = (i1 - i0 + C - 1) / C;
   int from = 0, next = 1;  // the segment of chunks since the list was last settled, and its end
-  fetch(i0);
+  fetch(raw, i0);
+  if (kTwo && chunks > 1) fetch(after, i0 + C);
   for (int c = 0; c < chunks; ++c) {
     const int c0 = i0 + c * C;
     take();
-    if (c + 1 < chunks) fetch(c0 + C);
+    if constexpr (kTwo) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) raw[i] = after[i];
+      if (c + 2 < chunks) fetch(after, c0 + 2 * C);
+    } else {
+      if (c + 1 < chunks) fetch(raw, c0 + C);
+    }
     const float best = largest();
     if (best > m) {
       const float a = m == -INFINITY ? 0.f : exp2_approx((m - best) * kLog2e);
@@ -357,11 +367,11 @@ __global__ void __launch_bounds__(kLpThreads, sizeof(T) * E >= 64 || (!kVec && E
       // the segment's chunks are read once more and chosen from one by one
       __syncthreads();
       for (int r = from; r <= c; ++r) {
-        fetch(i0 + r * C);
+        fetch(raw, i0 + r * C);
         take();
         choose(i0 + r * C);
       }
-      if (c + 1 < chunks) fetch(c0 + C);
+      if (c + 1 < chunks) fetch(raw, c0 + C);
     }
     from = c + 1;
     next = 2 * (c + 1);

@@ -178,14 +178,15 @@ cudaError_t launch_tree(const mk::TreeTmaParams& tp, int few, dim3 grid, cudaStr
 }
 
 // How a row is cut: chunks of 16 logits a thread or of one vector, and slices of
-// whole chunks. A CTA beside k - 1 others on its SM (four fit) takes about, in
-// hundredths of a microsecond, 300 + 200 k, 60 for each ranking after the first (they
-// come after 2, 4, 8 ... chunks), and 55 + 10 k a chunk of 16 (a smaller one costs more
-// than its share): latency more than work, so a second CTA costs little. The cut with the
-// least is taken. 128,256 bf16 logits, five alternatives: one row 10 us in 16 slices, 27
-// whole; 148 rows 21 in two, 28 whole; 200 rows 27 in two, 33 whole, 34 in three; 700
-// rows 62 whole, 67 in two. The slices of a row are a cluster; more than the portable
-// eight only for a few rows, which cannot fill the GPU otherwise.
+// whole chunks. A CTA beside k - 1 others on its SM (three fit, of the small chunks
+// four) takes about, in hundredths of a microsecond, 300 + 200 k, 60 for each ranking
+// after the first (they come after 2, 4, 8 ... chunks), and 55 + 10 k a chunk of 16 (a
+// smaller one costs more than its share): latency more than work, so a second CTA costs
+// little. The cut with the least is taken. 128,256 bf16 logits, five alternatives: one
+// row 10 us in 16 slices, 27 whole; 120 rows 20 in three, 24 in two, 31 whole; 200 rows
+// 25 in two, 34 whole, 36 in three; 300 rows 36 whole, 42 in two. The slices of a row are a
+// cluster; more than the portable eight only for a few rows, which cannot fill the GPU
+// otherwise.
 constexpr int kLpMaxVocab = 1 << 30;
 struct LpCut {
   int per, slices, len;
@@ -198,14 +199,14 @@ LpCut lp_cut(int rows, int vocab, int vector) {
     const int n = (int)(((long long)vocab + mk::kLpThreads * per - 1) / (mk::kLpThreads * per));
     for (int want = 1; want <= std::min(n, most); ++want) {
       const int e = (n + want - 1) / want, k = (n + e - 1) / e;
-      int ranks = 0;
+      int ranks = 0, fit = per == 16 ? 3 : 4;
       while ((1 << ranks) < e) ++ranks;
       auto wave = [&](long long on) -> long long {
         return on == 0 ? 0 : 300 + 200 * on + 60 * ranks + e * (per == 16 ? 16 : per + 2) * (55 + 10 * on) / 16;
       };
-      // clusters do not fill the last slots (148 rows in four: 28 us, in two 21)
+      // clusters do not fill the last slots (148 rows in three: 32 us, in two 24)
       const long long ctas = (long long)rows * k, on = (ctas + (k > 1 ? ctas / 32 : 0) + sms - 1) / sms;
-      const long long cost = on / 4 * wave(4) + wave(on % 4);
+      const long long cost = on / fit * wave(fit) + wave(on % fit);
       if (least < 0 || cost < least) {
         least = cost;
         best = {per, k, e * mk::kLpThreads * per};
