@@ -20,10 +20,10 @@
 // numbers are exact there, so a rotated value is rounded once by the sum and
 // once by its bf16 or e4m3 store.
 //
-// Both kernels move bytes. 4,093 rows of 48 heads are written in 13.5 us (47 MB, 3.5
-// TB/s): each thread has one 16-byte piece, so what remains is the latency of its two
-// rounds of loads (row, slot and position, then the tables and the page) against 174
-// instructions. 32 x 8,191 positions read back in 131 us (5.7 TB/s). One row: 1.6 us.
+// Both kernels move bytes. 4,093 rows of 48 heads are written in 13.0 us (47 MB, 3.6
+// TB/s; 13.5 with a head a lane group instead of two): what remains is the latency of two
+// rounds of loads (rows, slot and position, then the tables and the page) in three
+// waves of CTAs. 32 x 8,191 positions read back in 131 us (5.7 TB/s). One row: 1.9 us.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -90,97 +90,110 @@ struct KVWriteParams {
   int* error;
 };
 
-// Eight lanes per (row, head), 16 bytes of qkv (four RoPE pairs) each, so a warp
-// takes four heads with full 128-byte reads and a row's largest value is three
-// shuffles away; a lane's results are the dims 4 l .. 4 l + 3 and 32 more.
+// Eight lanes per two neighbouring heads of a row, 16 bytes of qkv (four RoPE pairs) of
+// each, so a warp reads full 128-byte lines, a row's largest value is three shuffles away,
+// and both heads share the rotation's tables; a lane's results are the dims
+// 4 l .. 4 l + 3 and 32 more.
 template <bool kFp8>
 __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KVWriteParams p) {
   pdl_trigger();
   pdl_wait();
   const KVLayer& kv = p.kv;
-  const uint32_t nh = p.NQ + 2 * kv.NKV;
-  // 32 bits: 2^32 of these would be 550 GB of qkv (a 64-bit division is a third of the kernel)
+  const uint32_t nh = p.NQ + 2 * kv.NKV, pairs = (nh + 1) / 2;
+  // 32 bits: 2^32 of these would be 550 GB of qkv (a 64-bit division was a third of the kernel)
   const uint32_t unit = blockIdx.x * 32u + (threadIdx.x >> 3);
   const int l = threadIdx.x & 7;
-  const int row = unit / nh, hd = unit - row * nh;
+  const int row = unit / pairs, h0 = 2 * (unit - row * pairs);
   const bool live = row < p.rows;  // whole groups of eight lanes
-  const uint4 u = live ? reinterpret_cast<const uint4*>(p.qkv)[(size_t)unit * 8 + l] : make_uint4(0, 0, 0, 0);
-  // all that does not wait for another load, then the page, under way with the rotation's tables
-  const bool stored = live && hd >= p.NQ;
-  const int pos = live && hd < p.NQ + kv.NKV ? p.positions[row] : 0;
+  const uint4* src = reinterpret_cast<const uint4*>(p.qkv) + ((size_t)row * nh + h0) * 8 + l;
+  uint4 u[2];
+  u[0] = live ? src[0] : make_uint4(0, 0, 0, 0);
+  u[1] = live && h0 + 1 < nh ? src[8] : make_uint4(0, 0, 0, 0);
+  // all that does not wait for another load, then the page, under way with the tables
+  const bool rotated = live && h0 < p.NQ + kv.NKV, stored = live && h0 + 1 >= p.NQ;
+  const int pos = rotated ? p.positions[row] : 0;
   const int slot = stored ? p.slots[row] : -1, seq = stored ? p.seqs[row] : 0;
   const int blk = slot / kv.ps, off = slot - blk * kv.ps;
   int page = -1;
   if (slot >= 0 && blk < kv.max_blocks && seq >= 0 && seq < kv.batch)
     page = kv.block_tables[(size_t)seq * kv.max_blocks + blk];
-  float lo[4] = {bf_lo(u.x), bf_lo(u.y), bf_lo(u.z), bf_lo(u.w)};
-  float hi[4] = {bf_hi(u.x), bf_hi(u.y), bf_hi(u.z), bf_hi(u.w)};
-  bool ok = live;
-  if (live && hd < p.NQ + kv.NKV) {
-    ok = pos >= 0 && pos < p.rope_len;
-    if (ok) {
+  const bool placed = pos >= 0 && pos < p.rope_len;
+  uint2 cs[4] = {};  // cosines of dims 4 l .., 32 + 4 l .., sines of the same
+  if (rotated) {
+    if (placed) {
       const uint2* c = reinterpret_cast<const uint2*>(p.cos_t + (size_t)pos * 64) + l;
       const uint2* s = reinterpret_cast<const uint2*>(p.sin_t + (size_t)pos * 64) + l;
-      const uint2 c0 = c[0], c1 = c[8], s0 = s[0], s1 = s[8];
-      const float cl[4] = {bf_lo(c0.x), bf_hi(c0.x), bf_lo(c0.y), bf_hi(c0.y)};
-      const float ch[4] = {bf_lo(c1.x), bf_hi(c1.x), bf_lo(c1.y), bf_hi(c1.y)};
-      const float sl[4] = {bf_lo(s0.x), bf_hi(s0.x), bf_lo(s0.y), bf_hi(s0.y)};
-      const float sh[4] = {bf_lo(s1.x), bf_hi(s1.x), bf_lo(s1.y), bf_hi(s1.y)};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = lo[i], b = hi[i];
-        lo[i] = a * cl[i] - b * sl[i];
-        hi[i] = b * ch[i] + a * sh[i];
-      }
+      cs[0] = c[0];
+      cs[1] = c[8];
+      cs[2] = s[0];
+      cs[3] = s[8];
     } else {
       atomicExch(p.error, 1);
     }
   }
-  uint32_t amax = 0;  // |x| as bits: their order is that of the numbers, NaN on top
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    amax = max(amax, max(__float_as_uint(lo[i]) & 0x7FFFFFFFu, __float_as_uint(hi[i]) & 0x7FFFFFFFu));
-  if (kFp8) {
+  for (int i = 0; i < 2; ++i) {
+    const int hd = h0 + i;
+    float lo[4] = {bf_lo(u[i].x), bf_lo(u[i].y), bf_lo(u[i].z), bf_lo(u[i].w)};
+    float hi[4] = {bf_hi(u[i].x), bf_hi(u[i].y), bf_hi(u[i].z), bf_hi(u[i].w)};
+    const bool turn = hd < p.NQ + kv.NKV;
+    if (turn) {
+      const float cl[4] = {bf_lo(cs[0].x), bf_hi(cs[0].x), bf_lo(cs[0].y), bf_hi(cs[0].y)};
+      const float ch[4] = {bf_lo(cs[1].x), bf_hi(cs[1].x), bf_lo(cs[1].y), bf_hi(cs[1].y)};
+      const float sl[4] = {bf_lo(cs[2].x), bf_hi(cs[2].x), bf_lo(cs[2].y), bf_hi(cs[2].y)};
+      const float sh[4] = {bf_lo(cs[3].x), bf_hi(cs[3].x), bf_lo(cs[3].y), bf_hi(cs[3].y)};
 #pragma unroll
-    for (int o = 4; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      for (int e = 0; e < 4; ++e) {
+        const float a = lo[e], b = hi[e];
+        lo[e] = a * cl[e] - b * sl[e];
+        hi[e] = b * ch[e] + a * sh[e];
+      }
+    }
+    uint32_t amax = 0;  // |x| as bits: their order is that of the numbers, NaN on top
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      amax = max(amax, max(__float_as_uint(lo[e]) & 0x7FFFFFFFu, __float_as_uint(hi[e]) & 0x7FFFFFFFu));
+    if (kFp8) {
+#pragma unroll
+      for (int o = 4; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
+    if (!live || hd >= nh || (turn && !placed)) continue;
+    auto pack = [](const float(&x)[4]) {
+      __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+      return make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+    };
+    if (hd < p.NQ) {
+      uint2* q = reinterpret_cast<uint2*>(p.q_out + ((size_t)row * p.NQ + hd) * 64) + l;
+      q[0] = pack(lo);
+      q[8] = pack(hi);
+      continue;
+    }
+    if (slot == -1) continue;
+    if (page < 0 || page >= kv.num_pages) {
+      atomicExch(p.error, 1);
+      continue;
+    }
+    const int g = hd - p.NQ - (turn ? 0 : kv.NKV);
+    const size_t r = ((size_t)page * kv.NKV + g) * kv.ps + off;
+    uint8_t* pool = turn ? kv.k : kv.v;
+    if (!kFp8) {
+      uint2* dst = reinterpret_cast<uint2*>(pool + r * 128) + l;
+      dst[0] = pack(lo);
+      dst[8] = pack(hi);
+      continue;
+    }
+    const int byte = e8m0_of(amax);
+    const float f = byte == kScaleNaN ? 0.f : inv_scale(byte);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(pool + r * 64) + l;
+    uint32_t a = 0, b = 0;
+    if (byte != kScaleNaN) {
+      a = e4m3x2(lo[0] * f, lo[1] * f) | (e4m3x2(lo[2] * f, lo[3] * f) << 16);
+      b = e4m3x2(hi[0] * f, hi[1] * f) | (e4m3x2(hi[2] * f, hi[3] * f) << 16);
+    }
+    dst[0] = a;
+    dst[8] = b;
+    if (l == 0) (turn ? kv.k_scales : kv.v_scales)[r] = (uint8_t)byte;
   }
-  if (!ok) return;
-  auto pack = [](const float(&x)[4]) {
-    __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-    return make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
-  };
-  if (hd < p.NQ) {
-    uint2* q = reinterpret_cast<uint2*>(p.q_out + ((size_t)row * p.NQ + hd) * 64) + l;
-    q[0] = pack(lo);
-    q[8] = pack(hi);
-    return;
-  }
-  if (slot == -1) return;
-  const bool is_k = hd < p.NQ + kv.NKV;
-  const int g = hd - p.NQ - (is_k ? 0 : kv.NKV);
-  if (page < 0 || page >= kv.num_pages) {
-    atomicExch(p.error, 1);
-    return;
-  }
-  const size_t r = ((size_t)page * kv.NKV + g) * kv.ps + off;
-  uint8_t* pool = is_k ? kv.k : kv.v;
-  if (!kFp8) {
-    uint2* dst = reinterpret_cast<uint2*>(pool + r * 128) + l;
-    dst[0] = pack(lo);
-    dst[8] = pack(hi);
-    return;
-  }
-  const int byte = e8m0_of(amax);
-  const float f = byte == kScaleNaN ? 0.f : inv_scale(byte);
-  uint32_t* dst = reinterpret_cast<uint32_t*>(pool + r * 64) + l;
-  uint32_t a = 0, b = 0;
-  if (byte != kScaleNaN) {
-    a = e4m3x2(lo[0] * f, lo[1] * f) | (e4m3x2(lo[2] * f, lo[3] * f) << 16);
-    b = e4m3x2(hi[0] * f, hi[1] * f) | (e4m3x2(hi[2] * f, hi[3] * f) << 16);
-  }
-  dst[0] = a;
-  dst[8] = b;
-  if (l == 0) (is_k ? kv.k_scales : kv.v_scales)[r] = (uint8_t)byte;
 }
 
 struct KVReadParams {

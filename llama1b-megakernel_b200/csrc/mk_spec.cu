@@ -279,9 +279,9 @@ int mk_kv_write(const MkKVLayer* kv, int32_t batch, const void* qkv, const void*
   p.rope_len = rope_len;
   p.q_out = static_cast<__nv_bfloat16*>(q_out);
   p.error = error;
-  const int64_t heads = (int64_t)rows * (num_q_heads + 2 * kv->num_kv_heads);
-  const int64_t ctas = (heads + 31) / 32;
-  if (ctas > 0x7ffffffLL) return fail(MK_EINVAL, "%d rows of %lld heads", rows, (long long)(heads / rows));
+  const int64_t pairs = (int64_t)rows * ((num_q_heads + 2 * kv->num_kv_heads + 1) / 2);
+  const int64_t ctas = (pairs + 31) / 32;
+  if (ctas > 0x7ffffffLL) return fail(MK_EINVAL, "%d rows of %d query heads", rows, num_q_heads);
   MK_CUDA(launch_pdl(kv->format == MK_KV_E4M3 ? mk::kv_write_kernel<true> : mk::kv_write_kernel<false>,
                      dim3((unsigned)ctas), dim3(256), 0, static_cast<cudaStream_t>(stream), p));
   return MK_OK;
