@@ -433,6 +433,18 @@ def test_more_ranges_than_a_cluster(fmt, nodes):
         _attend(s, workspace=ws[:nbytes - 16])
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("batch,nodes,nq,nkv", [(70, 20, 8, 4), (100, 1, 8, 8), (33, 40, 16, 8)])
+def test_many_ragged_sequences(fmt, batch, nodes, nq, nkv):
+    """More CTAs than SMs or slots: the longer sequences go first, each exactly once."""
+    lengths = [(37 * i * i) % 700 if i % 5 else 300 for i in range(batch)]
+    lengths[3] = 0
+    s = _setup(lengths, [nodes - (i % 2 if nodes > 1 else 0) for i in range(batch)], nq, nkv, 16, fmt, "tree", seed=batch)
+    out, lse, err = _attend(s)
+    assert int(err) == 0
+    _check(s, out, lse)
+
+
 def test_strided_sequences_of_a_larger_table_and_other_stream():
     """Fewer sequences than the table has rows, on a stream of its own."""
     s = _setup([90, 33, 200], [6, 2, 11], 8, 2, 16, "e4m3", "tree", seed=8)
