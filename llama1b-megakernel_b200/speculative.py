@@ -423,12 +423,14 @@ class SpeculativeDecoder:
         return x
 
     def _logits(self, x: torch.Tensor) -> torch.Tensor:
-        c, pw, rows = self.cfg, self.m.packed, x.shape[0]
-        _lib.check(self.lib.mk_rmsnorm_rows(
-            x.data_ptr(), pw.norm_final.data_ptr(), ctypes.c_float(c.rms_eps), rows, c.hidden, self._h.data_ptr(),
-            torch.cuda.current_stream(self.dev).cuda_stream))
-        logits = torch.empty(rows, c.vocab, dtype=torch.float32, device=self.dev)
-        self._gemm(pw.embed, self._h, rows, out_f32=logits)
+        """fp32 logits of the rows of x, as many at a time as the buffer of normed rows holds."""
+        c, pw = self.cfg, self.m.packed
+        logits = torch.empty(x.shape[0], c.vocab, dtype=torch.float32, device=self.dev)
+        for rows, out in zip(x.split(self.MAX_ROWS), logits.split(self.MAX_ROWS)):
+            _lib.check(self.lib.mk_rmsnorm_rows(
+                rows.data_ptr(), pw.norm_final.data_ptr(), ctypes.c_float(c.rms_eps), len(rows), c.hidden,
+                self._h.data_ptr(), torch.cuda.current_stream(self.dev).cuda_stream))
+            self._gemm(pw.embed, self._h, len(rows), out_f32=out)
         return logits
 
     # ------------------------------------------------------------------ API

@@ -1,0 +1,67 @@
+"""SpeculativeDecoder's host side on the CPU: a decoder whose passes are played by a stand-in, over a
+cache in host memory."""
+from __future__ import annotations
+
+import types
+
+import pytest
+import torch
+
+from llama1b_megakernel_b200.config import TINY
+from llama1b_megakernel_b200.kv_cache import QuantizedPagedKVCache
+from llama1b_megakernel_b200.speculative import SpeculativeDecoder
+
+
+class Recorder:
+    """Stands in for the library: notes the rows that each call is told to write."""
+
+    def __init__(self):
+        self.rows = []
+
+    def mk_rmsnorm_rows(self, x, gamma, eps, rows, hidden, out, stream):
+        self.rows.append(("norm", x, rows, out))
+        return 0
+
+    def mk_gemm_bf16(self, w, n, k, x, rows, pad, residual, out, out_f32, ws, nbytes, err, stream):
+        self.rows.append(("gemm", out_f32, rows, pad))
+        return 0
+
+
+def _decoder(monkeypatch, max_batch=2, max_seq_len=512, num_pages=None, forward=True):
+    dec = object.__new__(SpeculativeDecoder)
+    dec.cfg, dec.dev, dec.lib = TINY, torch.device("cpu"), Recorder()
+    dec.max_batch, dec.max_seq_len, dec.max_nodes, dec.top = max_batch, max_seq_len, 64, 4
+    dec.kv = QuantizedPagedKVCache(TINY, max_batch, max_seq_len, 8, num_pages, device="cpu")
+    dec._pending = [None] * max_batch
+    dec.err = torch.zeros(1, dtype=torch.int32)
+    dec._h = torch.zeros(dec.MAX_ROWS, TINY.hidden, dtype=torch.bfloat16)
+    embed = torch.zeros(TINY.vocab, TINY.hidden, dtype=torch.bfloat16)
+    dec.m = types.SimpleNamespace(packed=types.SimpleNamespace(embed=embed, norm_final=torch.zeros(TINY.hidden)))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: types.SimpleNamespace(cuda_stream=0))
+    dec.passes = []
+    if forward:  # a pass that reserves what it is to write, as the real one does
+        def play(trees):
+            dec.passes.append([list(t.tokens) for t in trees])
+            for b, t in enumerate(trees):
+                assert dec.kv.seq_lens[b] + len(t) <= dec.max_seq_len
+                dec.kv.reserve(b, dec.kv.seq_lens[b] + len(t))
+            return torch.zeros(sum(map(len, trees)), TINY.hidden, dtype=torch.bfloat16)
+        dec._forward = play
+    return dec
+
+
+@pytest.mark.parametrize("batch", [1, 127, 128, 129, 300])
+def test_logits_of_more_prompts_than_a_gemm_takes(monkeypatch, batch):
+    """No call writes more rows than its buffer has, and every prompt's row is computed once."""
+    dec = _decoder(monkeypatch, max_batch=batch)
+    logits = dec.prefill([[1]] * batch)
+    assert logits.shape == (batch, TINY.vocab) and dec.kv.seq_lens == [1] * batch
+    norms = [r for r in dec.lib.rows if r[0] == "norm"]
+    gemms = [r for r in dec.lib.rows if r[0] == "gemm"]
+    assert sum(r[2] for r in norms) == sum(r[2] for r in gemms) == batch
+    at = 0
+    for n, g in zip(norms, gemms):
+        assert 1 <= n[2] == g[2] <= g[3] <= dec.MAX_ROWS == dec._h.shape[0]
+        assert n[3] == dec._h.data_ptr()
+        assert n[1] == norms[0][1] + at * TINY.hidden * 2 and g[1] == logits.data_ptr() + at * TINY.vocab * 4
+        at += n[2]
