@@ -47,6 +47,10 @@ constexpr int kLpCandidates = 512;
 constexpr int kLpMaxSlices = 16;  // CTAs of a cluster
 static_assert(kLpMaxSlices * kLogprobsMaxTop <= kLpCandidates, "a cluster's lists fit the candidates");
 constexpr float kLog2e = 1.4426950408889634f;
+// Distances below a maximum count as no further than this: their exponential is 0 long before, and 0
+// times the distance times a count of logits has to be 0 (logits at the type's lowest value are 3e38
+// away: twice that is infinite, and 0 times it a NaN).
+constexpr float kLpFar = -1e20f;
 
 struct LogprobsParams {
   const void* logits;   // [rows][ld] fp32 or bf16, the first V columns
@@ -161,10 +165,9 @@ __device__ __forceinline__ void lp_join(LpShared& sh, float& m, float& s, float&
 #pragma unroll
   for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   auto shift = [](float m_, float M_, float& s_, float& w_) {
-    // a part without anything: exp(-inf), and no product with the infinite distance
-    const float d = m_ == -INFINITY ? -INFINITY : m_ - M_;
+    const float d = m_ == -INFINITY ? -INFINITY : m_ - M_;  // a part without anything: exp(-inf)
     const float a = __expf(d);
-    w_ = a * (w_ + (d == -INFINITY ? 0.f : d * s_));
+    w_ = a * (w_ + fmaxf(d, kLpFar) * s_);
     s_ = a * s_;
   };
   shift(m, M, s, w);
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(kLpThreads, E == 16 ? 3 : 4) logprobs_kernel(c
     const float best = largest();
     if (best > m) {
       const float a = m == -INFINITY ? 0.f : exp2_approx((m - best) * kLog2e);
-      w = m == -INFINITY ? 0.f * s : a * fmaf(m - best, s, w);  // 0 * s: a NaN stays
+      w = m == -INFINITY ? 0.f * s : a * fmaf(fmaxf(m - best, kLpFar), s, w);  // 0 * s: a NaN stays
       s *= a;
       m = best;
     }
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(kLpThreads, E == 16 ? 3 : 4) logprobs_kernel(c
       float2 d = add2(make_float2(v[e], v[e + 1]), shift);
       const float2 x2 = mul2(d, base2);
       const float2 a = make_float2(exp2_approx(x2.x), exp2_approx(x2.y));
-      d = make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f));  // 0 * -inf adds nothing
+      d = make_float2(fmaxf(d.x, kLpFar), fmaxf(d.y, kLpFar));  // 0 * -inf adds nothing
       const int c = (e >> 1) & 1;
       sx[c] = add2(sx[c], a);
       wx[c] = fma2(a, d, wx[c]);
