@@ -16,17 +16,23 @@
 //    Q goes to f16 under a power of two for each row that brings its largest value
 //    to 2^14: what is lost lies below 2^-38 of it. The row's K scale multiplies the
 //    score. A V fragment pairs two positions of a dim. V's scales multiply P, relative
-//    to the largest one so far (2^E; O is in units of it, and rescaled when it grows),
-//    so P fits f16, with 2^-12 of rounding. Where some V scale of 32 positions is
-//    below 2^(E - 10), f16 could lose P's low bits: those positions take P and V as
-//    bf16 instead (tree_decode's way), whose range holds everything.
+//    to the largest one so far (2^E; O is in units of it, and rescaled when it grows).
+//    A row's largest P is 2^7 (2^15 before O is rescaled), so that P in f16 is rounded
+//    by 2^-11 of itself down to 2^-14, 2^-21 of the largest. What is smaller loses up
+//    to 2^-25, however many positions there are: 32 of them lose at most 2^-23 of a
+//    row's sum of such products if that is 8 or more (kFewEnough), which is looked at
+//    before the products are rounded, until it is. Where a row has less (its largest P met
+//    values of little size, or one of great size came by that it does not look at) the 32
+//    positions are done again with P and V as bf16 (tree_decode's way), which rounds the
+//    smallest by 2^-8 as well. (64 sequences of 2,600 to 4,100 positions: 54.9 us without
+//    a look, 55.6 so; one of 1,025: 5.7 and 5.9.)
 //    The positions of a block of 8 are permuted between fragment columns and rows
 //    in memory (few_place) so that both loads are free of bank conflicts under the
 //    64-byte swizzle.
 // O is rescaled when a maximum grew by more than 8 powers of two, as in mk_tree.cuh.
 //
 // What bounds it: memory, where sequences fill the GPU (36 of 1,000 to 2,000 positions in
-// 8 bits: 18 us; 64 of 2,600 to 4,100: 55 us, 4.1 TB/s, as their 512 CTAs end one by one),
+// 8 bits: 19 us; 64 of 2,600 to 4,100: 56 us, 4.0 TB/s, as their 512 CTAs end one by one),
 // and the latency of a CTA's few chunks where they do not (one of 1,025 bf16: 6.0 us).
 // The split of an SM was measured (consumers x stages x CTAs; 64 of 2,600 to 4,100 in 8
 // bits, and 32 of 2,700 to 4,100 in bf16 with 16 rows): 3 x 6 x 4 55 and 45 us, 4 x 8 x 3 80
@@ -47,6 +53,8 @@ constexpr int kFewStages = 6;
 static_assert(kFewStages % kFewWarps == 0, "a stage belongs to one warp");
 constexpr int kFewCtas = 4;           // of an SM: 16 warps of 128 registers, 12 of them consumers
 constexpr int kFewStageBytes = 8192;  // K rows, then V rows
+constexpr float kFewLead = 7.f;       // 8-bit: log2 of a row's largest P
+constexpr float kFewEnough = 8.f;     // 8-bit: a row's sum of P times V's scale with which f16 loses nothing that shows
 
 template <bool kFp8>
 struct FewShape {
@@ -244,7 +252,11 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
         }
       }
     }
-    float m[2], l[2], o[8][4];
+    constexpr float kLead = kFp8 ? kFewLead : 0.f;
+    float m[2], l[2], o[8][4];  // m: P is 2^(score - m), the maximum's 2^kLead
+    float mass[2] = {};         // 8-bit: this thread's share of a row's sum of P times V's scale, until all rows have
+    bool enough = false;        // kFewEnough; it stays that unless a maximum or V's largest scale grows
+    bool short_of = false;      // the last positions were not enough
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.f;
 #pragma unroll
@@ -259,7 +271,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
     for (int j = warp; j < nchunks; j += kFewWarps) {
       ok = wait_all(full(st), phase);
       if (!ok) break;
-      bool odd = false, wide = false;  // 8-bit: the chunk has a NaN scale; V's scales span more than f16 holds
+      bool odd = false;  // 8-bit: the chunk has a NaN scale
       if (kFp8) {
         // the scales of positions 2 lane and 2 lane + 1; those behind the end, and NaN, do not count
         const uint8_t* sc = smem + L::kScales + st * 2 * C;
@@ -274,12 +286,15 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
           for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int e = 0; e < 2 * X; ++e) o[i][e] *= f;
+          mass[0] *= f;
+          mass[1] *= f;
+          enough = false;
           top_v = most;
         }
-        wide = __reduce_min_sync(0xffffffffu, min(in0 ? v0 : 255, in1 ? v1 : 255)) < top_v - 10;
       }
       const float v_unit = kFp8 ? e8m0_value(max(254 - top_v, 1)) : 1.f;  // 2^(127 - top_v)
-      // 32 positions; kPlain: all committed, every scale a number and V's within f16's reach
+      // 32 positions; kPlain: all committed, every scale a number, P in f16's range (if it is
+      // not: false, and nothing added)
       auto step = [&](auto plain, const int sub) {
         constexpr bool kPlain = decltype(plain)::value;
         const int c0 = p0 + j * C + sub * 32;
@@ -387,18 +402,20 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
 #pragma unroll
           for (int nb = 0; nb < 4; ++nb) t = tree_max3(t, s[nb][2 * x], s[nb][2 * x + 1]);
           mx[x] = t * fac[x];
-          grow |= mx[x] > m[x] + 8.f;
+          grow |= mx[x] > m[x] + (8.f + kLead);
         }
         if (__any_sync(0xffffffffu, grow)) {
+          enough = false;
 #pragma unroll
           for (int x = 0; x < X; ++x) {
             float t = mx[x];  // the row's four lanes agree
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            if (t > m[x] + 8.f) {
-              const float alpha = exp2_approx(m[x] - t);  // 0 for the first maximum
-              m[x] = t;
+            if (t > m[x] + (8.f + kLead)) {
+              const float alpha = exp2_approx(m[x] - (t - kLead));  // 0 for the first maximum
+              m[x] = t - kLead;
               l[x] *= alpha;
+              mass[x] *= alpha;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 o[i][2 * x] *= alpha;
@@ -409,6 +426,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
         }
         // ---- probabilities, as the A fragments of P V
         uint32_t pa[2][4] = {};
+        const float l_was[2] = {l[0], l[1]};
 #pragma unroll
         for (int x = 0; x < X; ++x) {
           const float mu = m[x] == -INFINITY ? 0.f : m[x];
@@ -417,19 +435,53 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
             float e0 = exp2_approx(fmaf(s[nb][2 * x], fac[x], -mu));
             float e1 = exp2_approx(fmaf(s[nb][2 * x + 1], fac[x], -mu));
             l[x] += e0 + e1;
-            uint32_t& a = pa[nb >> 1][(nb & 1) * 2 + x];
             if (kFp8) {
-              e0 *= sv[nb][0];
-              e1 *= sv[nb][1];
-            }
-            if (!kFp8 || (!kPlain && wide)) {
-              __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-              a = *reinterpret_cast<uint32_t*>(&h);
+              s[nb][2 * x] = e0 * sv[nb][0];
+              s[nb][2 * x + 1] = e1 * sv[nb][1];
             } else {
-              __half2 h = __floats2half2_rn(e0, e1);
-              a = *reinterpret_cast<uint32_t*>(&h);
+              __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
+              pa[nb >> 1][(nb & 1) * 2 + x] = *reinterpret_cast<uint32_t*>(&h);
             }
           }
+        }
+        bool wide = false;  // 8-bit: P needs bf16's range
+        if (kFp8) {
+          if (!enough) {
+            bool little = false;
+            float with[2];
+#pragma unroll
+            for (int x = 0; x < X; ++x) {
+              with[x] = mass[x];
+#pragma unroll
+              for (int nb = 0; nb < 4; ++nb) with[x] += s[nb][2 * x] + s[nb][2 * x + 1];
+              float w = with[x];
+              w += __shfl_xor_sync(0xffffffffu, w, 1);
+              w += __shfl_xor_sync(0xffffffffu, w, 2);
+              little |= w < kFewEnough && m[x] > -INFINITY;
+            }
+            wide = __any_sync(0xffffffffu, little);
+            enough = !wide;
+            if (kPlain && wide) {
+#pragma unroll
+              for (int x = 0; x < X; ++x) l[x] = l_was[x];
+              return false;
+            }
+#pragma unroll
+            for (int x = 0; x < X; ++x) mass[x] = with[x];
+          }
+#pragma unroll
+          for (int x = 0; x < X; ++x)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) {
+              uint32_t& a = pa[nb >> 1][(nb & 1) * 2 + x];
+              if (!kPlain && wide) {
+                __nv_bfloat162 h = __floats2bfloat162_rn(s[nb][2 * x], s[nb][2 * x + 1]);
+                a = *reinterpret_cast<uint32_t*>(&h);
+              } else {
+                __half2 h = __floats2half2_rn(s[nb][2 * x], s[nb][2 * x + 1]);
+                a = *reinterpret_cast<uint32_t*>(&h);
+              }
+            }
         }
         // ---- P . V: two steps of 16 positions, eight blocks of 8 dims
 #pragma unroll
@@ -484,15 +536,17 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
             }
           }
         }
+        return true;
       };
 #pragma unroll 1
       for (int sub = 0; sub < C / 32; ++sub) {
         const int c0 = p0 + j * C + sub * 32;
         if (c0 >= p1) break;
-        if (c0 + 32 > prefix || odd || wide)
+        // where the last one was short of mass this one is likely to be, so it is not tried in f16
+        if (c0 + 32 > prefix || odd || (kFp8 && short_of) || !step(std::true_type{}, sub)) {
           step(std::false_type{}, sub);
-        else
-          step(std::true_type{}, sub);
+          short_of = !enough;
+        }
       }
       __syncwarp();
       if (lane == 0) tree_arrive(empty(st));
@@ -503,17 +557,17 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
       }
     }
 
-    // ---- the four warps joined; their states lie over the ring, which nobody reads any more
+    // ---- the three warps joined; their states lie over the ring, which nobody reads any more
     float* state = reinterpret_cast<float*>(smem);  // [warp][R][kTreePartial]
-    const float unit = kFp8 && top_v ? e8m0_value(top_v) : 1.f;
+    const float lead = kFp8 ? exp2f(-kLead) : 1.f, unit = kFp8 && top_v ? e8m0_value(top_v) * lead : 1.f;
     asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
 #pragma unroll
     for (int x = 0; x < X; ++x) {
-      float t = l[x];
+      float t = l[x] * lead;
       t += __shfl_xor_sync(0xffffffffu, t, 1);
       t += __shfl_xor_sync(0xffffffffu, t, 2);
       float* d = state + (warp * R + x * 8 + g8) * kTreePartial;
-      if (t4 == 0) *reinterpret_cast<float2*>(d + 64) = make_float2(m[x], t);
+      if (t4 == 0) *reinterpret_cast<float2*>(d + 64) = make_float2(m[x] + kLead, t);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (!kFp8) {  // dims 8 i + 2 t4 (+ 1)

@@ -1,4 +1,15 @@
-"""The speculative-decoding operators where their arithmetic is easiest to break."""
+"""The speculative-decoding operators where their arithmetic is easiest to break: rows of an
+8-bit cache whose scales lie far apart, logits at their type's lowest value, cache formats
+that other code may write, places that are refused.
+
+Tolerances follow from the roundings, beside those of tests/test_gpu_speculative.py:
+* scores here are sums of one product that is exact, so what is left of a score's error is its
+  rounding in powers of two, 2^-23 |x| for |x| <= 64, and that of exp2: e = 2^-16 in all;
+* P in 8 significant bits (bf16) or more has u = 2^-8 of every p_j |v_j|, the output u once
+  more; where P is f16, what its smallest numbers lose is kept below 2^-16 of
+  sum_j p_j max_d |v_jd|:
+    |err_d| <= (u + e) sum_j p_j |v_jd| + 2^-16 sum_j p_j max_d |v_jd| + u |o_d|.
+"""
 from __future__ import annotations
 
 import math
@@ -11,6 +22,134 @@ from tests import test_gpu_speculative as base
 
 pytestmark = pytest.mark.gpu
 DEV, U = base.DEV, base.U
+
+
+def _put(s, x, b, pos, rows):
+    """Rows `rows` [n, nkv, 64] (fp64) at places `pos` of sequence b in the pool x ("k" or "v")."""
+    page, off = s["tables"][b].long()[pos // s["ps"]], pos % s["ps"]
+    if s[x + "s"] is None:
+        s[x][page, :, off] = rows.bfloat16()
+        s[x + "64"][page, :, off] = rows.bfloat16().double()
+        return
+    y, byte, _ = base._quantise(rows)
+    s[x].view(torch.uint8)[page, :, off] = y.float().to(torch.float8_e4m3fn).view(torch.uint8)
+    s[x + "s"][page, :, off] = byte
+    s[x + "64"][page, :, off] = y * base._pow2(byte.to(torch.int64) - 127)[..., None]
+
+
+def _compare(s, out, lse, skip=()):
+    """Against the definition in 64 bits, the scores taken as exact."""
+    nq, nkv, ps = s["q"].shape[1], s["k"].shape[1], s["ps"]
+    group, at = nq // nkv, 0
+    for b, (p, n) in enumerate(zip(s["prefixes"], s["nodes"])):
+        j = torch.arange(p + n, device=DEV)
+        pg = s["right_tables"][b].long()[j // ps]
+        kk, vv = (s[x][pg, :, j % ps].transpose(0, 1).repeat_interleave(group, 0) for x in ("k64", "v64"))
+        q = s["q"][at:at + n].double().transpose(0, 1)
+        seen = torch.cat([torch.ones(n, p, dtype=torch.bool), s["masks"][b]], 1).to(DEV)
+        vv = torch.where(seen.any(0)[None, :, None], vv, 0.0)
+        x = torch.where(seen, (q @ kk.transpose(1, 2)) * 0.125, -math.inf)
+        w = torch.softmax(x, -1)
+        want = torch.logsumexp(x, -1)
+        for i in range(n):
+            if (b, i) in skip:
+                continue
+            vi = torch.where(seen[i][None, :, None], vv, 0.0)
+            wi = w[:, i:i + 1]
+            ref, size, most = (wi @ vi)[:, 0], (wi @ vi.abs())[:, 0], wi @ vi.abs().amax(-1, keepdim=True)
+            tol = (U + 2.0 ** -16) * size + 2.0 ** -16 * most[:, 0] + U * ref.abs()
+            off = (out[at + i].double() - ref).abs()
+            assert (off <= tol).all(), (b, i, float((off / tol).max()))
+            assert ((lse[at + i].double() - want[:, i]).abs() <= 2.0 ** -16 + 2.0 ** -22 * want[:, i].abs()).all(), (b, i)
+        at += n
+
+
+def _scored(prefix, nodes, score, fmt="e4m3", nq=8, nkv=1, ps=64, seed=0):
+    """One sequence whose scores are score[j] (multiples that an 8-bit row holds exactly), of
+    every node alike: q is 8 in dim 0, and a key's dim 0 its score."""
+    s = base._setup([prefix], [nodes], nq, nkv, ps, fmt, "chain", seed=seed)
+    s["q"].zero_()
+    s["q"][..., 0] = 8
+    n = prefix + nodes
+    k = torch.randn(n, nkv, 64, generator=base._gen(seed + 1), device=DEV).double()
+    k[..., 0] = score[:n, None]
+    _put(s, "k", 0, torch.arange(n, device=DEV), k)
+    return s
+
+
+def _many(s, batch=600):
+    """The one sequence of s as many that share its pages, so that none is cut into ranges; the
+    comparison is of the first, and every one has to give its bits."""
+    nodes = s["nodes"][0]
+    return dict(s, tables=s["tables"].repeat(batch, 1), q=s["q"].repeat(batch, 1, 1), mask=s["mask"].repeat(batch, 1),
+                prefix=s["prefix"].repeat(batch), cu=torch.arange(batch + 1, dtype=torch.int32, device=DEV) * nodes)
+
+
+def _attend_many(s):
+    nodes = s["nodes"][0]
+    out, lse, err = base._attend(_many(s))
+    assert int(err) == 0
+    for x in (out, lse):
+        assert torch.equal(x.view(-1, nodes, *x.shape[1:]), x[:nodes].expand(x.shape[0] // nodes, *x[:nodes].shape))
+    return out[:nodes], lse[:nodes]
+
+
+# ------------------------------------------------------------------ scales far apart
+@pytest.mark.parametrize("nodes", [1, 2, 20])
+@pytest.mark.parametrize("spread", [0, 2, 4, 7, 10, 14, 24])
+@pytest.mark.parametrize("peak,sink", [(10, False), (10, True), (14, True), (20, False), (20, True)])
+def test_flat_tail_beside_a_peak(nodes, spread, peak, sink):
+    """Thousands of keys of one small probability behind some with e^peak times theirs (with
+    `sink`, of no value), where rows of 2^spread times the size came by that nobody looks at:
+    the small probabilities together are the result, or a part of it that shows."""
+    n = 4096 + nodes
+    j = torch.arange(n, device=DEV)
+    score = torch.zeros(n, dtype=torch.float64, device=DEV)
+    outlier = j % 64 == 5
+    score[outlier] = -208.0
+    score[10:400:64] = peak  # one for each warp, wherever a block of positions goes
+    s = _scored(4096, nodes, score, seed=peak + spread)
+    v = torch.randn(n, 1, 64, generator=base._gen(7), device=DEV).double()
+    v[outlier] *= 2.0 ** spread
+    if sink:
+        v[10:400:64] = 0
+    _put(s, "v", 0, j, v)
+    _compare(s, *_attend_many(s))
+
+
+@pytest.mark.parametrize("nodes", [1, 2, 20])
+@pytest.mark.parametrize("prefix", [100, 3000])
+@pytest.mark.parametrize("late", [True, False])
+def test_small_probabilities_of_large_values(nodes, prefix, late):
+    """Half of the rows are 2^20 times as large and e^-14 times as probable: both halves count
+    alike, whichever comes first."""
+    n = prefix + nodes
+    j = torch.arange(n, device=DEV)
+    large = (j >= prefix // 2) == late
+    s = _scored(prefix, nodes, torch.where(large, -14.0, 0.0).double(), seed=prefix)
+    v = torch.randn(n, 1, 64, generator=base._gen(prefix), device=DEV).double()
+    _put(s, "v", 0, j, torch.where(large[:, None, None], v * 2.0 ** 20, v))
+    _compare(s, *_attend_many(s))
+
+
+@pytest.mark.parametrize("nodes,nq,nkv", [(1, 8, 1), (4, 8, 2), (30, 8, 2)])
+@pytest.mark.parametrize("lowest", [-4, -14, -40])
+@pytest.mark.parametrize("size", [0, 20])
+def test_rows_of_every_size(nodes, nq, nkv, lowest, size):
+    """K and V rows of sizes spread over powers of two, and all of them large (scale bytes that
+    take two factors to become bf16), with queries as much smaller."""
+    s = base._setup([700, 0, 65], [nodes] * 3, nq, nkv, 16, "e4m3", "tree", seed=nodes - lowest)
+    g = base._gen(size)
+    for b, p in enumerate(s["prefixes"]):
+        n = p + nodes
+        j = torch.arange(n, device=DEV)
+        for x, low in (("k", max(lowest, -6)), ("v", lowest)):
+            e = torch.rand(n, nkv, 1, generator=g, device=DEV) * low + size
+            _put(s, x, b, j, torch.randn(n, nkv, 64, generator=g, device=DEV).double() * torch.exp2(e.double()))
+    s["q"] *= 2.0 ** -size
+    out, lse, err = base._attend(s)
+    assert int(err) == 0
+    base._check(s, out, lse)
 
 
 # ------------------------------------------------------------------ log probabilities
