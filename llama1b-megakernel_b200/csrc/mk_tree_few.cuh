@@ -16,7 +16,8 @@
 //    Q goes to f16 under a power of two for each row that brings its largest value
 //    to 2^14: what is lost lies below 2^-38 of it. The row's K scale multiplies the
 //    score. A V fragment pairs two positions of a dim. V's scales multiply P, relative
-//    to the largest one so far (2^E; O is in units of it, and rescaled when it grows).
+//    to the largest one that the row has seen so far (2^E; O is in units of it, and
+//    rescaled when it grows; a drafted node counts for the rows that see it).
 //    A row's largest P is 2^7 (2^15 before O is rescaled), so that P in f16 is rounded
 //    by 2^-11 of itself down to 2^-14, 2^-21 of the largest. What is smaller loses up
 //    to 2^-25, however many positions there are: 32 of them lose at most 2^-23 of a
@@ -25,7 +26,7 @@
 //    values of little size, or one of great size came by that it does not look at) the 32
 //    positions are done again with P and V as bf16 (tree_decode's way), which rounds the
 //    smallest by 2^-8 as well. (64 sequences of 2,600 to 4,100 positions: 54.9 us without
-//    a look, 55.6 so; one of 1,025: 5.7 and 5.9.)
+//    a look, 55.8 so; one of 1,025: 5.7 and 5.9.)
 //    The positions of a block of 8 are permuted between fragment columns and rows
 //    in memory (few_place) so that both loads are free of bank conflicts under the
 //    64-byte swizzle.
@@ -261,8 +262,19 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
     l[0] = l[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    int top_v = 0;  // 8-bit: O's unit is 2^(top_v - 127)
+    int top_v[2] = {};  // 8-bit: a row's unit of O is 2^(top_v - 127); the rows' are equal before drafted positions
     bool ok = true;
+    // 8-bit: O in a unit 2^down as large; what falls out of fp32 is that far below a value that the row sees
+    auto grow_unit = [&](int x, int down) {
+      const float f = down <= 126 ? e8m0_value(127 - down) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        o[i][2 * x] *= f;
+        o[i][2 * x + 1] *= f;
+      }
+      mass[x] *= f;
+      top_v[x] += down;
+    };
     // this thread's places in 32 rows of a chunk
     const uint32_t k_at = kFp8 ? few_place(g8) * 64 + ((t4 ^ ((few_place(g8) >> 1) & 3)) << 4) : (lane & 7) * 128;
     const uint32_t v_at[2] = {few_v_at(2 * t4, g8), few_v_at(2 * t4 + 1, g8)};
@@ -273,26 +285,20 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
       if (!ok) break;
       bool odd = false;  // 8-bit: the chunk has a NaN scale
       if (kFp8) {
-        // the scales of positions 2 lane and 2 lane + 1; those behind the end, and NaN, do not count
+        // the scales of positions 2 lane and 2 lane + 1; of V's those of committed positions that are numbers count
         const uint8_t* sc = smem + L::kScales + st * 2 * C;
         const uint32_t k2 = reinterpret_cast<const uint16_t*>(sc)[lane], v2 = reinterpret_cast<const uint16_t*>(sc + C)[lane];
         const int v0 = v2 & 255, v1 = v2 >> 8, pos = p0 + j * C + 2 * lane;
         odd = __any_sync(0xffffffffu, (k2 & 255) == kScaleNaN || (k2 >> 8) == kScaleNaN || v0 == kScaleNaN || v1 == kScaleNaN);
-        const bool in0 = pos < end && v0 != kScaleNaN, in1 = pos + 1 < end && v1 != kScaleNaN;
+        const bool in0 = pos < prefix && v0 != kScaleNaN, in1 = pos + 1 < prefix && v1 != kScaleNaN;
         const int most = __reduce_max_sync(0xffffffffu, max(in0 ? v0 : 0, in1 ? v1 : 0));
-        if (most > top_v) {
-          const float f = top_v ? e8m0_value(max(127 + top_v - most, 1)) : 1.f;
+        if (most > top_v[0]) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 2 * X; ++e) o[i][e] *= f;
-          mass[0] *= f;
-          mass[1] *= f;
+          for (int x = 0; x < X; ++x) grow_unit(x, most - top_v[x]);
           enough = false;
-          top_v = most;
         }
       }
-      const float v_unit = kFp8 ? e8m0_value(max(254 - top_v, 1)) : 1.f;  // 2^(127 - top_v)
+      const float all_unit = kFp8 ? e8m0_value(max(254 - top_v[0], 1)) : 1.f;  // 2^(127 - top_v), before drafted positions
       // 32 positions; kPlain: all committed, every scale a number, P in f16's range (if it is
       // not: false, and nothing added)
       auto step = [&](auto plain, const int sub) {
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
             for (int e = 0; e < 2; ++e) {
               // the byte on top, then down by one: a float's exponent
               const uint32_t kx = __byte_perm(ks, 0, e ? pick1 : pick0) >> 1, vx = __byte_perm(vs, 0, e ? pick1 : pick0) >> 1;
-              float kf = __uint_as_float(kx), vf = __uint_as_float(vx) * v_unit;
+              float kf = __uint_as_float(kx), vf = __uint_as_float(vx);
               if (!kPlain && (tail || odd)) {
                 if (kx == 0x7F800000u) kf = __uint_as_float(0x7FFFFFFFu);
                 if (vx == 0x7F800000u) vf = __uint_as_float(0x7FFFFFFFu);
@@ -392,6 +398,28 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
               for (int x = 0; x < X; ++x)
                 if (!((vis[x] >> at) & 1)) s[nb][2 * x + e] = -INFINITY;
             }
+          if (kFp8) {  // the largest scale of V that a row sees here
+#pragma unroll
+            for (int x = 0; x < X; ++x) {
+              float t = 0.f;
+#pragma unroll
+              for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if ((vis[x] >> (nb * 8 + few_place(2 * t4 + e))) & 1) t = fmaxf(t, sv[nb][e]);  // not a NaN's
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+              const int most = (int)(__float_as_uint(t) >> 23);
+              const bool more = most > top_v[x];
+              if (more) grow_unit(x, most - top_v[x]);
+              if (__any_sync(0xffffffffu, more)) enough = false;
+            }
+          }
+        }
+        float v_unit[2] = {all_unit, all_unit};
+        if (kFp8 && tail) {
+#pragma unroll
+          for (int x = 0; x < X; ++x) v_unit[x] = e8m0_value(max(254 - top_v[x], 1));
         }
         // ---- maxima
         float mx[2];
@@ -436,8 +464,14 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
             float e1 = exp2_approx(fmaf(s[nb][2 * x + 1], fac[x], -mu));
             l[x] += e0 + e1;
             if (kFp8) {
-              s[nb][2 * x] = e0 * sv[nb][0];
-              s[nb][2 * x + 1] = e1 * sv[nb][1];
+              // V's scales in the row's unit: at most 1 where it sees the position
+              float w0 = sv[nb][0] * v_unit[x], w1 = sv[nb][1] * v_unit[x];
+              if (tail) {
+                w0 = w0 > 1.f ? 1.f : w0;  // (a NaN stays)
+                w1 = w1 > 1.f ? 1.f : w1;
+              }
+              s[nb][2 * x] = e0 * w0;
+              s[nb][2 * x + 1] = e1 * w1;
             } else {
               __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
               pa[nb >> 1][(nb & 1) * 2 + x] = *reinterpret_cast<uint32_t*>(&h);
@@ -475,7 +509,8 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
             for (int nb = 0; nb < 4; ++nb) {
               uint32_t& a = pa[nb >> 1][(nb & 1) * 2 + x];
               if (!kPlain && wide) {
-                __nv_bfloat162 h = __floats2bfloat162_rn(s[nb][2 * x], s[nb][2 * x + 1]);
+                // 2^60 from V to P: P may be as small as V's scales lie apart
+                __nv_bfloat162 h = __floats2bfloat162_rn(s[nb][2 * x] * 0x1p60f, s[nb][2 * x + 1] * 0x1p60f);
                 a = *reinterpret_cast<uint32_t*>(&h);
               } else {
                 __half2 h = __floats2half2_rn(s[nb][2 * x], s[nb][2 * x + 1]);
@@ -519,7 +554,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
                 few_mma<true>(o[d + 1], pa[ks], bf[1][0], bf[1][1]);
               }
             } else {
-              const __nv_bfloat162 f = tree_pow2(247);  // 2^120
+              const __nv_bfloat162 f = tree_pow2(247 - 60);  // 2^120 of the code, 2^-60
 #pragma unroll
               for (int d = 0; d < 8; ++d) {
                 uint32_t bf[2];
@@ -559,13 +594,14 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
 
     // ---- the three warps joined; their states lie over the ring, which nobody reads any more
     float* state = reinterpret_cast<float*>(smem);  // [warp][R][kTreePartial]
-    const float lead = kFp8 ? exp2f(-kLead) : 1.f, unit = kFp8 && top_v ? e8m0_value(top_v) * lead : 1.f;
+    const float lead = kFp8 ? exp2f(-kLead) : 1.f;
     asm volatile("bar.sync 1, %0;" ::"n"(kFewWarps * 32) : "memory");
 #pragma unroll
     for (int x = 0; x < X; ++x) {
       float t = l[x] * lead;
       t += __shfl_xor_sync(0xffffffffu, t, 1);
       t += __shfl_xor_sync(0xffffffffu, t, 2);
+      const float unit = kFp8 && top_v[x] ? e8m0_value(top_v[x]) * lead : 1.f;
       float* d = state + (warp * R + x * 8 + g8) * kTreePartial;
       if (t4 == 0) *reinterpret_cast<float2*>(d + 64) = make_float2(m[x] + kLead, t);
 #pragma unroll

@@ -152,6 +152,31 @@ def test_rows_of_every_size(nodes, nq, nkv, lowest, size):
     base._check(s, out, lse)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("nodes", [2, 4, 30])
+@pytest.mark.parametrize("prefix", [0, 40, 700])
+@pytest.mark.parametrize("small", [0, 20, 60])
+def test_huge_values_in_masked_places(fmt, nodes, prefix, small):
+    """A node of 3e38 that only itself sees does not take a bit from the other rows, of size
+    1 or 2^-small."""
+    s = base._setup([prefix, 64], [nodes] * 2, 8, 2, 16, fmt, "tree", seed=prefix + nodes, qscale=6.0)
+    j = torch.arange(prefix + nodes, device=DEV)
+    v = torch.randn(prefix + nodes, 2, 64, generator=base._gen(small), device=DEV).double()
+    _put(s, "v", 0, j, v * 2.0 ** -small)
+    leaf = nodes - 1
+    s["masks"][0][leaf, :leaf] = False  # a root of its own
+    s["mask"] = base._words(s["masks"], s["T"])
+    huge = torch.full((1, 2, 64), 3.0e38, dtype=torch.float64, device=DEV)
+    huge[..., ::2] *= -1
+    at = torch.tensor([prefix + leaf], device=DEV)
+    _put(s, "k", 0, at, huge)
+    _put(s, "v", 0, at, huge)
+    out, lse, err = base._attend(s)
+    assert int(err) == 0
+    finite = dict(s, k64=torch.where(s["k64"].abs() > 1e38, 0.0, s["k64"]))  # the tolerance is of what rows see
+    base._check(finite, out, lse, skip={(0, leaf)})
+
+
 # ------------------------------------------------------------------ log probabilities
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab", [(1, 128256), (2, 20000), (300, 4099), (700, 9000), (3, 700)])
