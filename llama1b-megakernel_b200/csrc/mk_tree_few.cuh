@@ -262,7 +262,9 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
     l[0] = l[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    int top_v[2] = {};  // 8-bit: a row's unit of O is 2^(top_v - 127); the rows' are equal before drafted positions
+    // 8-bit: a row's unit of O is 2^(top_v - 127); before drafted positions the rows' are equal, and all_unit 1 / it
+    int top_v[2] = {};
+    float all_unit = e8m0_value(254);
     bool ok = true;
     // 8-bit: O in a unit 2^down as large; what falls out of fp32 is that far below a value that the row sees
     auto grow_unit = [&](int x, int down) {
@@ -283,22 +285,28 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
     for (int j = warp; j < nchunks; j += kFewWarps) {
       ok = wait_all(full(st), phase);
       if (!ok) break;
-      bool odd = false;  // 8-bit: the chunk has a NaN scale
+      bool odd = false;  // 8-bit: the chunk has a scale byte whose float is not its power of two: 255 (NaN) or 0 (2^-127)
       if (kFp8) {
-        // the scales of positions 2 lane and 2 lane + 1; of V's those of committed positions that are numbers count
+        // the scales of positions 2 lane and 2 lane + 1; what lies behind the end is nothing
         const uint8_t* sc = smem + L::kScales + st * 2 * C;
         const uint32_t k2 = reinterpret_cast<const uint16_t*>(sc)[lane], v2 = reinterpret_cast<const uint16_t*>(sc + C)[lane];
         const int v0 = v2 & 255, v1 = v2 >> 8, pos = p0 + j * C + 2 * lane;
-        odd = __any_sync(0xffffffffu, (k2 & 255) == kScaleNaN || (k2 >> 8) == kScaleNaN || v0 == kScaleNaN || v1 == kScaleNaN);
-        const bool in0 = pos < prefix && v0 != kScaleNaN, in1 = pos + 1 < prefix && v1 != kScaleNaN;
-        const int most = __reduce_max_sync(0xffffffffu, max(in0 ? v0 : 0, in1 ? v1 : 0));
+        const bool whole = p0 + j * C + C <= prefix;
+        uint32_t four = k2 | v2 << 16;
+        if (!whole) four = pos + 1 < end ? four : pos < end ? (four & 0x00FF00FFu) | 0x7F007F00u : 0x7F7F7F7Fu;
+        const uint32_t zero = (four - 0x01010101u) & ~four, ones = (~four - 0x01010101u) & four;  // a byte of 0, of 255
+        odd = __any_sync(0xffffffffu, (zero | ones) & 0x80808080u);
+        int most = max(v0, v1);  // of V's, those of committed positions that are numbers count
+        if (!whole || odd)
+          most = max(pos < prefix && v0 != kScaleNaN ? v0 : 0, pos + 1 < prefix && v1 != kScaleNaN ? v1 : 0);
+        most = __reduce_max_sync(0xffffffffu, most);
         if (most > top_v[0]) {
 #pragma unroll
           for (int x = 0; x < X; ++x) grow_unit(x, most - top_v[x]);
+          all_unit = e8m0_value(254 - most);
           enough = false;
         }
       }
-      const float all_unit = kFp8 ? e8m0_value(max(254 - top_v[0], 1)) : 1.f;  // 2^(127 - top_v), before drafted positions
       // 32 positions; kPlain: all committed, every scale a number, P in f16's range (if it is
       // not: false, and nothing added)
       auto step = [&](auto plain, const int sub) {
@@ -375,7 +383,11 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               // the byte on top, then down by one: a float's exponent
-              const uint32_t kx = __byte_perm(ks, 0, e ? pick1 : pick0) >> 1, vx = __byte_perm(vs, 0, e ? pick1 : pick0) >> 1;
+              uint32_t kx = __byte_perm(ks, 0, e ? pick1 : pick0) >> 1, vx = __byte_perm(vs, 0, e ? pick1 : pick0) >> 1;
+              if (!kPlain) {
+                kx = max(kx, 0x00400000u);  // byte 0: 2^-127
+                vx = max(vx, 0x00400000u);
+              }
               float kf = __uint_as_float(kx), vf = __uint_as_float(vx);
               if (!kPlain && (tail || odd)) {
                 if (kx == 0x7F800000u) kf = __uint_as_float(0x7FFFFFFFu);
@@ -419,7 +431,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
         float v_unit[2] = {all_unit, all_unit};
         if (kFp8 && tail) {
 #pragma unroll
-          for (int x = 0; x < X; ++x) v_unit[x] = e8m0_value(max(254 - top_v[x], 1));
+          for (int x = 0; x < X; ++x) v_unit[x] = e8m0_value(254 - top_v[x]);
         }
         // ---- maxima
         float mx[2];
@@ -601,7 +613,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
       float t = l[x] * lead;
       t += __shfl_xor_sync(0xffffffffu, t, 1);
       t += __shfl_xor_sync(0xffffffffu, t, 2);
-      const float unit = kFp8 && top_v[x] ? e8m0_value(top_v[x]) * lead : 1.f;
+      const float unit = kFp8 ? e8m0_value(top_v[x]) * lead : 1.f;
       float* d = state + (warp * R + x * 8 + g8) * kTreePartial;
       if (t4 == 0) *reinterpret_cast<float2*>(d + 64) = make_float2(m[x] + kLead, t);
 #pragma unroll

@@ -144,6 +144,7 @@ def decode_rows(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """What codes and scale bytes stand for, in bf16 (exact)."""
     byte = scales.to(torch.int32)
     f = (byte << 23).view(torch.float32)
+    f = torch.where(byte == 0, torch.full_like(f, 2.0 ** -127), f)
     f = torch.where(byte == 255, torch.full_like(f, float("nan")), f)
     return (codes.float() * f[..., None]).to(torch.bfloat16)
 

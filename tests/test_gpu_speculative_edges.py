@@ -177,6 +177,47 @@ def test_huge_values_in_masked_places(fmt, nodes, prefix, small):
     base._check(finite, out, lse, skip={(0, leaf)})
 
 
+# ------------------------------------------------------------------ scale bytes that other code may write
+@pytest.mark.parametrize("nodes", [1, 2, 20])
+@pytest.mark.parametrize("x,byte", [("k", 0), ("v", 0), ("v", 1), ("v", 254)])
+def test_extreme_scale_bytes(nodes, x, byte):
+    """Byte 0 stands for 2^-127 and 254 for 2^127, as every other byte for its power."""
+    prefix = 40
+    s = base._setup([prefix], [nodes], 8, 1, 8, "e4m3", "chain", seed=byte)
+    g, n = base._gen(byte + 1), prefix + nodes
+    lo, hi = (64, 448) if byte < 254 else (2.0 ** -9, 2.0 ** -6)
+    mag = torch.rand(n, 1, 64, generator=g, device=DEV) * (hi - lo) + lo
+    code = (mag * torch.where(torch.rand(n, 1, 64, generator=g, device=DEV) < 0.5, -1.0, 1.0)).to(torch.float8_e4m3fn)
+    j = torch.arange(n, device=DEV)
+    page, off = s["tables"][0].long()[j // 8], j % 8
+    s[x].view(torch.uint8)[page, :, off] = code.view(torch.uint8)
+    s[x + "s"][page, :, off] = byte
+    s[x + "64"][page, :, off] = code.double() * 2.0 ** (byte - 127)
+    if x == "k":
+        s["q"] *= 2.0 ** 118
+    else:
+        s["q"].zero_()
+    out, lse, err = base._attend(s)
+    assert int(err) == 0
+    if x == "k":
+        base._check(s, out, lse)
+    else:
+        _compare(s, out, lse)
+
+
+def test_rows_of_scale_byte_0_read_back():
+    from llama1b_megakernel_b200.kv_cache import decode_rows
+
+    codes = torch.linspace(-448, 448, 64, device=DEV).to(torch.float8_e4m3fn).view(1, 1, 1, 64).expand(1, 1, 8, 64).contiguous()
+    scales = torch.tensor([0, 1, 17, 127, 128, 200, 246, 255], dtype=torch.uint8, device=DEV).view(1, 1, 8)
+    layer = sp.KVLayer(codes, codes, torch.zeros(1, 1, dtype=torch.int32, device=DEV), scales, scales)
+    k, _ = sp.kv_read(layer, torch.tensor([8], dtype=torch.int32, device=DEV), 8)
+    want = (codes.double() * torch.exp2(scales.double() - 127)[..., None]).bfloat16()[0]
+    host = decode_rows(codes.cpu(), scales.cpu())[0]
+    assert torch.equal(k[0, :, :7], want[:, :7]) and torch.equal(host[:, :7], want[:, :7].cpu())
+    assert k[0, :, 7].isnan().all() and host[:, 7].isnan().all()
+
+
 # ------------------------------------------------------------------ log probabilities
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab", [(1, 128256), (2, 20000), (300, 4099), (700, 9000), (3, 700)])

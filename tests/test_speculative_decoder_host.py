@@ -65,3 +65,12 @@ def test_logits_of_more_prompts_than_a_gemm_takes(monkeypatch, batch):
         assert n[3] == dec._h.data_ptr()
         assert n[1] == norms[0][1] + at * TINY.hidden * 2 and g[1] == logits.data_ptr() + at * TINY.vocab * 4
         at += n[2]
+
+
+def test_every_scale_byte_is_its_power_of_two():
+    from llama1b_megakernel_b200.kv_cache import decode_rows
+
+    codes = torch.full((256, 64), 1.5).to(torch.float8_e4m3fn)
+    got = decode_rows(codes, torch.arange(256, dtype=torch.uint8)).double()
+    assert torch.equal(got[:255, 0], 1.5 * torch.exp2(torch.arange(255, dtype=torch.float64) - 127))
+    assert got[255].isnan().all()
