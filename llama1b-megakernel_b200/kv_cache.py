@@ -67,13 +67,11 @@ class PagedKVCache:
             raise ValueError(f"length {length} exceeds max_seq_len {self.max_seq_len}")
         need = (length + self.page_size - 1) // self.page_size
         table = self._host_tables[seq]
-        changed = False
-        while len(table) < need:
-            if not self._free:
-                raise RuntimeError("KV page pool exhausted")
-            table.append(self._free.pop())
-            changed = True
-        if changed:
+        more = need - len(table)
+        if more > len(self._free):
+            raise RuntimeError("KV page pool exhausted")
+        if more > 0:
+            table += [self._free.pop() for _ in range(more)]
             row = torch.tensor(table + [-1] * (self.max_blocks - len(table)), dtype=torch.int32)
             self.block_tables[seq].copy_(row.to(self.device))
 
