@@ -75,6 +75,16 @@ class PagedKVCache:
             row = torch.tensor(table + [-1] * (self.max_blocks - len(table)), dtype=torch.int32)
             self.block_tables[seq].copy_(row.to(self.device))
 
+    def reserve_all(self, lengths) -> None:
+        """``reserve`` for sequences 0, 1, ... together: where one does not fit, none is."""
+        if max(lengths) > self.max_blocks * self.page_size:
+            raise ValueError(f"length {max(lengths)} exceeds max_seq_len {self.max_seq_len}")
+        more = sum(max(0, -(-n // self.page_size) - len(table)) for n, table in zip(lengths, self._host_tables))
+        if more > len(self._free):
+            raise RuntimeError(f"KV page pool exhausted: {more} pages wanted, {len(self._free)} free")
+        for seq, n in enumerate(lengths):
+            self.reserve(seq, n)
+
     def shuffle_free_pages(self, seed: int) -> None:
         """Hand out free pages in a seeded random order (exercises the page indirection)."""
         g = torch.Generator().manual_seed(seed)

@@ -367,6 +367,17 @@ class SpeculativeDecoder:
         self._pending: list[DraftTree | None] = [None] * max_batch
 
     # ------------------------------------------------------------------ one pass
+    def _admit(self, tokens: list[list[int]]) -> None:
+        """Pages for each sequence's new tokens behind its committed positions. What does not
+        fit is refused before anything has changed."""
+        lengths = [self.kv.seq_lens[b] + len(t) for b, t in enumerate(tokens)]
+        for b, (t, n) in enumerate(zip(tokens, lengths)):
+            if n > self.max_seq_len:
+                raise ValueError(f"sequence {b}: {n - len(t)} + {len(t)} positions exceed max_seq_len {self.max_seq_len}")
+            if t and not 0 <= min(t) <= max(t) < self.cfg.vocab:
+                raise ValueError(f"sequence {b}: token id outside the vocabulary")
+        self.kv.reserve_all(lengths)
+
     def _gemm(self, w, x, rows, out=None, out_f32=None, residual=None):
         n, k = w.shape
         pad = 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128
@@ -377,24 +388,18 @@ class SpeculativeDecoder:
 
     @torch.no_grad()
     def _forward(self, trees: list[DraftTree]) -> torch.Tensor:
-        """The nodes of one tree per sequence through the layers, their K/V behind the
-        committed positions; the residual stream [rows, hidden] after the last."""
+        """The nodes of one tree per sequence (after ``_admit``) through the layers, their K/V
+        behind the committed positions; the residual stream [rows, hidden] after the last."""
         c, pw, lib, kv, dev = self.cfg, self.m.packed, self.lib, self.kv, self.dev
         sizes = [len(t) for t in trees]
         rows = sum(sizes)
         base = [kv.seq_lens[b] for b in range(len(trees))]
-        for b, n in enumerate(sizes):
-            if base[b] + n > self.max_seq_len:
-                raise ValueError(f"sequence {b}: {base[b]} + {n} positions exceed max_seq_len {self.max_seq_len}")
-            kv.reserve(b, base[b] + n)
         T = max(sizes)
         max_len = max(p + n for p, n in zip(base, sizes))
         seqs = [b for b, n in enumerate(sizes) for _ in range(n)]
         slots = [base[b] + i for b, n in enumerate(sizes) for i in range(n)]
         positions = [base[b] + d for b, t in enumerate(trees) for d in t.depths()]
         tokens = [x for t in trees for x in t.tokens]
-        if min(tokens) < 0 or max(tokens) >= c.vocab:
-            raise ValueError("token id outside the vocabulary")
         cu = [sum(sizes[:b]) for b in range(len(sizes) + 1)]
         ints = torch.tensor(tokens + seqs + slots + positions + cu + base, dtype=torch.int32).to(dev)
         tokens, seqs, slots, positions = (ints[i * rows:(i + 1) * rows] for i in range(4))
@@ -437,12 +442,14 @@ class SpeculativeDecoder:
     def prefill(self, prompts) -> torch.Tensor:
         """Commit one prompt per sequence (a list of 1-D token tensors or lists, any
         lengths), continuing from what each has; returns the fp32 logits [B, vocab]
-        after each prompt's last token."""
+        after each prompt's last token. Prompts that do not fit (``max_seq_len``, the
+        page pool, the vocabulary) are refused before any is taken."""
         prompts = [torch.as_tensor(p).reshape(-1).tolist() for p in prompts]
         if not 1 <= len(prompts) <= self.max_batch or not all(prompts):
             raise ValueError(f"prefill takes 1 to {self.max_batch} prompts with at least one token each")
         if any(self._pending):
             raise ValueError("commit or drop the scored trees first")
+        self._admit(prompts)
         done = [0] * len(prompts)
         last = torch.empty(len(prompts), self.cfg.hidden, dtype=torch.bfloat16, device=self.dev)
         while any(d < len(p) for d, p in zip(done, prompts)):
@@ -469,6 +476,7 @@ class SpeculativeDecoder:
         sizes = [len(t) for t in trees]
         if min(sizes) < 1 or max(sizes) > self.max_nodes or sum(sizes) > self.MAX_ROWS:
             raise ValueError(f"trees of {sizes} nodes: 1 to {self.max_nodes} each, {self.MAX_ROWS} together")
+        self._admit([t.tokens for t in trees])
         logits = self._logits(self._forward(trees))
         kids = [t.children() for t in trees]
         most = max(1, max(len(k) for ks in kids for k in ks[:-1]))

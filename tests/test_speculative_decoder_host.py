@@ -9,7 +9,7 @@ import torch
 
 from llama1b_megakernel_b200.config import TINY
 from llama1b_megakernel_b200.kv_cache import QuantizedPagedKVCache
-from llama1b_megakernel_b200.speculative import SpeculativeDecoder
+from llama1b_megakernel_b200.speculative import DraftTree, SpeculativeDecoder
 
 
 class Recorder:
@@ -74,3 +74,51 @@ def test_every_scale_byte_is_its_power_of_two():
     got = decode_rows(codes, torch.arange(256, dtype=torch.uint8)).double()
     assert torch.equal(got[:255, 0], 1.5 * torch.exp2(torch.arange(255, dtype=torch.float64) - 127))
     assert got[255].isnan().all()
+
+
+# ------------------------------------------------------------------ refusals leave things as they were
+def _state(dec):
+    kv = dec.kv
+    return list(kv.seq_lens), [kv.pages_of(b) for b in range(kv.max_batch)], sorted(kv._free), kv.block_tables.clone()
+
+
+def _same(a, b):
+    return a[:3] == b[:3] and torch.equal(a[3], b[3])
+
+
+@pytest.mark.parametrize("prompts,error", [
+    ([[1] * 300, [2] * 513], ValueError),               # the second is too long, after three passes of the first
+    ([[1] * 300 + [TINY.vocab]], ValueError),           # a bad token in the third pass
+    ([[1] * 10, [2] * 140 + [-1]], ValueError),
+    ([[1] * 200, [2] * 200], RuntimeError),             # more pages than there are
+])
+def test_refused_prefill_changes_nothing(monkeypatch, prompts, error):
+    dec = _decoder(monkeypatch, num_pages=64 if error is ValueError else 40)
+    dec.prefill([[3] * 5, [4]])  # something committed before
+    was, passes = _state(dec), len(dec.passes)
+    with pytest.raises(error):
+        dec.prefill(prompts)
+    assert _same(was, _state(dec)) and len(dec.passes) == passes
+    dec.prefill([[1, 2, 3]])
+    assert dec.kv.seq_lens == [8, 1]
+
+
+def test_prefill_in_passes(monkeypatch):
+    """What is right still goes through: every token once, in order."""
+    dec = _decoder(monkeypatch)
+    a, b = list(range(1, 301)), list(range(400, 500))
+    dec.prefill([a, b])
+    assert dec.kv.seq_lens == [300, 100]
+    assert [t for p in dec.passes for t in p[0]] == a and [t for p in dec.passes for t in p[1]] == b
+    assert all(sum(map(len, p)) <= 128 for p in dec.passes)
+
+
+@pytest.mark.parametrize("bad,error", [(DraftTree.chain([2] * 60), ValueError), (DraftTree.chain([2, TINY.vocab]), ValueError),
+                                       (DraftTree.chain([2] * 30), RuntimeError)])
+def test_refused_score_changes_nothing(monkeypatch, bad, error):
+    dec = _decoder(monkeypatch, max_seq_len=64, num_pages=4 if error is RuntimeError else None)
+    dec.prefill([[3] * 5, [4] * 8])
+    was, passes = _state(dec), len(dec.passes)
+    with pytest.raises(error):
+        dec.score([DraftTree.chain([1] * 9), bad])
+    assert _same(was, _state(dec)) and len(dec.passes) == passes and not any(dec._pending)
