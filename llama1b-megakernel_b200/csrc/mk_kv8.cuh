@@ -20,10 +20,10 @@
 // numbers are exact there, so a rotated value is rounded once by the sum and
 // once by its bf16 or e4m3 store.
 //
-// Both kernels move bytes. 4,093 rows of 48 heads are written in 13.0 us (47 MB, 3.6
-// TB/s; 13.5 with a head a lane group instead of two): what remains is the latency of two
+// Both kernels move bytes. 4,093 rows of 48 heads are written in 13.3 us (47 MB, 3.6
+// TB/s; 0.5 more with a head a lane group instead of two): what remains is the latency of two
 // rounds of loads (rows, slot and position, then the tables and the page) in three
-// waves of CTAs. 32 x 8,191 positions read back in 131 us (5.7 TB/s). One row: 1.9 us.
+// waves of CTAs. 32 x 8,191 positions read back in 131 us (5.7 TB/s). One row: 1.8 us.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
   u[1] = live && h0 + 1 < nh ? src[8] : make_uint4(0, 0, 0, 0);
   // all that does not wait for another load, then the page, under way with the tables
   const bool rotated = live && h0 < p.NQ + kv.NKV, stored = live && h0 + 1 >= p.NQ;
-  const int pos = rotated ? p.positions[row] : 0;
+  const int pos = live ? p.positions[row] : 0;
   const int slot = stored ? p.slots[row] : -1, seq = stored ? p.seqs[row] : 0;
   const int blk = slot / kv.ps, off = slot - blk * kv.ps;
   int page = -1;
@@ -119,17 +119,13 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     page = kv.block_tables[(size_t)seq * kv.max_blocks + blk];
   const bool placed = pos >= 0 && pos < p.rope_len;
   uint2 cs[4] = {};  // cosines of dims 4 l .., 32 + 4 l .., sines of the same
-  if (rotated) {
-    if (placed) {
-      const uint2* c = reinterpret_cast<const uint2*>(p.cos_t + (size_t)pos * 64) + l;
-      const uint2* s = reinterpret_cast<const uint2*>(p.sin_t + (size_t)pos * 64) + l;
-      cs[0] = c[0];
-      cs[1] = c[8];
-      cs[2] = s[0];
-      cs[3] = s[8];
-    } else {
-      atomicExch(p.error, 1);
-    }
+  if (rotated && placed) {
+    const uint2* c = reinterpret_cast<const uint2*>(p.cos_t + (size_t)pos * 64) + l;
+    const uint2* s = reinterpret_cast<const uint2*>(p.sin_t + (size_t)pos * 64) + l;
+    cs[0] = c[0];
+    cs[1] = c[8];
+    cs[2] = s[0];
+    cs[3] = s[8];
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -157,7 +153,11 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
 #pragma unroll
       for (int o = 4; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     }
-    if (!live || hd >= nh || (turn && !placed)) continue;
+    if (!live || hd >= nh) continue;
+    if (!placed) {  // a row of no position is stored nowhere, not even its V
+      atomicExch(p.error, 1);
+      continue;
+    }
     auto pack = [](const float(&x)[4]) {
       __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
       return make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));

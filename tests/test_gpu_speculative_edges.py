@@ -218,6 +218,30 @@ def test_rows_of_scale_byte_0_read_back():
     assert k[0, :, 7].isnan().all() and host[:, 7].isnan().all()
 
 
+# ------------------------------------------------------------------ refusals
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("nq,nkv", [(1, 1), (4, 2), (8, 8)])
+@pytest.mark.parametrize("pos", [-1, 4, 1 << 30])
+def test_row_of_a_bad_position_is_not_stored(fmt, nq, nkv, pos):
+    """Neither K nor V: the place keeps the row that it has."""
+    k, v, ks, vs, _, _ = base._pool(2, nkv, 8, fmt, base._gen(3))
+    pools = [t if t.dtype == torch.uint8 else t.view(torch.uint8) for t in (k, v, ks, vs) if t is not None]
+    was = [t.clone() for t in pools]
+    layer = sp.KVLayer(k, v, torch.tensor([[1, 0]], dtype=torch.int32, device=DEV), ks, vs)
+    cos = torch.ones(4, 64, device=DEV).bfloat16()
+    qkv = torch.randn(2, (nq + 2 * nkv) * 64, generator=base._gen(4), device=DEV).bfloat16()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    q, err = torch.zeros(2, nq, 64, dtype=torch.bfloat16, device=DEV), base._err()
+    sp.kv_write(layer, qkv, cos, cos, i32(0, 0), i32(3, 9), i32(pos, 2), q, error=err)
+    assert int(err) == 1
+    for t, w in zip(pools, was):
+        assert torch.equal(t[1], w[1])      # the bad row's page
+        assert not torch.equal(t[0], w[0]) or t.dim() == 3  # the other row is there (a scale may stay the same)
+    err = base._err()
+    sp.kv_write(layer, qkv, cos, cos, i32(0, 0), i32(3, 9), i32(1, 2), q, error=err)
+    assert int(err) == 0
+
+
 # ------------------------------------------------------------------ log probabilities
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab", [(1, 128256), (2, 20000), (300, 4099), (700, 9000), (3, 700)])
