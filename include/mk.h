@@ -425,7 +425,8 @@ int mk_schedule_gap(const MkConfig* cfg, int32_t batch, int32_t grid, int32_t* g
  * One layer of a paged cache. MK_KV_BF16: k_pages / v_pages as in MkKVCache,
  * scales NULL. MK_KV_E4M3: pages hold e4m3 codes and k_scales / v_scales one
  * E8M0 byte per row: dim d of a row is code_d * 2^(byte - 127), byte 255 a row
- * of NaN (the NaN codes 0x7F and 0xFF are not used). page_size a multiple of 8; pools 16-byte aligned. */
+ * of NaN (the NaN codes 0x7F and 0xFF are not used). page_size a multiple of 8;
+ * pages 16-byte, scales 4-byte aligned. */
 #define MK_KV_BF16 0
 #define MK_KV_E4M3 1
 typedef struct MkKVLayer {

@@ -27,8 +27,11 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
       (long long)kv->page_size * kv->max_blocks > 0x7fffffffLL)
     return fail(MK_EINVAL, "cache geometry (page_size %d, num_pages %d, num_kv_heads %d, max_blocks %d)",
                 kv->page_size, kv->num_pages, kv->num_kv_heads, kv->max_blocks);
-  if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages) || !aligned16(kv->k_scales) || !aligned16(kv->v_scales))
+  if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages))
     return fail(MK_EINVAL, "the page pools must be 16-byte aligned");
+  // four scale bytes are copied at a time; a layer's begin at a multiple of its pages, heads and page size
+  if (kv->format == MK_KV_E4M3 && ((reinterpret_cast<uintptr_t>(kv->k_scales) | reinterpret_cast<uintptr_t>(kv->v_scales)) & 3))
+    return fail(MK_EINVAL, "k_scales and v_scales must be 4-byte aligned");
   if (batch < 1 || batch > 65535) return fail(MK_EINVAL, "batch %d outside [1, 65535]", batch);
   out->k = static_cast<uint8_t*>(kv->k_pages);
   out->v = static_cast<uint8_t*>(kv->v_pages);

@@ -242,6 +242,31 @@ def test_row_of_a_bad_position_is_not_stored(fmt, nq, nkv, pos):
     assert int(err) == 0
 
 
+# ------------------------------------------------------------------ caches and calls that are right
+def test_cache_whose_scales_start_on_8_bytes():
+    """One K/V head, pages of 8 and an odd number of them: the second layer's scales lie on 8 bytes, not 16."""
+    g = base._gen(2)
+    pages, ps, nq, n, T = 5, 8, 4, 21, 3
+    k, v = (torch.randn(2, pages, 1, ps, 64, generator=g, device=DEV).to(torch.float8_e4m3fn) for _ in range(2))
+    ks, vs = (torch.randint(120, 130, (2, pages, 1, ps), generator=g, device=DEV).to(torch.uint8) for _ in range(2))
+    table = torch.tensor([[3, 0, 4, 1]], dtype=torch.int32, device=DEV)
+    qkv = torch.randn(T, (nq + 2) * 64, generator=g, device=DEV).bfloat16()
+    ang = torch.rand(64, 32, generator=g, device=DEV)
+    cos, sin = (torch.cat([f(ang), f(ang)], 1).bfloat16() for f in (torch.cos, torch.sin))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    got = []
+    assert ks[1].data_ptr() % 16 == 8
+    for x in ((k[1], v[1], ks[1], vs[1]), tuple(t[1].clone() for t in (k, v, ks, vs))):
+        layer, err = sp.KVLayer(*x[:2], table, *x[2:]), base._err()
+        q = torch.empty(T, nq, 64, dtype=torch.bfloat16, device=DEV)
+        sp.kv_write(layer, qkv, cos, sin, i32(0, 0, 0), i32(n, n + 1, n + 2), i32(n, n + 1, n + 2), q, error=err)
+        mask = i32(1, 3, 7).long()[:, None].contiguous()
+        o, lse = sp.tree_attention(q, layer, i32(0, T), mask, i32(n), T, n + T, error=err)
+        got.append((q, o, lse, *sp.kv_read(layer, i32(n + T), n + T, error=err)))
+        assert int(err) == 0
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 # ------------------------------------------------------------------ log probabilities
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab", [(1, 128256), (2, 20000), (300, 4099), (700, 9000), (3, 700)])

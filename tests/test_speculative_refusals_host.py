@@ -1,0 +1,20 @@
+"""What the speculative-decoding entry points accept and refuse at the edge, before they touch CUDA."""
+from __future__ import annotations
+
+import pytest
+
+from llama1b_megakernel_b200 import _lib
+from tests import test_speculative_host as base
+from tests.test_speculative_host import lib  # noqa: F401  (a fixture)
+
+
+@pytest.mark.parametrize("off", [4, 8, 12])
+def test_scales_on_four_bytes(lib, off):  # noqa: F811
+    """A layer's slice of a pool of scale bytes starts where it starts."""
+    layer = base._layer(k_scales=base.PTR + off, v_scales=base.PTR + 4)
+    assert base._write(lib, layer, rows=0) == _lib.MK_OK
+    assert base._read(lib, layer, max_len=0) == _lib.MK_OK
+    assert base._attend(lib, layer, rows=0) == _lib.MK_OK
+    for bad in (dict(k_scales=base.PTR + off + 2), dict(v_scales=base.PTR + off + 1)):
+        assert base._attend(lib, base._layer(**bad)) == _lib.MK_EINVAL
+        assert "aligned" in lib.mk_last_error().decode()
