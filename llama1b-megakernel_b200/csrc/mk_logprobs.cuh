@@ -198,8 +198,10 @@ __device__ __forceinline__ void lp_finish(const LogprobsParams& p, const LpShare
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.ld;
   const float nan = __uint_as_float(0x7FFFFFFFu);
   const bool none = m == -INFINITY && s == 0.f;    // nothing but -inf (a NaN makes s one)
-  const float lse = none ? 0.f : m + logf(s);
-  if (threadIdx.x == 0) p.entropy[row] = none ? 0.f : logf(s) - w / s;
+  // x - m before log s is subtracted: rounded together, m and log s would lose as many of log s's
+  // bits as m is larger (all of them at the type's lowest value)
+  const float top = none ? 0.f : m, ls = none ? 0.f : logf(s);
+  if (threadIdx.x == 0) p.entropy[row] = none ? 0.f : ls - w / s;
   for (int j = threadIdx.x; j < p.num_targets; j += kLpThreads) {
     const int t = p.targets[(int64_t)row * p.num_targets + j];
     float v = 0.f;
@@ -207,14 +209,14 @@ __device__ __forceinline__ void lp_finish(const LogprobsParams& p, const LpShare
       atomicExch(p.error, 1);
       v = nan;
     } else if (t >= 0) {
-      v = lp_load(x, t) - lse;
+      v = (lp_load(x, t) - top) - ls;
     }
     p.logprobs[(int64_t)row * p.num_targets + j] = v;
   }
   if (threadIdx.x < p.top) {
     const unsigned long long k = sh.list[threadIdx.x];  // 0 only beside a NaN
     p.top_ids[(int64_t)row * p.top + threadIdx.x] = k ? lp_id(k) : (int)threadIdx.x;
-    p.top_logprobs[(int64_t)row * p.top + threadIdx.x] = lp_value(k) - lse;
+    p.top_logprobs[(int64_t)row * p.top + threadIdx.x] = (lp_value(k) - top) - ls;
   }
 }
 

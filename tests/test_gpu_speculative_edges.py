@@ -293,3 +293,19 @@ def test_logprobs_of_tokens_at_the_lowest_value(dtype, rows, vocab, where):
     xd = x[:, ~off].double()
     mean = ((xd - xd.amax(-1, keepdim=True)) * torch.softmax(xd, -1)).sum(-1).abs()
     assert ((ent.double() - rent).abs() <= (2.0 ** -14 + 2.0 ** -22 * size) * (1 + mean)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 128256), (300, 4099)])
+@pytest.mark.parametrize("level", ["lowest", 0.0, 96.0, -30000.0])
+def test_logprobs_of_equal_logits_at_any_level(dtype, rows, vocab, level):
+    """log p_t = (x_t - m) - log s: what the logits are has no part in it, so of equal ones it is
+    -log V to a few units of log's last place (|log V| < 16, an ulp is 2^-20 of 1)."""
+    level = torch.finfo(dtype).min if level == "lowest" else level
+    x = torch.full((rows, vocab), level, dtype=dtype, device=DEV)
+    t = torch.full((rows, 1), vocab // 2, dtype=torch.int32, device=DEV)
+    lp, ent, ids, tlp = sp.token_logprobs(x, t, 3)
+    want = math.log(vocab)
+    for got, ref in ((lp, -want), (tlp, -want), (ent, want)):
+        assert ((got.double() - ref).abs() <= 2.0 ** -19).all()
+    assert (ids == torch.arange(3, device=DEV)).all()
