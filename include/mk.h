@@ -420,7 +420,8 @@ int mk_schedule_gap(const MkConfig* cfg, int32_t batch, int32_t grid, int32_t* g
  * sequence in one pass, over a cache of half the bytes where wanted, and score
  * them. All are asynchronous on `stream`; device-side failures set *error
  * (device, zeroed by the caller) to the code named at each entry point, and
- * nothing outside the caller's buffers is read or written.
+ * nothing outside the caller's buffers is read or written. A call of no rows
+ * (max_len 0 for mk_kv_read) does nothing, and its arrays may be NULL.
  *
  * One layer of a paged cache. MK_KV_BF16: k_pages / v_pages as in MkKVCache,
  * scales NULL. MK_KV_E4M3: pages hold e4m3 codes and k_scales / v_scales one

@@ -264,13 +264,13 @@ int mk_kv_write(const MkKVLayer* kv, int32_t batch, const void* qkv, const void*
                 int32_t* error, void* stream) {
   mk::KVWriteParams p{};
   if (int rc = check_layer(kv, batch, &p.kv)) return rc;
-  if (!qkv || !rope_cos || !rope_sin || !seqs || !slots || !positions || !q_out || !error)
-    return fail(MK_EINVAL, "NULL argument");
   if (rows < 0 || num_q_heads < 1 || num_q_heads > 65535 || rope_len < 1)
     return fail(MK_EINVAL, "rows %d, num_q_heads %d, rope_len %d", rows, num_q_heads, rope_len);
+  if (rows == 0) return MK_OK;  // arrays of nothing may be NULL
+  if (!qkv || !rope_cos || !rope_sin || !seqs || !slots || !positions || !q_out || !error)
+    return fail(MK_EINVAL, "NULL argument");
   if (!aligned16(qkv) || !aligned16(rope_cos) || !aligned16(rope_sin) || !aligned16(q_out))
     return fail(MK_EINVAL, "qkv, the RoPE tables and q_out must be 16-byte aligned");
-  if (rows == 0) return MK_OK;
   p.qkv = static_cast<const uint8_t*>(qkv);
   p.cos_t = static_cast<const __nv_bfloat16*>(rope_cos);
   p.sin_t = static_cast<const __nv_bfloat16*>(rope_sin);
@@ -294,11 +294,11 @@ int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32
                void* k_out, void* v_out, int32_t* error, void* stream) {
   mk::KVReadParams p{};
   if (int rc = check_layer(kv, batch, &p.kv)) return rc;
-  if (!lengths || !k_out || !v_out || !error) return fail(MK_EINVAL, "NULL argument");
   if (max_len < 0 || max_len > (long long)kv->page_size * kv->max_blocks)
     return fail(MK_EINVAL, "max_len %d outside [0, page_size * max_blocks]", max_len);
-  if (!aligned16(k_out) || !aligned16(v_out)) return fail(MK_EINVAL, "k_out and v_out must be 16-byte aligned");
   if (max_len == 0) return MK_OK;
+  if (!lengths || !k_out || !v_out || !error) return fail(MK_EINVAL, "NULL argument");
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(MK_EINVAL, "k_out and v_out must be 16-byte aligned");
   p.lengths = lengths;
   p.max_len = max_len;
   p.k_out = static_cast<__nv_bfloat16*>(k_out);
@@ -325,7 +325,6 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   mk::TreeTmaParams tp{};
   mk::TreeParams& p = tp.p;
   if (int rc = check_layer(kv, batch, &p.kv)) return rc;
-  if (!q || !cu_nodes || !mask || !prefix_lens || !out || !error) return fail(MK_EINVAL, "NULL argument");
   const int nkv = kv->num_kv_heads;
   const int group = num_q_heads / nkv;
   if (num_q_heads < 1 || num_q_heads % nkv || (group != 1 && group != 2 && group != 4 && group != 8))
@@ -336,6 +335,8 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
     return fail(MK_EINVAL, "rows %d, max_len %d (page_size %d, max_blocks %d)", rows, max_len, kv->page_size,
                 kv->max_blocks);
   if (!(scale > 0.f) || !(scale < 3.0e38f)) return fail(MK_EINVAL, "scale %g must be positive and finite", (double)scale);
+  if (rows == 0) return MK_OK;
+  if (!q || !cu_nodes || !mask || !prefix_lens || !out || !error) return fail(MK_EINVAL, "NULL argument");
   if (!aligned16(q) || !aligned16(out)) return fail(MK_EINVAL, "q and out must be 16-byte aligned");
   const long long pool_rows = (long long)kv->num_pages * nkv * kv->page_size;
   if (pool_rows > 0x7fffffffLL) return fail(MK_EINVAL, "KV pool of %lld rows", pool_rows);
@@ -344,7 +345,6 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(MK_EINVAL, "workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   if (need > 0 && !aligned16(workspace)) return fail(MK_EINVAL, "workspace must be 16-byte aligned");
-  if (rows == 0) return MK_OK;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.cu_nodes = cu_nodes;
   p.mask = reinterpret_cast<const unsigned long long*>(mask);
@@ -391,18 +391,18 @@ int mk_token_logprobs(const void* logits, int32_t dtype, int32_t rows, int32_t v
                       const int32_t* targets, int32_t num_targets, int32_t top, void* workspace,
                       int64_t workspace_bytes, float* logprobs, float* entropy, int32_t* top_ids,
                       float* top_logprobs, int32_t* error, void* stream) {
-  if (!logits || !entropy || !error) return fail(MK_EINVAL, "NULL argument");
   if (dtype != MK_F32 && dtype != MK_BF16) return fail(MK_EINVAL, "logits type %d", dtype);
   if (rows < 0 || vocab < 1 || vocab > kLpMaxVocab || ld < vocab) return fail(MK_EINVAL, "rows %d, vocab %d, ld %lld", rows, vocab, (long long)ld);
-  if (num_targets < 0 || (num_targets && (!targets || !logprobs)))
-    return fail(MK_EINVAL, "num_targets %d needs targets and logprobs", num_targets);
-  if (top < 0 || top > mk::kLogprobsMaxTop || top > vocab || (top && (!top_ids || !top_logprobs)))
-    return fail(MK_EINVAL, "top %d must be in [0, min(%d, vocab)] and needs top_ids and top_logprobs", top,
-                mk::kLogprobsMaxTop);
+  if (num_targets < 0) return fail(MK_EINVAL, "num_targets %d", num_targets);
+  if (top < 0 || top > mk::kLogprobsMaxTop || top > vocab)
+    return fail(MK_EINVAL, "top %d must be in [0, min(%d, vocab)]", top, mk::kLogprobsMaxTop);
+  if (rows == 0) return MK_OK;
+  if (!logits || !entropy || !error) return fail(MK_EINVAL, "NULL argument");
+  if (num_targets && (!targets || !logprobs)) return fail(MK_EINVAL, "num_targets %d needs targets and logprobs", num_targets);
+  if (top && (!top_ids || !top_logprobs)) return fail(MK_EINVAL, "top %d needs top_ids and top_logprobs", top);
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == MK_F32 ? 4 : 2)) return fail(MK_EINVAL, "logits are not aligned to their type");
   (void)workspace;
   (void)workspace_bytes;
-  if (rows == 0) return MK_OK;
   mk::LogprobsParams p{};
   p.logits = logits;
   p.ld = ld;

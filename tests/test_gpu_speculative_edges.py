@@ -267,6 +267,26 @@ def test_cache_whose_scales_start_on_8_bytes():
     assert all(torch.equal(a, b) for a, b in zip(*got))
 
 
+def test_calls_without_rows():
+    """No rows, no positions, no tokens: empty results, not a refusal."""
+    s = base._setup([20, 3], [2, 1], 8, 2, 16, "e4m3", "chain", seed=1)
+    layer, err = sp.KVLayer(s["k"], s["v"], s["tables"], s["ks"], s["vs"]), base._err()
+    i0 = torch.zeros(0, dtype=torch.int32, device=DEV)
+    one = torch.ones(4, 64, device=DEV).bfloat16()
+    q = torch.empty(0, 8, 64, dtype=torch.bfloat16, device=DEV)
+    sp.kv_write(layer, torch.empty(0, 12 * 64, dtype=torch.bfloat16, device=DEV), one, one, i0, i0, i0, q, error=err)
+    k, v = sp.kv_read(layer, s["prefix"], 0, error=err)
+    assert k.shape == v.shape == (2, 2, 0, 64)
+    cu = torch.zeros(3, dtype=torch.int32, device=DEV)
+    out, lse = sp.tree_attention(q, layer, cu, torch.empty(0, 1, dtype=torch.int64, device=DEV), s["prefix"], 2, 22, error=err)
+    assert out.shape == (0, 8, 64) and lse.shape == (0, 8)
+    for n, top in ((0, 0), (2, 3)):
+        t = torch.empty(0, n, dtype=torch.int32, device=DEV)
+        lp, ent, ids, tlp = sp.token_logprobs(torch.empty(0, 50, device=DEV), t, top, error=err)
+        assert lp.shape == (0, n) and ent.shape == (0,) and ids.shape == tlp.shape == (0, top)
+    assert int(err) == 0
+
+
 # ------------------------------------------------------------------ log probabilities
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab", [(1, 128256), (2, 20000), (300, 4099), (700, 9000), (3, 700)])

@@ -18,3 +18,16 @@ def test_scales_on_four_bytes(lib, off):  # noqa: F811
     for bad in (dict(k_scales=base.PTR + off + 2), dict(v_scales=base.PTR + off + 1)):
         assert base._attend(lib, base._layer(**bad)) == _lib.MK_EINVAL
         assert "aligned" in lib.mk_last_error().decode()
+
+
+def test_arrays_of_nothing_may_be_null(lib):  # noqa: F811
+    """Empty tensors have no address; sizes are still looked at."""
+    layer = base._layer()
+    assert base._write(lib, layer, rows=0, qkv=None, slots=None, q_out=None) == _lib.MK_OK
+    assert base._read(lib, layer, max_len=0, k=None, v=None) == _lib.MK_OK
+    assert base._attend(lib, layer, rows=0, q=None, mask=None, out=None) == _lib.MK_OK
+    assert base._logprobs(lib, rows=0, logits=None, targets=None, lp=None, ent=None, ids=None, tlp=None) == _lib.MK_OK
+    assert base._write(lib, layer, rows=0, nq=0) == _lib.MK_EINVAL
+    assert base._read(lib, layer, max_len=-1, k=None) == _lib.MK_EINVAL
+    assert base._attend(lib, layer, rows=0, max_nodes=257) == _lib.MK_EINVAL
+    assert base._logprobs(lib, rows=0, top=33) == _lib.MK_EINVAL
