@@ -85,6 +85,10 @@ class PagedKVCache:
         for seq, n in enumerate(lengths):
             self.reserve(seq, n)
 
+    def room(self, seq: int) -> int:
+        """Positions that sequence ``seq`` has pages for, the free ones counted."""
+        return min(self.max_blocks, len(self._host_tables[seq]) + len(self._free)) * self.page_size
+
     def shuffle_free_pages(self, seed: int) -> None:
         """Hand out free pages in a seeded random order (exercises the page indirection)."""
         g = torch.Generator().manual_seed(seed)

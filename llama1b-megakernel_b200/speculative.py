@@ -530,15 +530,20 @@ class SpeculativeDecoder:
     def generate(self, prompt, max_new_tokens: int, draft=None) -> tuple[list[int], int]:
         """Greedy tokens after ``prompt`` (sequence 0, from an empty cache):
         ``draft(tokens)`` proposes a ``DraftTree`` of continuations of the tokens so
-        far (None or empty: no draft). Returns (tokens, passes)."""
+        far (None or empty: no draft). Returns (tokens, passes). What does not fit in
+        ``max_seq_len`` or the page pool is refused before the first pass."""
         if self.kv.seq_lens[0]:
             raise ValueError("sequence 0 is not empty: release it first")
         tokens = torch.as_tensor(prompt).reshape(-1).tolist()
         start = len(tokens)
+        most = start + max(max_new_tokens, 1) - 1  # the last token has no row in the cache
+        if most > self.max_seq_len:
+            raise ValueError(f"{start} + {max_new_tokens} tokens exceed max_seq_len {self.max_seq_len}")
+        self.kv.reserve(0, most)
         tokens.append(int(self.prefill([tokens])[0].argmax()))
         passes = 1
         while len(tokens) - start < max_new_tokens:
-            room = min(self.max_nodes - 1, self.max_seq_len - self.kv.seq_lens[0] - 1)
+            room = min(self.max_nodes - 1, min(self.max_seq_len, self.kv.room(0)) - self.kv.seq_lens[0] - 1)
             proposal = draft(tokens) if draft is not None else None
             if proposal is not None and len(proposal) and room > 0:
                 n = min(len(proposal), room)  # parents come first, so a cut tree is a tree

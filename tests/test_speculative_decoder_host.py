@@ -122,3 +122,30 @@ def test_refused_score_changes_nothing(monkeypatch, bad, error):
     with pytest.raises(error):
         dec.score([DraftTree.chain([1] * 9), bad])
     assert _same(was, _state(dec)) and len(dec.passes) == passes and not any(dec._pending)
+
+
+@pytest.mark.parametrize("prompt,new,pages,error", [([1] * 500, 14, None, ValueError), ([1] * 20, 46, 8, RuntimeError)])
+def test_generate_that_does_not_fit_is_refused_first(monkeypatch, prompt, new, pages, error):
+    """Not after most of its tokens, which would be lost."""
+    dec = _decoder(monkeypatch, num_pages=pages)
+    was = _state(dec)
+    with pytest.raises(error):
+        dec.generate(prompt, new)
+    assert _same(was, _state(dec)) and not dec.passes
+
+
+def test_generate_cuts_drafts_to_the_pool(monkeypatch):
+    """Tokens that fit come out although the drafts on the way would not have."""
+    from llama1b_megakernel_b200 import speculative as sp
+
+    dec = _decoder(monkeypatch, num_pages=4)
+    monkeypatch.setattr(dec, "check", lambda: None, raising=False)
+
+    def zeros(logits, targets, top, error):
+        n = logits.shape[0]
+        return torch.zeros(targets.shape), torch.zeros(n), torch.zeros(n, top, dtype=torch.int32), torch.zeros(n, top)
+    monkeypatch.setattr(sp, "token_logprobs", zeros)
+    dec._logits = lambda x: torch.zeros(x.shape[0], TINY.vocab)
+    tokens, passes = dec.generate([5] * 20, 13, lambda tokens: DraftTree.chain([0, 7, 7, 7, 7, 7]))
+    assert tokens == [0] * 13 and dec.kv.seq_lens[0] <= 32
+    assert max(len(p[0]) for p in dec.passes[1:]) == 7  # whole drafts while there is room
