@@ -476,7 +476,7 @@ int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32
  * places and the pages behind the last node hold has no effect on a row. A
  * row that attends a node whose K or V is not finite is not finite.
  * num_q_heads is 1, 2, 4 or 8 times num_kv_heads; max_nodes (1..256) and max_len
- * bound every sequence's nodes and prefix + nodes. One node per sequence with
+ * (1..2^30) bound every sequence's nodes and prefix + nodes. One node per sequence with
  * its own bit is a plain decode step. q, out and the workspace (NULL where its
  * size is 0) are 16-byte aligned. *error = 1: lengths or node ranges beyond
  * the bounds (that sequence is not computed) or a page id out of range (its

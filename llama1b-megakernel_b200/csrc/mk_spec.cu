@@ -72,6 +72,7 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 // that share positions drift apart (4 sequences of 256 nodes at 16,000: 182 us whole, 205
 // in two).
 constexpr int kTreeFewRows = 16;
+constexpr int kTreeMaxLen = 1 << 30;  // positions are ints that a range's and a block's length are added to
 constexpr int kTreeSort = 128;
 using mk::kTreeCluster;
 struct TreePlan {
@@ -312,8 +313,11 @@ int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32
 
 int64_t mk_tree_attention_workspace(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                     int32_t max_nodes, int32_t max_len) {
-  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_nodes < 1 || max_len < 1) return 0;
+  if (batch < 1 || batch > 65535 || num_kv_heads < 1 || num_q_heads < num_kv_heads || max_nodes < 1 ||
+      max_nodes > mk::kTreeMaxNodes || max_len < 1 || max_len > kTreeMaxLen)
+    return 0;
   const int group = num_q_heads / num_kv_heads;
+  if (group > 8) return 0;
   return tree_workspace(tree_plan(batch, num_kv_heads, max_nodes * group, max_len), batch, num_kv_heads, max_nodes * group);
 }
 
@@ -331,9 +335,9 @@ int mk_tree_attention(const void* q, const MkKVLayer* kv, const int32_t* cu_node
     return fail(MK_EINVAL, "num_q_heads %d must be 1, 2, 4 or 8 times num_kv_heads %d", num_q_heads, nkv);
   if (max_nodes < 1 || max_nodes > mk::kTreeMaxNodes)
     return fail(MK_EINVAL, "max_nodes %d outside [1, %d]", max_nodes, mk::kTreeMaxNodes);
-  if (rows < 0 || max_len < 1 || max_len > (long long)kv->page_size * kv->max_blocks)
-    return fail(MK_EINVAL, "rows %d, max_len %d (page_size %d, max_blocks %d)", rows, max_len, kv->page_size,
-                kv->max_blocks);
+  if (rows < 0 || max_len < 1 || max_len > kTreeMaxLen || max_len > (long long)kv->page_size * kv->max_blocks)
+    return fail(MK_EINVAL, "rows %d, max_len %d (at most %d; page_size %d, max_blocks %d)", rows, max_len, kTreeMaxLen,
+                kv->page_size, kv->max_blocks);
   if (!(scale > 0.f) || !(scale < 3.0e38f)) return fail(MK_EINVAL, "scale %g must be positive and finite", (double)scale);
   if (rows == 0) return MK_OK;
   if (!q || !cu_nodes || !mask || !prefix_lens || !out || !error) return fail(MK_EINVAL, "NULL argument");

@@ -31,3 +31,20 @@ def test_arrays_of_nothing_may_be_null(lib):  # noqa: F811
     assert base._read(lib, layer, max_len=-1, k=None) == _lib.MK_EINVAL
     assert base._attend(lib, layer, rows=0, max_nodes=257) == _lib.MK_EINVAL
     assert base._logprobs(lib, rows=0, top=33) == _lib.MK_EINVAL
+
+
+@pytest.mark.parametrize("max_len", [(1 << 30) + 1, (1 << 31) - 128, (1 << 31) - 8])
+def test_lengths_beyond_the_kernels_indexes(lib, max_len):  # noqa: F811
+    """Positions are ints that a range's or block's end is added to: 2^30 is the limit, and
+    what is above it is refused by name."""
+    layer = base._layer(page_size=8, max_blocks=(1 << 28) - 1)
+    for rows in (0, 6):
+        assert base._attend(lib, layer, max_len=max_len, rows=rows) == _lib.MK_EINVAL
+        assert "max_len" in lib.mk_last_error().decode()
+    assert base._attend(lib, layer, max_len=1 << 30, rows=0) == _lib.MK_OK
+
+
+@pytest.mark.parametrize("args", [(1, 8, 2, 257, 17000), (1, 8, 2, 1 << 30, 17000), (1, 8, 2, 3, (1 << 31) - 8),
+                                  (70000, 8, 2, 3, 17000), (1, 1 << 30, 1, 2, 17000)])
+def test_workspace_of_what_is_refused_is_nothing(lib, args):  # noqa: F811
+    assert lib.mk_tree_attention_workspace(*args) == 0
