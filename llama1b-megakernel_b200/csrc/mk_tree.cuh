@@ -166,6 +166,15 @@ __device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatil
   return tree_try(bar, parity) || tree_wait_slow(bar, parity, abort_word, error);
 }
 
+// Until a phase that nothing holds up any more has ended: copies and MMAs under way finish
+// before the CTA gives up its memory, also where its other waits have run out. 4 s and a
+// thousand looks, as above.
+__device__ __noinline__ void tree_land(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = global_ns();
+  for (uint32_t looks = 0; !tree_try(bar, parity); ++looks)
+    if (looks >= 1000 && (int64_t)(global_ns() - t0) > 4000000000ll) return;
+}
+
 // The pages of a range as a producer warp walks through it: 32 entries of the block
 // table in a register of each lane and the next 32 on their way, so that no copy
 // waits for a load, and no division a position (with both, an iteration of the
@@ -678,12 +687,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
       ++issued;
     }
     // every box issued lands before the CTA may exit (bounded)
-    for (int j = max(0, issued - L::kStages); j < issued; ++j) {
-      const uint64_t t0 = global_ns();
-      while (!mbar_try_wait(reinterpret_cast<uint64_t*>(smem + L::kBars) + j % L::kStages, (j / L::kStages) & 1) &&
-             global_ns() - t0 < 4000000000ull) {
-      }
-    }
+    for (int j = max(0, issued - L::kStages); j < issued; ++j) tree_land(full(j % L::kStages), (j / L::kStages) & 1);
   } else if (warp == 13) {
     // ---- issuer, the whole warp converged
     constexpr uint32_t id_s = tree_idesc(kTreeHalf, false), id_o = tree_idesc(64, true);
@@ -719,7 +723,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_attn_kernel(const __grid
     }
     // what was issued finishes before the results are read and TMEM is released
     tree_commit(b_o);
-    wait_all(b_o, 0);
+    if (!wait_all(b_o, 0)) tree_land(b_o, 0);
   } else if (warp >= 8) {
     // ---- block warps, one thread per position. They pass every block, also those that
     // need nothing: a wait for a phase means something only to who has waited for the last

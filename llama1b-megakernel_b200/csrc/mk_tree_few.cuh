@@ -201,12 +201,7 @@ __global__ void __launch_bounds__((kFewWarps + 1) * 32, kFewCtas)
       ++issued;
     }
     // every box issued lands before the CTA may exit (bounded)
-    for (int j = max(0, issued - kFewStages); j < issued; ++j) {
-      const uint64_t t0 = global_ns();
-      while (!mbar_try_wait(reinterpret_cast<uint64_t*>(smem + L::kBars) + j % kFewStages, (j / kFewStages) & 1) &&
-             global_ns() - t0 < 4000000000ull) {
-      }
-    }
+    for (int j = max(0, issued - kFewStages); j < issued; ++j) tree_land(full(j % kFewStages), (j / kFewStages) & 1);
   } else {
     // ---- consumers. Fragment rows of thread (g8, t4): g8 and g8 + 8 of each 16.
     const int g8 = lane >> 2, t4 = lane & 3;
