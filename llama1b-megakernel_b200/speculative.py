@@ -20,9 +20,11 @@ every node is scored for its children, and accepted nodes stay in the cache.
 
 All run asynchronously on the current stream of their tensors' device, allocate
 outputs and workspaces that are not passed in from PyTorch's allocator, and raise
-``ValueError`` on arguments that do not fit. What only the device can see (a page
-id, a length or a token out of range) sets the caller's ``error`` word, an int32
-tensor of one zero that the caller reads when it synchronises.
+``ValueError`` on tensors that do not fit and ``MkError`` on sizes that the library
+refuses. What only the device can see (a page id, a length or a token out of range)
+sets the caller's ``error`` word, an int32 tensor of one zero that the caller reads
+when it synchronises; a call without one has nobody to tell, and such a row is wrong
+without a word.
 """
 from __future__ import annotations
 
@@ -144,7 +146,7 @@ def kv_read(layer: KVLayer, lengths, max_len: int, k_out=None, v_out=None, error
     """Positions [0, lengths[b]) of every sequence as bf16 [batch, nkv, max_len, 64]
     (K, V), zeros behind them."""
     index, dev = layer.index, layer.device
-    n = lengths.shape[0]
+    n, = lengths.shape
     if n > layer.batch:
         raise ValueError(f"{n} lengths for a table of {layer.batch} sequences")
     shape = (n, layer.num_kv_heads, max_len, 64)
@@ -177,7 +179,7 @@ def tree_attention(q, layer: KVLayer, cu_nodes, mask, prefix_lens, max_nodes: in
     rows, nq, _ = shape = q.shape
     if shape[2] != 64:
         raise ValueError(f"q must be [rows, query heads, 64], got {tuple(shape)}")
-    n = prefix_lens.shape[0]
+    n, = prefix_lens.shape
     if n > layer.batch:
         raise ValueError(f"{n} sequences for a table of {layer.batch}")
     at = _check(q, _BF16, "q", index)
@@ -231,7 +233,7 @@ def token_logprobs(logits, targets=None, top: int = 0, logprobs=None, entropy=No
         dtype = _lib.MK_BF16
     else:
         raise ValueError(f"logits must be fp32 or bf16, got {logits.dtype}")
-    n = 0 if targets is None else targets.shape[1]
+    _, n = (rows, 0) if targets is None else targets.shape
     if logprobs is None:
         logprobs = logits.new_empty(rows, n, dtype=_F32)
         lp = logprobs.data_ptr()

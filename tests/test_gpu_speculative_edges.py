@@ -177,6 +177,28 @@ def test_huge_values_in_masked_places(fmt, nodes, prefix, small):
     base._check(finite, out, lse, skip={(0, leaf)})
 
 
+# ------------------------------------------------------------------ exponentials
+@pytest.mark.parametrize("shift", [0, 1])
+def test_exponentials_of_either_pipe(shift):
+    """Of 32 committed positions the large tiles take columns 6, 7, 16, 17, 26 and 27 with a
+    polynomial. Where only those (or only others) count, lse is a sum of such exponentials: right to
+    the polynomial's 2^-22, the score's rounding (2^-24 of up to 2^4.5), the sum's and the
+    logarithm's, 2^-18 in all."""
+    prefix, nodes = 2048, 20
+    n = prefix + nodes
+    j = torch.arange(n, device=DEV)
+    counts = (((j % 32)[:, None] - shift * 3 == torch.tensor([6, 7, 16, 17, 26, 27], device=DEV)).any(1)) & (j < prefix)
+    x = torch.randint(-4096, 1, (n,), generator=base._gen(5), device=DEV).double() / 256  # -16 .. 0
+    x = x.bfloat16().double()
+    score = torch.where(counts, x, -60.0)
+    s = _scored(prefix, nodes, score, fmt="bf16")
+    out, lse = _attend_many(s)
+    _compare(s, out, lse)
+    seen = score.clone()
+    want = torch.logsumexp(seen, 0)
+    assert ((lse.double() - want).abs() <= 2.0 ** -18).all()
+
+
 # ------------------------------------------------------------------ scale bytes that other code may write
 @pytest.mark.parametrize("nodes", [1, 2, 20])
 @pytest.mark.parametrize("x,byte", [("k", 0), ("v", 0), ("v", 1), ("v", 254)])
@@ -329,3 +351,19 @@ def test_logprobs_of_equal_logits_at_any_level(dtype, rows, vocab, level):
     for got, ref in ((lp, -want), (tlp, -want), (ent, want)):
         assert ((got.double() - ref).abs() <= 2.0 ** -19).all()
     assert (ids == torch.arange(3, device=DEV)).all()
+
+
+def test_arguments_of_other_shapes():
+    """Vectors where matrices belong and the other way round are a ValueError, as other shapes are."""
+    s = base._setup([20], [3], 8, 2, 16, "e4m3", "chain", seed=1)
+    layer = sp.KVLayer(s["k"], s["v"], s["tables"], s["ks"], s["vs"])
+    i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=DEV)  # noqa: E731
+    x = torch.zeros(2, 50, device=DEV)
+    for bad in (lambda: sp.token_logprobs(x, i32(2)), lambda: sp.token_logprobs(x, i32(2, 1, 1)),
+                lambda: sp.kv_read(layer, torch.tensor(3, dtype=torch.int32, device=DEV), 4),
+                lambda: sp.kv_read(layer, i32(1, 1), 4),
+                lambda: sp.tree_attention(s["q"], layer, s["cu"], s["mask"], s["prefix"][0], 3, 23),
+                lambda: sp.tree_attention(s["q"], layer, s["cu"], s["mask"], s["prefix"][:, None], 3, 23),
+                lambda: sp.tree_attention(s["q"][0], layer, s["cu"], s["mask"], s["prefix"], 3, 23)):
+        with pytest.raises(ValueError):
+            bad()
