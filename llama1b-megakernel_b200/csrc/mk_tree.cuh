@@ -325,13 +325,13 @@ __device__ __forceinline__ float tree_max3(float a, float b, float c) {  // NaN 
 // 2^x of two numbers on the FMA pipe, for some of a row's: the special function unit
 // (16 exponentials a cycle) is what bounds the softmax of bf16 rows. x = n + f, |f| <= 1/2, and a polynomial for 2^f (least largest relative error, fitted by
 // reweighted least squares: 2^-22.1 in fp32, as good as ex2.approx); n goes into the
-// exponent by a multiplication, which keeps a NaN. Below 2^-126 the result is 2^-126, so
-// it is not for masked scores. 4 sequences of 256 nodes at 16,000: none 199 us, 2 of 16
+// exponent by a multiplication, which keeps a NaN. Below 2^-126.5 the result is 0 (an
+// exponent field of 0 for n = -127), as a value of 3e38 may go with it. 4 sequences of 256 nodes at 16,000: none 199 us, 2 of 16
 // 184, 3 of 16 181, 4 of 16 183, 5 of 16 195; with 8-bit rows, whose conversion takes the issue slots,
 // 32 x 64 nodes: none 223 us, 2 of 16 235.
 __device__ __forceinline__ float2 tree_exp2(float2 x) {
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
   auto both = [](float c) { return make_float2(c, c); };
   const float2 t = add2(x, both(12583039.f));  // 1.5 * 2^23 + 127: n, biased, in the low bits
   const float2 f = fma2(add2(t, both(-12583039.f)), both(-1.f), x);

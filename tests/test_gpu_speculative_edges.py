@@ -177,6 +177,23 @@ def test_huge_values_in_masked_places(fmt, nodes, prefix, small):
     base._check(finite, out, lse, skip={(0, leaf)})
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("nodes", [1, 2, 20])
+def test_huge_values_of_no_probability(fmt, nodes):
+    """Committed rows of 3e38 with a probability of e^-208 of the others' add nothing (6e-53)."""
+    prefix = 700
+    n = prefix + nodes
+    j = torch.arange(n, device=DEV)
+    huge = (j % 32 == 6) & (j < 200)
+    s = _scored(prefix, nodes, torch.where(huge, -208.0, 0.0).double(), fmt=fmt, seed=nodes)
+    v = torch.randn(n, 1, 64, generator=base._gen(nodes), device=DEV).double()
+    v[huge] = torch.where(v[huge] < 0, -3.0e38, 3.0e38).double()
+    _put(s, "v", 0, j, v)
+    out, lse, err = base._attend(s)
+    assert int(err) == 0
+    _compare(s, out, lse)
+
+
 # ------------------------------------------------------------------ exponentials
 @pytest.mark.parametrize("shift", [0, 1])
 def test_exponentials_of_either_pipe(shift):
