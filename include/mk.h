@@ -474,7 +474,8 @@ int mk_kv_read(const MkKVLayer* kv, const int32_t* lengths, int32_t batch, int32
  * q K^T) V, scale > 0; lse [rows][num_q_heads] fp32 (may be NULL) the log of the
  * normaliser. A node that attends nothing gets out 0, lse -inf; what masked
  * places and the pages behind the last node hold has no effect on a row. A
- * row that attends a node whose K or V is not finite is not finite.
+ * row that attends a node whose V is not finite, or whose score is NaN or
+ * +inf, is not finite.
  * num_q_heads is 1, 2, 4 or 8 times num_kv_heads; max_nodes (1..256) and max_len
  * (1..2^30) bound every sequence's nodes and prefix + nodes. One node per sequence with
  * its own bit is a plain decode step. q, out and the workspace (NULL where its

@@ -26,10 +26,10 @@
 // slices of a row are a cluster; its first CTA joins them, ranking out of their lists
 // what reaches the largest of the lists' last keys.
 //
-// Many fp32 rows are bound by memory: 2,047 of 128,256 in 185 us, 5.7 TB/s. Of bf16, with
-// half the bytes for as many exponentials and comparisons, by instruction latency: 200
-// rows with five alternatives in 25.3 us (2.0 TB/s, 15 instructions a logit), 17.4 without. One row is latency:
-// 9.9 us with twenty.
+// Many fp32 rows are bound by memory: 2,047 of 128,256 in 184 to 193 us (two GPUs), 5.4 to
+// 5.7 TB/s. Of bf16, with half the bytes for as many exponentials and comparisons, by
+// instruction latency: 200 rows with five alternatives in 24.9 us (2.0 TB/s, 15
+// instructions a logit), 17.4 without. One row is latency: 9.9 to 10.5 us with twenty.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -49,7 +49,7 @@ int check_layer(const MkKVLayer* kv, int32_t batch, mk::KVLayer* out) {
 // Which kernel a call takes and how the positions of a sequence are split over its
 // CTAs. Up to kTreeFewRows rows (nodes x query heads of a K/V head) go to the
 // mma.sync kernel, in one tile of 8 or 16; more to the tcgen05 kernel in tiles of 128.
-// (16 rows at 32 x 4096: 44.8 us against 45.0 of bf16, 39 against 56 of 8-bit rows; 20
+// (16 rows at 32 x 4096: 44.8 us against 45.0 of bf16, 40 against 56 of 8-bit rows; 20
 // to 32 rows in a small tile of 32: 64 to 66 against 45, 57 to 59 against 56.)
 //
 // The cut with the least estimated time is taken, in tenths of a microsecond, fitted to

@@ -42,8 +42,8 @@
 //
 // What bounds it: a lone CTA takes 5.1 us and 1.1 us a block, the latency of the chain S,
 // softmax, P V; two on an SM 1.8 us a block each, 16,384 exponentials at 16 a cycle being
-// 0.55 us of it apiece. 4 sequences of 256 nodes behind 11,000 to 16,000 positions: 181 us,
-// 660 TFLOP/s; 32 of 64 nodes over 5,200 to 8,200 8-bit positions: 205 us, 543 TFLOP/s, bound by
+// 0.55 us of it apiece. 4 sequences of 256 nodes behind 11,000 to 16,000 positions: 181 to
+// 197 us (two GPUs), 610 to 660 TFLOP/s; 32 of 64 nodes over 5,200 to 8,200 8-bit positions: 205 us, 543 TFLOP/s, bound by
 // instructions (a block warp issues 425 for a block's conversion beside the softmax's
 // 271 a half block).
 #pragma once

@@ -26,7 +26,7 @@
 //    values of little size, or one of great size came by that it does not look at) the 32
 //    positions are done again with P and V as bf16 (tree_decode's way), which rounds the
 //    smallest by 2^-8 as well. (64 sequences of 2,600 to 4,100 positions: 54.9 us without
-//    a look, 55.8 so; one of 1,025: 5.7 and 5.9.)
+//    a look, 55.8 so; one of 1,025: 5.7 and 6.0.)
 //    The positions of a block of 8 are permuted between fragment columns and rows
 //    in memory (few_place) so that both loads are free of bank conflicts under the
 //    64-byte swizzle.
@@ -34,7 +34,7 @@
 //
 // What bounds it: memory, where sequences fill the GPU (36 of 1,000 to 2,000 positions in
 // 8 bits: 19 us; 64 of 2,600 to 4,100: 56 us, 4.0 TB/s, as their 512 CTAs end one by one),
-// and the latency of a CTA's few chunks where they do not (one of 1,025 bf16: 6.0 us).
+// and the latency of a CTA's few chunks where they do not (one of 1,025 bf16: 6.2 us).
 // The split of an SM was measured (consumers x stages x CTAs; 64 of 2,600 to 4,100 in 8
 // bits, and 32 of 2,700 to 4,100 in bf16 with 16 rows): 3 x 6 x 4 55 and 45 us, 4 x 8 x 3 80
 // and 50, 4 x 4 x 4 (32 of 8-bit: 35 against 34) and 45; with 5 or 6 CTAs registers spill.
